@@ -404,6 +404,92 @@ int pjx_kv_cache_append(void* k_cache, void* v_cache, const void* k_new, const v
                         int dtype, int advance, int32_t* overflow, void* stream);
 
 /*
+ * Attention of a tree of drafted tokens over a KV cache (the verification step of speculative decoding): query (b, i) sees
+ * the kv_lengths[b] cached keys of its sequence and, among the N drafts, itself and its ancestors.
+ *
+ *   q            [B, N, Hq, D]    heads dense; sequence and token strides in elements, so that a slice of a fused projection
+ *   k_new, v_new [B, N, Hkv, D|Dv]  is taken as it is
+ *   k_cache, v_cache  [B, capacity, Hkv, D|Dv], or with block_table (int32 [B, max_pages]) page pools
+ *                [num_pages, page_size, Hkv, D|Dv], page_size a multiple of 16 (`capacity` is then max_pages * page_size).  Rows
+ *                at or past kv_lengths[b] may hold anything; a page number outside the pool reads as zeros.
+ *   parents      int32 [B, N] (parents_batch_stride in entries, 0: one tree for all): -1 hangs on the cached context,
+ *                0 <= parents[i] < i on that draft.  Any other value marks an absent draft (padding of a ragged batch):
+ *                it and what hangs on it give o = 0 and lse = +inf, and nobody sees their keys.
+ *   o            [B, N, Hq, Dv];  lse  [B, Hq, N] natural log, or NULL.
+ *   workspace    pjx_attn_decode_tree_workspace_bytes(...) bytes, 16-byte aligned.
+ *
+ * N <= 256.  The drafts' keys and values are read beside the cache, which is not written: pjx_kv_cache_accept puts the
+ * accepted path's rows there.  bf16 / fp16 with D = Dv in {64, 128}, up to 128 query heads a KV head and addresses and strides
+ * of whole 16 bytes run on the tensor cores (impl as in pjx_attn_fwd; `status` as there), everything else with head
+ * widths up to 256 in exact fp32.  No counterpart in the reference, which decodes one token at a time (probjax/nn/layers/attention.py:603-675).
+ */
+int pjx_attn_decode_tree(const void* q, int64_t q_batch_stride, int64_t q_token_stride, const void* k_new,
+                         int64_t k_new_batch_stride, int64_t k_new_token_stride, const void* v_new,
+                         int64_t v_new_batch_stride, int64_t v_new_token_stride, const void* k_cache,
+                         const void* v_cache, const int32_t* parents, int64_t parents_batch_stride,
+                         const int32_t* kv_lengths, const int32_t* block_table, void* o, float* lse, int B, int N,
+                         int Hq, int Hkv, int D, int Dv, int capacity, int page_size, int max_pages, int num_pages,
+                         int dtype, float sm_scale, int impl, void* workspace, size_t workspace_bytes,
+                         int32_t* status, void* stream);
+size_t pjx_attn_decode_tree_workspace_bytes(int B, int N, int Hq, int Hkv, int Dv, int capacity);
+
+/*
+ * The accepted path of a tree of drafts enters the cache: row path[b, i] of the drafts' keys and values goes to cache row
+ * lengths[b] + i for i < counts[b] (clamped to [0, P]), and lengths_out[b] = min(lengths[b] + counts[b], capacity);
+ * lengths_out may be lengths.  Caches and block_table as in pjx_attn_decode_tree (any page_size).  A path entry outside [0, N), a row
+ * past the capacity or a page outside the pool leaves its row as it was; `overflow` (int32 device word or NULL) is set to 1
+ * where a sequence ran past the capacity.  A token's keys, its values and the drafts' strides are whole 16-byte units.
+ */
+int pjx_kv_cache_accept(void* k_cache, void* v_cache, const void* k_new, int64_t k_new_batch_stride,
+                        int64_t k_new_token_stride, const void* v_new, int64_t v_new_batch_stride,
+                        int64_t v_new_token_stride, const int32_t* lengths, const int32_t* path, const int32_t* counts,
+                        const int32_t* block_table, int B, int N, int P, int Hkv, int D, int Dv, int capacity,
+                        int page_size, int max_pages, int num_pages, int dtype, int32_t* lengths_out, int32_t* overflow,
+                        void* stream);
+
+/*
+ * pjx_attn_decode_splitkv that also adds up the attention every key receives:
+ *   weights_out[b, hk, j] = weights_in[b, hk, j] + sum over the query tokens and the heads of the group of the probability of
+ *   key j, for j < kv_lengths[b]; behind the valid keys weights_out is weights_in.
+ * weights: float32 [B, Hkv, capacity]; weights_in NULL is zeros, weights_out may be weights_in.  The scores are kept in the
+ * workspace (pjx_attn_decode_weights_workspace_bytes, 16-byte aligned) and turned into weights once the log-sum-exp is known, so K
+ * is read once.  Calls that the streaming kernel does not take run the forward kernels and pjx_attn_key_weights.
+ */
+int pjx_attn_decode_weights(const void* q, const void* k_cache, const void* v_cache, const int32_t* kv_lengths,
+                            const float* weights_in, float* weights_out, void* o, float* lse, int B, int Lq, int Hq,
+                            int Hkv, int D, int Dv, int capacity, int dtype, float sm_scale, int split_len,
+                            void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+size_t pjx_attn_decode_weights_workspace_bytes(int B, int Lq, int Hq, int Hkv, int Dv, int capacity, int split_len);
+
+/*
+ * The same sum for queries whose attention has been taken: from q [B, Lq, Hq, D], k [B, Lkv, Hkv, D] and the call's
+ * natural-log lse [B, Hq, Lq], weights_out[b, hk, j] = weights_in[b, hk, j] + sum over the rows that see key j of
+ * exp(sm_scale q.k - lse).  Mask: the band of pjx_attn_fwd_band and kv_lengths.  Rows with lse = +inf add nothing.  A fixed order of
+ * summation: results repeat bit by bit.
+ */
+int pjx_attn_key_weights(const void* q, const void* k, const float* lse, const float* weights_in, float* weights_out,
+                         const int32_t* kv_lengths, int B, int Lq, int Lkv, int Hq, int Hkv, int D, int dtype,
+                         int band_lo, int band_hi, float sm_scale, int impl, int32_t* status, void* stream);
+
+/*
+ * Eviction from a cache by accumulated attention weight.  A sequence with more than `keep` valid keys keeps, per KV head, its
+ * `recent` last keys and the keep - recent others with the largest weights (ties: the lowest index; NaN ranks last); shorter ones keep
+ * all.  The kept rows move, in order, to the front of k_out, v_out [B, capacity_out, Hkv, D|Dv] and weights_out [B, Hkv, capacity_out].
+ *
+ *   kept         int32 [B, Hkv, keep]: the kept keys' indices in order, -1 behind them
+ *   lengths_out  int32 [B]: min(lengths[b], keep); may be lengths
+ *   k_out ...    either k_cache, v_cache, weights themselves (in place, capacity_out = capacity) or other buffers.  Rows behind the
+ *                kept ones are not written; the weights of the rows that fell free are cleared (in place: up to lengths[b],
+ *                otherwise up to capacity_out), so that new keys start at zero.
+ *   workspace    pjx_kv_cache_evict_workspace_bytes(B, Hkv) bytes, 8-byte aligned.
+ */
+int pjx_kv_cache_evict(const void* k_cache, const void* v_cache, const float* weights, const int32_t* lengths, void* k_out,
+                       void* v_out, float* weights_out, int32_t* lengths_out, int32_t* kept, int B, int Hkv, int D,
+                       int Dv, int capacity, int capacity_out, int keep, int recent, int dtype, void* workspace,
+                       size_t workspace_bytes, void* stream);
+size_t pjx_kv_cache_evict_workspace_bytes(int B, int Hkv);
+
+/*
  * y [M, N] = x [M, K] . w [N, K]^T, fp32 accumulation, y in `dtype`: a bias-free linear layer
  * with the weight stored [out, in].  16-bit inputs with K >= 64, K % 8 == 0 and 16-byte aligned
  * operands run the persistent tcgen05 kernel (the one behind pjx_mla_fwd's up-projections),
@@ -457,6 +543,24 @@ int pjx_rms_norm(const void* x, const float* scale, void* y, int64_t rows, int w
  */
 int pjx_rope_interleaved(const void* x, void* y, const float* positions, float offset, int64_t outer,
                          int T, int H, int D, int rotary_dim, float base, int dtype, void* stream);
+
+/*
+ * Rotary position embedding with several axes (video, images) and a position per token and sequence.  x [B, T, H, D] (heads
+ * dense, strides of a sequence and a token in elements) into a dense y [B, T, H, D] (may be x where that is dense).  Axis a rotates
+ * sections[a] elements (even; host array), one axis after the other from the start of the head vector; the rest is copied.
+ * Pair i of axis a turns by positions[b, t, a] * base^(-2 i / sections[a]), or with `shared` by base^(-2 p / sum(sections)) for the
+ * pair's number p over all axes.  interleaved: pairs are (x[2p], x[2p + 1]), else (x[p], x[p + sum(sections) / 2]).
+ * inverse: the opposite angle, which is the gradient.
+ *
+ *   positions  [B, T, axes] of position_type (sequence stride in entries, 0: shared by all sequences)
+ *
+ * Generalises the rotary layer behind pjx_rope_interleaved (probjax/nn/layers/encoding.py:171-211), whose positions are one axis
+ * shared by the batch.  Angles are formed in float64.
+ */
+typedef enum pjx_position_type { PJX_POS_F32 = 0, PJX_POS_I32 = 1, PJX_POS_I64 = 2 } pjx_position_type;
+int pjx_rope_axes(const void* x, int64_t x_batch_stride, int64_t x_token_stride, void* y, const void* positions,
+                  int position_type, int64_t position_batch_stride, int axes, const int32_t* sections, int B, int T,
+                  int H, int D, int shared, int interleaved, int inverse, float base, int dtype, void* stream);
 
 /*
  * Latent attention forward: q over a shared latent cache with per-head

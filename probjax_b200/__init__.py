@@ -23,7 +23,9 @@ from .attention import (  # noqa: F401
     splitkv_forward,
     use_splitkv,
 )
-from .cache import DecodeCache, decode_paged, linear, rope_interleaved  # noqa: F401
+from .cache import DecodeCache, decode_paged, linear, rope_axes, rope_interleaved  # noqa: F401
+from .drafts import accept_drafts, decode_tree  # noqa: F401
+from .eviction import decode_weights, evict, key_weights  # noqa: F401
 from .latent_layer import MultiHeadLatentAttention, per_head_linear, rms_norm  # noqa: F401
 from .dispatch import b200_attention_or_none, device_attention_defaults  # noqa: F401
 from .masks import (  # noqa: F401

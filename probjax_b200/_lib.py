@@ -17,6 +17,7 @@ LIB_PATH = Path(os.environ.get("PJX_ATTENTION_LIB", _PKG / "libpjx_attention.so"
 PJX_OK, PJX_ERR_BAD_ARG, PJX_ERR_UNSUPPORTED, PJX_ERR_WORKSPACE, PJX_ERR_DEVICE_TIMEOUT, PJX_ERR_CUDA = range(6)
 PJX_F32, PJX_BF16, PJX_F16 = 0, 1, 2
 IMPL_AUTO, IMPL_GENERIC, IMPL_SM100 = 0, 1, 2
+POS_F32, POS_I32, POS_I64 = 0, 1, 2
 
 _vp, _i, _i64, _f, _sz = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_size_t
 
@@ -82,6 +83,18 @@ SIGNATURES = {
     "pjx_rope_interleaved": (_i, [_vp, _vp, _vp, _f, _i64, _i, _i, _i, _i, _f, _i, _vp]),
     "pjx_attn_decode_paged": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i,
                                    _vp, _sz, _vp]),
+    "pjx_attn_decode_tree": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp,
+                                  _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _vp, _sz, _vp, _vp]),
+    "pjx_attn_decode_tree_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "pjx_kv_cache_accept": (_i, [_vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp,
+                                 _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp]),
+    "pjx_attn_decode_weights": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i,
+                                     _vp, _sz, _vp, _vp]),
+    "pjx_attn_decode_weights_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
+    "pjx_attn_key_weights": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _vp, _vp]),
+    "pjx_kv_cache_evict": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "pjx_kv_cache_evict_workspace_bytes": (_sz, [_i, _i]),
+    "pjx_rope_axes": (_i, [_vp, _i64, _i64, _vp, _vp, _i, _i64, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _i, _vp]),
     "pjx_kv_cache_append": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _vp]),
     "pjx_attn_combine": (_i, [_vp, _vp, _i, _i64, _i, _vp, _vp, _i, _vp]),
     "pjx_mla_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64,

@@ -76,6 +76,14 @@ def _scratch_bytes(device, tag: str, nbytes: int) -> torch.Tensor:
     return buf
 
 
+def _workspace(device, tag: str, nbytes: int) -> torch.Tensor:
+    """:func:`_scratch_bytes`, but memory of its own while a graph is captured: graphs captured on one stream may replay on
+    several at once, and a cached buffer must not outlive the graph whose pool it came from."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+    return _scratch_bytes(device, tag, nbytes)
+
+
 def _check_call(q, k, v, *, bias=None, kv_lengths=None, o=None, lse=None, d_o=None, what="attention"):
     """Shape, dtype and device agreement of the tensors of one kernel call.  The C ABI takes
     sizes from q, k and v and indexes every other buffer with them, so a mismatch here would

@@ -28,8 +28,12 @@ SOURCES = [
     "attn_decode.cu",
     "attn_decode_latent.cu",
     "attn_decode_latent_sm100.cu",
+    "attn_tree.cu",
+    "key_weights.cu",
     "kv_cache.cu",
+    "kv_compact.cu",
     "rope.cu",
+    "rope_axes.cu",
     "rmsnorm.cu",
     "gemm_sm100.cu",
 ]

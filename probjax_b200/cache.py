@@ -12,18 +12,24 @@ kernel with ``kv_lengths = positions``.
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
 
 from . import _lib
-from .attention import _DTYPES, _IMPL, _ptr, _require_gpu, _scratch_bytes, _status_word, _stream, mha
+from .attention import _DTYPES, _IMPL, _ptr, _require_gpu, _scratch_bytes, _status_word, _stream, _wants_grad, mha
+from .drafts import accept_drafts, decode_tree
+from .eviction import decode_weights, evict, key_weights
 from .masks import CausalFromBottomRightMask, KVLenMask
 
 
 class DecodeCache:
+    """Keys and values of a batch of sequences, each with its own position.  ``track_weights`` also keeps, in ``key_weights``
+    float32 ``[B, Hkv, capacity]``, the attention that every key has received so far, by which :meth:`evict` cuts the cache."""
+
     def __init__(self, batch: int, capacity: int, num_kv_heads: int, head_dim: int, v_head_dim: int | None = None,
-                 dtype=torch.bfloat16, device=None):
+                 dtype=torch.bfloat16, device=None, track_weights: bool = False):
         _require_gpu()
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         v_head_dim = head_dim if v_head_dim is None else v_head_dim
@@ -33,6 +39,7 @@ class DecodeCache:
         # [0, B): positions; [B, 2B): scratch counters of the append kernel (zero between launches)
         self._positions = torch.zeros((2 * batch,), dtype=torch.int32, device=device)
         self._overflow = torch.zeros((1,), dtype=torch.int32, device=device)
+        self.key_weights = torch.zeros((batch, num_kv_heads, capacity), dtype=torch.float32, device=device) if track_weights else None
 
     @property
     def cache_index(self) -> torch.Tensor:
@@ -42,6 +49,8 @@ class DecodeCache:
     def reset(self, lengths=None):
         self._positions.zero_()
         self._overflow.zero_()
+        if self.key_weights is not None:
+            self.key_weights.zero_()
         if lengths is not None:
             self._positions[: self.batch] = torch.as_tensor(lengths, dtype=torch.int32, device=self._positions.device)
 
@@ -70,19 +79,58 @@ class DecodeCache:
         _lib.check(rc)
 
     def attend(self, query: torch.Tensor, *, sm_scale: float | None = None, return_lse: bool = False,
-               prefix_length: int | None = None):
+               prefix_length: int | None = None, window: int | None = None):
         """Attention of ``query [B, n, Hq, D]`` over the filled prefix.  One query token per
         sequence is a decode step (split-KV kernel, ragged positions).  Several query tokens
         (a prefill chunk just appended) need ``prefix_length``: the common number of valid
-        tokens after the append, for the bottom-right causal mask."""
+        tokens after the append, for the bottom-right causal mask.
+
+        With ``track_weights`` the attention that every key receives is added to ``key_weights``: of all queries, or of the last
+        ``window`` ones (which costs one more pass over the keys for those queries)."""
         if sm_scale is None:
             sm_scale = 1.0 / math.sqrt(query.shape[-1])
         mask = KVLenMask(self.cache_index)
-        if query.shape[1] > 1:
+        n = query.shape[1]
+        if n > 1:
             if prefix_length is None:
                 raise ValueError("attend with several query tokens needs prefix_length (tokens valid after the append)")
-            mask = mask & CausalFromBottomRightMask(query.shape[1], int(prefix_length))
-        return mha(query, self.cached_key, self.cached_value, mask=mask, sm_scale=sm_scale, return_lse=return_lse)
+            mask = mask & CausalFromBottomRightMask(n, int(prefix_length))
+        if window is not None and (self.key_weights is None or window < 1):
+            raise ValueError("window is a positive number of queries whose attention counts, with track_weights")
+        if self.key_weights is None:
+            return mha(query, self.cached_key, self.cached_value, mask=mask, sm_scale=sm_scale, return_lse=return_lse)
+        if n == 1 and not _wants_grad(query, self.cached_key, self.cached_value):
+            res = decode_weights(query, self.cached_key, self.cached_value, self.key_weights, kv_lengths=self.cache_index, sm_scale=sm_scale,
+                                 return_lse=return_lse, out=self.key_weights)
+            return res[:2] if return_lse else res[0]
+        out, lse = mha(query, self.cached_key, self.cached_value, mask=mask, sm_scale=sm_scale, return_lse=True)
+        q, part = query.detach(), lse.detach()
+        if window is not None and window < n:
+            q, part = q[:, n - window:], part[:, :, n - window:]
+            mask = KVLenMask(self.cache_index) & CausalFromBottomRightMask(window, int(prefix_length))
+        key_weights(q, self.cached_key, part, weights=self.key_weights, mask=mask, sm_scale=sm_scale, out=self.key_weights)
+        return (out, lse) if return_lse else out
+
+    def attend_tree(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, parents, *, sm_scale: float | None = None,
+                    return_lse: bool = False):
+        """Attention of a tree of drafted tokens ``query [B, N, Hq, D]`` over the filled prefix and their ancestors among the
+        drafts (:func:`decode_tree`); ``key`` / ``value`` ``[B, N, Hkv, D]`` are the drafts' own and do not enter the cache."""
+        return decode_tree(query, key, value, self.cached_key, self.cached_value, parents, kv_lengths=self.cache_index, sm_scale=sm_scale,
+                           return_lse=return_lse)
+
+    def accept(self, key: torch.Tensor, value: torch.Tensor, path, counts):
+        """Append the accepted drafts ``path[b, :counts[b]]`` of ``key`` / ``value`` and advance the positions on the device
+        (:func:`accept_drafts`)."""
+        accept_drafts(key, value, self.cached_key, self.cached_value, path, counts, kv_lengths=self.cache_index, out=self.cache_index,
+                      overflow=self._overflow)
+
+    def evict(self, keep: int, *, recent: int = 0) -> torch.Tensor:
+        """Cut every sequence to ``keep`` keys per KV head, by ``key_weights`` and with the ``recent`` last ones kept
+        (:func:`evict`), in place.  Returns the kept keys' former indices ``int32 [B, Hkv, keep]``."""
+        if self.key_weights is None:
+            raise ValueError("evict needs a cache with track_weights=True")
+        return evict(self.cached_key, self.cached_value, self.key_weights, self.cache_index, keep, recent=recent,
+                     lengths_out=self.cache_index)[1]
 
     def step(self, query, key, value, *, sm_scale: float | None = None):
         """One decode step: append the token's key / value, then attend over the prefix."""
@@ -111,6 +159,88 @@ def rope_interleaved(x: torch.Tensor, positions=None, *, base: float = 10_000.0,
                                              float(base), _DTYPES[x.dtype], _stream(x.device))
     _lib.check(rc)
     return y
+
+
+_POSITION_TYPES = {torch.float32: _lib.POS_F32, torch.int32: _lib.POS_I32, torch.int64: _lib.POS_I64}
+
+
+def _rope_axes_call(x, positions, sections, base, shared, interleaved, inverse, out=None):
+    """One ``pjx_rope_axes`` call: ``x [B, T, H, D]`` with any sequence and token stride, ``positions [B|1, T, axes]`` dense."""
+    B, T, H, D = x.shape
+    if (x.stride(3) != 1 and D > 1) or (x.stride(2) != D and H > 1):
+        x = x.contiguous()
+    y = torch.empty((B, T, H, D), dtype=x.dtype, device=x.device) if out is None else out
+    with torch.cuda.device(x.device):
+        rc = _lib.lib().pjx_rope_axes(_ptr(x), x.stride(0) if B > 1 else 0, x.stride(1) if T > 1 else 0, _ptr(y), _ptr(positions),
+                                      _POSITION_TYPES[positions.dtype], 0 if positions.shape[0] == 1 else positions.stride(0), len(sections),
+                                      (ctypes.c_int32 * len(sections))(*sections), B, T, H, D, int(shared), int(interleaved), int(inverse),
+                                      float(base), _DTYPES[x.dtype], _stream(x.device))
+    _lib.check(rc)
+    return y
+
+
+class _RopeAxesFunction(torch.autograd.Function):
+    """A rotation.  Its gradient is the rotation by the opposite angles, its tangent the same rotation."""
+
+    @staticmethod
+    def forward(ctx, x, positions, args, inverse):
+        ctx.save_for_backward(positions)
+        ctx.save_for_forward(positions)
+        ctx.args, ctx.inverse = args, inverse
+        return _rope_axes_call(x, positions, *args, inverse)
+
+    @staticmethod
+    def backward(ctx, dy):
+        return _RopeAxesFunction.apply(dy, ctx.saved_tensors[0], ctx.args, not ctx.inverse), None, None, None
+
+    @staticmethod
+    def jvp(ctx, tx, *_):
+        return _rope_axes_call(tx, ctx.saved_tensors[0], *ctx.args, ctx.inverse)
+
+
+def rope_axes(x: torch.Tensor, positions, sections, *, base: float = 10_000.0, shared: bool = False, interleaved: bool = True,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary embedding with several axes and positions of every sequence's own (``pjx_rope_axes``): ``x [..., T, H, D]``,
+    ``positions [T, axes]`` or ``[..., T, axes]`` (float32, int32 or int64, leading dimensions as ``x``), ``sections`` the
+    elements of a head vector that each axis rotates (even; they follow one another, the rest is copied).  Pair ``i`` of an axis turns
+    by ``position * base**(-2 i / section)``; with ``shared`` the frequencies run through all axes,
+    ``base**(-2 p / sum(sections))`` for pair ``p``.  ``interleaved``: pairs are neighbours, otherwise the two halves of the rotated
+    part.  A slice of a fused projection is read in place.  Differentiable with respect to ``x``; ``out`` (dense, may be a dense ``x``)
+    takes the result where no gradient is wanted.  One axis is :func:`rope_interleaved` with positions per sequence."""
+    _require_gpu()
+    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dim() < 3 or x.dtype not in _DTYPES:
+        raise ValueError("rope_axes takes a CUDA tensor [..., T, H, D] of dtype float32, bfloat16 or float16")
+    sections = tuple(int(s) for s in sections)
+    T, H, D = x.shape[-3:]
+    lead = tuple(x.shape[:-3])
+    pos = torch.as_tensor(positions)
+    if pos.dtype not in _POSITION_TYPES:
+        if pos.is_complex() or pos.dtype == torch.bool:
+            raise ValueError(f"positions must be numbers, got {pos.dtype}")
+        pos = pos.to(torch.float32 if pos.is_floating_point() else torch.int64)
+    pos = pos.to(x.device)
+    if tuple(pos.shape) == (T, len(sections)):
+        pos = pos[None].contiguous()
+    elif tuple(pos.shape) == lead + (T, len(sections)):
+        pos = pos.reshape(-1, T, len(sections)).contiguous()
+    else:
+        raise ValueError(f"positions must be [T={T}, axes={len(sections)}] or [..., T, axes] with the leading dimensions {list(lead)}, "
+                         f"got {tuple(pos.shape)}")
+    x4 = x[None] if x.dim() == 3 else x if x.dim() == 4 else x.reshape((-1,) + tuple(x.shape[-3:]))
+    if _wants_grad(x):
+        if out is not None:
+            raise ValueError("rope_axes: out cannot be given where a gradient is wanted")
+        return _RopeAxesFunction.apply(x4, pos, (sections, base, shared, interleaved), False).reshape(x.shape)
+    if out is not None:
+        if tuple(out.shape) != tuple(x.shape) or out.dtype != x.dtype or out.device != x.device or not out.is_contiguous():
+            raise ValueError("rope_axes: out must be a dense tensor like x")
+        n = out.numel() * out.element_size()
+        same = out.data_ptr() == x.data_ptr() and x.is_contiguous()
+        if not same and x.numel() and out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr():
+            first, last = x.data_ptr(), x.data_ptr() + (sum((d - 1) * s for d, s in zip(x.shape, x.stride())) + 1) * x.element_size()
+            if first < out.data_ptr() + n and out.data_ptr() < last:
+                raise ValueError("rope_axes: out overlaps x without being it")
+    return _rope_axes_call(x4, pos, sections, base, shared, interleaved, False, out).reshape(x.shape)
 
 
 def _check_layers(x, *weights) -> None:

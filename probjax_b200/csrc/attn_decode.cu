@@ -54,7 +54,8 @@ __device__ __forceinline__ uint4 ld_volatile_v4(const uint4* p) {
 // Streams keys [start, end) of (batch b, kv head hk) and writes the partial result -- O normalised by
 // its own sum and a base-2 LSE per packed query row -- at row offset `part` of the partial arrays.
 // Every thread of the CTA takes part; on return the shared memory is free again.
-template <typename T, int HD, bool PAGED>
+// SCORES: the scores are also left in p.scores, for the attention that every key receives.
+template <typename T, int HD, bool PAGED, bool SCORES = false>
 __device__ __forceinline__ void stream_segment(const DecodeParams& p, unsigned char* smem_raw, int b, int hk, int start,
                                                int end, int64_t part) {
   constexpr int CH = HD / 8;               // 16-byte chunks per row
@@ -169,6 +170,17 @@ __device__ __forceinline__ void stream_segment(const DecodeParams& p, unsigned c
         s[nt][e] = x;
         tmax[e >> 1] = fmaxf(tmax[e >> 1], x);
       }
+    if constexpr (SCORES) {  // (rows of score_pitch floats hold whole 64-key tiles: what lies past `end` is not read)
+      float* sc = p.scores + ((int64_t)b * p.Hkv + hk) * p.rows * p.score_pitch + key_w + (lane & 3) * 2;
+#pragma unroll
+      for (int hrow = 0; hrow < 2; ++hrow) {
+        const int r = (lane >> 2) + hrow * 8;
+        if (r >= p.rows) continue;
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+          *reinterpret_cast<float2*>(sc + (int64_t)r * p.score_pitch + nt * 8) = make_float2(s[nt][2 * hrow], s[nt][2 * hrow + 1]);
+      }
+    }
 #pragma unroll
     for (int hrow = 0; hrow < 2; ++hrow) {
       tmax[hrow] = fmaxf(tmax[hrow], __shfl_xor_sync(0xffffffffu, tmax[hrow], 1));
@@ -284,7 +296,7 @@ __device__ __forceinline__ void stream_segment(const DecodeParams& p, unsigned c
 // head) to finish combines the head's splits, stores the rank's partial into every rank's
 // exchange buffer, raises the head's flag there, waits (bounded) for the same head's flags of
 // all ranks and writes the final result -- the whole exchange inside this one launch.
-template <typename T, int HD, bool PAGED, bool FUSED>
+template <typename T, int HD, bool PAGED, bool FUSED, bool SCORES = false>
 __global__ void __launch_bounds__(NTHR, 2) decode_splitkv_kernel(const DecodeParams p) {
   extern __shared__ __align__(128) unsigned char smem_raw[];
   const int split = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
@@ -299,7 +311,7 @@ __global__ void __launch_bounds__(NTHR, 2) decode_splitkv_kernel(const DecodePar
   // combine of the splits always is (it waits for this grid before it reads a partial), the next
   // step's kernel of a sharded decode is with ex_overlap.
   if (!FUSED || p.ex_overlap) asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-  stream_segment<T, HD, PAGED>(p, smem_raw, b, hk, start, end,
+  stream_segment<T, HD, PAGED, SCORES>(p, smem_raw, b, hk, start, end,
                                (((int64_t)b * p.Hkv + hk) * p.num_splits + split) * p.rows);
   [[maybe_unused]] const int tid = threadIdx.x;
   [[maybe_unused]] const int G = p.Hq / p.Hkv;
@@ -424,11 +436,7 @@ __global__ void __launch_bounds__(NTHR, 2) decode_splitkv_kernel(const DecodePar
 
 // One CTA per packed row (b, kv head, r): exact combine of the valid splits.
 template <typename TO>
-__global__ void combine_splits_kernel(const DecodeParams p) {
-  const int r = blockIdx.x, hk = blockIdx.y;
-  // Launched with programmatic stream serialization, the grid may be resident before the split kernel
-  // has finished: wait for that grid and its stores.  (Does nothing under a plain launch.)
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+__device__ __forceinline__ void combine_row(const DecodeParams& p, int r, int hk) {
   const DecodeSeq sq = decode_seq(p, blockIdx.z);
   const int len = sq.len;
   const int ns = (len + p.split_len - 1) / p.split_len;
@@ -453,6 +461,80 @@ __global__ void combine_splits_kernel(const DecodeParams p) {
   }
   if (p.lse && threadIdx.x == 0)
     p.lse[decode_lse_index(p, sq, h, t)] = denom > 0.f ? (msafe + log2f(denom)) * kLn2 : INFINITY;
+}
+
+template <typename TO>
+__global__ void combine_splits_kernel(const DecodeParams p) {
+  // Launched with programmatic stream serialization, the grid may be resident before the split kernel
+  // has finished: wait for that grid and its stores.  (Does nothing under a plain launch.)
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  combine_row<TO>(p, blockIdx.x, blockIdx.y);
+}
+
+// The combine of a decode with key weights: CTAs x < rows combine a row's splits, the others turn a chunk of scores into the
+// attention its keys received.  Both need the splits' log-sum-exps only, so they run side by side.
+constexpr int kWeightChunk = 1024;  // keys per CTA: eight per thread
+template <typename TO>
+__global__ void __launch_bounds__(128) combine_weights_kernel(const DecodeParams p) {
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  const int hk = blockIdx.y, b = blockIdx.z;
+  if (blockIdx.x < p.rows) {
+    combine_row<TO>(p, blockIdx.x, hk);
+    return;
+  }
+  __shared__ float lse2[16];
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int len = p.kv_lengths ? max(0, min(p.capacity, p.kv_lengths[b])) : p.capacity;
+  const int ns = (len + p.split_len - 1) / p.split_len;
+  const int64_t unit = (int64_t)b * p.Hkv + hk;
+  for (int r = tid >> 5; r < p.rows; r += 4) {
+    const float* part = p.lse_part + unit * p.num_splits * p.rows + r;
+    float m = -INFINITY;
+    for (int s = lane; s < ns; s += 32) m = fmaxf(m, part[(int64_t)s * p.rows]);
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float msafe = m == -INFINITY ? 0.f : m;
+    float sum = 0.f;
+    for (int s = lane; s < ns; s += 32) sum += exp2f(part[(int64_t)s * p.rows] - msafe);
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) lse2[r] = sum > 0.f ? msafe + log2f(sum) : INFINITY;  // +inf: no key adds anything
+  }
+  __syncthreads();
+  const float* sc = p.scores + unit * p.rows * p.score_pitch;
+  const float* in = p.weights_in ? p.weights_in + unit * p.capacity : nullptr;
+  float* out = p.weights_out + unit * p.capacity;
+  const bool vec = ((p.capacity & 3) == 0) && ((reinterpret_cast<uintptr_t>(p.weights_in) | reinterpret_cast<uintptr_t>(p.weights_out)) & 15) == 0;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int j = (blockIdx.x - p.rows) * kWeightChunk + half * 512 + tid * 4;
+    if (j >= p.capacity) break;
+    float w[4] = {0.f, 0.f, 0.f, 0.f};
+    if (j < len) {
+      for (int r = 0; r < p.rows; ++r) {
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(sc + (int64_t)r * p.score_pitch + j));
+        const float l = lse2[r];
+        w[0] += exp2f(x.x - l);
+        w[1] += exp2f(x.y - l);
+        w[2] += exp2f(x.z - l);
+        w[3] += exp2f(x.w - l);
+      }
+    } else if (in == out) {
+      continue;  // behind the valid keys nothing changes
+    }
+    if (vec) {
+      float4 old = in ? *reinterpret_cast<const float4*>(in + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+      if (j + 0 < len) old.x += w[0];
+      if (j + 1 < len) old.y += w[1];
+      if (j + 2 < len) old.z += w[2];
+      if (j + 3 < len) old.w += w[3];
+      *reinterpret_cast<float4*>(out + j) = old;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (j + e < p.capacity) out[j + e] = (in ? in[j + e] : 0.f) + (j + e < len ? w[e] : 0.f);
+    }
+  }
 }
 
 // The same for a balanced latent decode: the splits of a sequence are numbered by the device-side plan.  Their weights are
@@ -665,8 +747,8 @@ __global__ void gather_combine_kernel(const DecodeParams p) {
 template <typename TO>
 cudaError_t launch_combine_splits(const DecodeParams& p, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.rows, p.Hkv, p.B);
-  cfg.blockDim = dim3(p.balanced || p.Dv >= 128 ? 128 : 64);
+  cfg.gridDim = dim3(p.rows + (p.scores ? (p.capacity + kWeightChunk - 1) / kWeightChunk : 0), p.Hkv, p.B);
+  cfg.blockDim = dim3(p.scores || p.balanced || p.Dv >= 128 ? 128 : 64);
   cfg.dynamicSmemBytes = 0;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -674,6 +756,7 @@ cudaError_t launch_combine_splits(const DecodeParams& p, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  if (p.scores) return cudaLaunchKernelEx(&cfg, combine_weights_kernel<TO>, p);
   if (p.balanced) return cudaLaunchKernelEx(&cfg, combine_balanced_kernel<TO>, p);
   return cudaLaunchKernelEx(&cfg, combine_splits_kernel<TO>, p);
 }
@@ -698,7 +781,8 @@ template <typename T, int HD>
 int launch_decode_t(const DecodeParams& p, cudaStream_t stream) {
   constexpr int smem = NSTAGE * 2 * BK * HD * 2;
   static_assert(smem >= (NWARP * 16 * HD + 2 * NWARP * 16) * 4, "merge scratch must fit in the ring");
-  auto kern = p.block_table
+  auto kern = p.scores ? decode_splitkv_kernel<T, HD, false, false, true>
+              : p.block_table
                   ? (p.ex_fused ? decode_splitkv_kernel<T, HD, true, true> : decode_splitkv_kernel<T, HD, true, false>)
                   : (p.ex_fused ? decode_splitkv_kernel<T, HD, false, true> : decode_splitkv_kernel<T, HD, false, false>);
   int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),

@@ -400,6 +400,59 @@ int pjx_attn_decode_paged(const void* q, const void* k_pool, const void* v_pool,
   return launch_decode(p, dtype, static_cast<cudaStream_t>(stream));
 }
 
+// Scores of a decode with key weights: rows of whole 64-key tiles.
+static int score_pitch(int capacity) { return (capacity + 63) / 64 * 64; }
+
+size_t pjx_attn_decode_weights_workspace_bytes(int B, int Lq, int Hq, int Hkv, int Dv, int capacity, int split_len) {
+  if (B < 1 || Hkv < 1 || Hq < 1 || Lq < 1 || Dv < 1 || capacity < 0 || Hq % Hkv) return 0;
+  const size_t rows = (size_t)(Hq / Hkv) * Lq;
+  if (rows > 16) return align_up((size_t)B * Hq * Lq * sizeof(float));  // (the log-sum-exps of the regular kernels)
+  return pjx_attn_decode_workspace_bytes(B, Lq, Hq, Hkv, Dv, capacity, split_len) +
+         align_up((size_t)B * Hkv * rows * score_pitch(capacity) * sizeof(float));
+}
+
+int pjx_attn_decode_weights(const void* q, const void* k_cache, const void* v_cache, const int32_t* kv_lengths,
+                            const float* weights_in, float* weights_out, void* o, float* lse, int B, int Lq, int Hq, int Hkv,
+                            int D, int Dv, int capacity, int dtype, float sm_scale, int split_len, void* workspace,
+                            size_t workspace_bytes, int32_t* status, void* stream) {
+  int rc = validate_common(q, k_cache, v_cache, o, B, Lq, capacity, Hq, Hkv, D, Dv, dtype);
+  if (rc) return rc;
+  if ((rc = decode_limits(B, Hkv, capacity))) return rc;
+  if (B == 0 || Lq == 0) return PJX_OK;
+  if (capacity > 0 && !weights_out) return fail(PJX_ERR_BAD_ARG, "decode with key weights: null buffer");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const size_t need = pjx_attn_decode_weights_workspace_bytes(B, Lq, Hq, Hkv, Dv, capacity, split_len);
+  if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))
+    return fail(PJX_ERR_WORKSPACE, "decode workspace: need %zu bytes, 16-byte aligned, got %zu", need, workspace ? workspace_bytes : (size_t)0);
+  DecodeParams p;
+  p.q = q; p.k = k_cache; p.v = v_cache; p.kv_lengths = kv_lengths; p.o = o; p.lse = lse;
+  p.B = B; p.Lq = Lq; p.Hq = Hq; p.Hkv = Hkv; p.D = D; p.Dv = Dv; p.capacity = capacity;
+  p.rows = (Hq / Hkv) * Lq;
+  p.sm_scale = sm_scale;
+  p.o_is_f32 = 0;
+  const bool aligned =
+      ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15) == 0;
+  if (!decode_fast_supported(p, dtype) || !aligned || capacity == 0) {
+    // Shapes the streaming kernel does not take: the forward kernels, then one more pass over the keys.
+    float* l = lse ? lse : static_cast<float*>(workspace);
+    if (!lse && workspace_bytes < (size_t)B * Hq * Lq * sizeof(float))
+      return fail(PJX_ERR_WORKSPACE, "decode workspace: need %zu bytes, got %zu", (size_t)B * Hq * Lq * sizeof(float), workspace_bytes);
+    if ((rc = pjx_attn_fwd(q, k_cache, v_cache, o, l, kv_lengths, nullptr, 0, 0, B, Lq, capacity, Hq, Hkv, D, Dv, dtype, 0,
+                           sm_scale, PJX_IMPL_AUTO, status, stream)))
+      return rc;
+    if (capacity == 0) return PJX_OK;
+    return pjx_attn_key_weights(q, k_cache, l, weights_in, weights_out, kv_lengths, B, Lq, capacity, Hq, Hkv, D, dtype,
+                                PJX_BAND_NO_LOWER, PJX_BAND_NO_UPPER, sm_scale, PJX_IMPL_AUTO, status, stream);
+  }
+  if ((rc = decode_place_partials(p, dtype, split_len, workspace, workspace_bytes, true))) return rc;
+  p.scores = reinterpret_cast<float*>(static_cast<char*>(workspace) +
+                                      decode_partial_bytes((size_t)B * Hkv * p.num_splits * p.rows, Dv));
+  p.score_pitch = score_pitch(capacity);
+  p.weights_in = weights_in;
+  p.weights_out = weights_out;
+  return launch_decode(p, dtype, st);
+}
+
 size_t pjx_attn_decode_sharded_buffer_bytes(int B, int Lq, int Hq, int Dv, int world) {
   if (B < 1 || Lq < 1 || Hq < 1 || Dv < 1 || world < 1 || world > kMaxExchangeRanks) return 0;
   return align_up(exchange_buffer_bytes(world, (int64_t)B * Lq * Hq, Dv));

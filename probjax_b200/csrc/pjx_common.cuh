@@ -116,6 +116,12 @@ struct DecodeParams {
   // Latent decode over ragged sequences (balanced > 0): the split length is chosen on the device from the valid lengths
   // (balanced_plan below) so that `balanced` splits in all cover the batch; grid x walks them, partials are indexed by it.
   int balanced = 0;
+  // Decode that adds up the attention every key receives: the split kernel leaves its scores, in the exp2 domain, in
+  // scores [B, Hkv, rows, score_pitch], and the combine adds sum_rows exp2(score - lse) to weights_in [B, Hkv, capacity].
+  float* scores = nullptr;
+  int score_pitch = 0;
+  const float* weights_in = nullptr;  // null: zeros
+  float* weights_out = nullptr;       // may be weights_in
 };
 constexpr int kBalancedMaxSeqs = 128;   // sequences the device-side plan takes (4 per lane)
 constexpr int kBalancedMaxItems = 256;  // splits of one row group
@@ -270,6 +276,48 @@ struct BwdParams {
   bool lse_natural = false;   // lse2 holds the natural log-sum-exp (tcgen05 kernels that add terms to the scores)
 };
 
+// Attention that every key receives from the query rows of its group (key_weights.cu): out[b, hk, j] = in[b, hk, j] +
+// sum over the visible rows (t, h) of exp(sm_scale q.k - lse).
+struct KeyWeightsParams {
+  const void* q;              // [B, Lq, Hq, D]
+  const void* k;              // [B, Lkv, Hkv, D]
+  const float* lse;           // [B, Hq, Lq] natural log, +inf for rows without keys
+  const float* weights_in;    // [B, Hkv, Lkv] or null (zeros)
+  float* weights_out;         // may be weights_in
+  const int32_t* kv_lengths;  // [B] or null
+  int B, Lq, Lkv, Hq, Hkv, D;
+  int band_lo, band_hi;       // key j is visible to query i iff i + band_lo <= j <= i + band_hi
+  float sm_scale;
+  int32_t* status = nullptr;
+};
+
+// Attention of a tree of drafted tokens over a cache (attn_tree.cu, attn_tree_sm100.cu).  Keys of a sequence in tiles of
+// kTreeTile: first those of the cached prefix, then those of the drafts.
+constexpr int kTreeTile = 128;
+constexpr int kTreeMaxNodes = 256;
+struct TreeParams {
+  const void* q;      // row (b, t) at b * q_bs + t * q_ts elements; heads dense
+  const void* k_new;  // drafts' keys and values, strided the same way
+  const void* v_new;
+  int64_t q_bs, q_ts, kn_bs, kn_ts, vn_bs, vn_ts;
+  const void* k;      // [B, capacity, Hkv, D], or page pools
+  const void* v;
+  const int32_t* parents;  // [B, N] (parents_bs = 0: one tree for all)
+  int64_t parents_bs;
+  const int32_t* kv_lengths;   // [B]
+  const int32_t* block_table;  // [B, max_pages] or null
+  int page_size, max_pages, num_pages;
+  void* o;            // [B, N, Hq, Dv]
+  float* lse;         // [B, Hq, N] or null
+  float* o_part;      // [Hkv, splits, N * G, Dv] fp32, rows (t, g)
+  float* lse_part;    // [Hkv, splits, N * G] base 2, -inf for a split without keys
+  int B, N, Hq, Hkv, D, Dv, capacity;
+  int splits;         // splits of the whole batch (grid x)
+  int per_seq;        // > 0: that many splits for every sequence; 0: dealt out on the device from the lengths
+  float sm_scale;
+  int32_t* status;
+};
+
 constexpr int kMaxExchangeRanks = 16;
 __host__ __device__ inline size_t exchange_record_floats(int world, int64_t n_rows, int Dv) { return (size_t)world * n_rows * (Dv + 1); }
 // byte offset of unit_flags inside an exchange buffer (16-byte aligned)
@@ -342,6 +390,10 @@ int launch_gemm_tn(const void* A, const void* Bm, void* C, int64_t M, int N, int
 int launch_gemm_tn2(const void* A, const void* B0, void* C0, int N0, const void* B1, void* C1, int N1,
                     int64_t M, int K, int dtype, int impl, int32_t* status, cudaStream_t stream,
                     int64_t lda = 0, int64_t ldc = 0);
+
+bool key_weights_sm100_supported(const KeyWeightsParams& p, int dtype);
+int launch_key_weights_sm100(const KeyWeightsParams& p, int dtype, cudaStream_t stream);
+int launch_key_weights(const KeyWeightsParams& p, int dtype, int impl, cudaStream_t stream);
 
 // Gradients of the layers y_p = x . w_p^T (p < pairs <= 2) from dy_p; null outputs are skipped.
 struct LinearGrad {
