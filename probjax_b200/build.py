@@ -29,6 +29,7 @@ SOURCES = [
     "attn_decode_latent.cu",
     "attn_decode_latent_sm100.cu",
     "attn_tree.cu",
+    "attn_tree_sm100.cu",
     "key_weights.cu",
     "kv_cache.cu",
     "kv_compact.cu",

@@ -34,6 +34,7 @@
 
 #include "pjx_common.cuh"
 #include "sm100_ptx.cuh"
+#include "sm100_softmax.cuh"
 
 namespace pjx {
 namespace {
@@ -42,17 +43,6 @@ using namespace sm100;
 
 constexpr int BM = 128;          // rows per query tile (= tensor-memory lanes)
 constexpr int NTHREADS = 320;    // 10 warps
-
-__device__ __forceinline__ float ex2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float fmax3(float a, float b, float c) {
-  float y;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-  return y;
-}
 
 template <int DQK, int DV, int BN, int KST, int VST, bool BIAS_STAGED = false, bool REL_STAGED = false>
 struct Cfg {
@@ -80,40 +70,6 @@ struct Cfg {
   static_assert(TMEM_USED <= 512, "tensor memory has 512 columns");
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
 };
-
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
-  if constexpr (BF16) {
-    __nv_bfloat162 t = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<uint32_t*>(&t);
-  } else {
-    __half2 t = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<uint32_t*>(&t);
-  }
-}
-
-// p = exp2(x * cs - m) for one row of BN scores, running sums, pack to 16 bits and
-// store over the scores in tensor memory. All exponentials of the row form one
-// straight-line block (the stores come last) so that the scheduler can overlap the
-// latencies of independent elements.
-template <int BN, bool BF16>
-__device__ __forceinline__ void exp_pack_store(const float (&s)[BN], float2 cs2, float2 nm2, float2& sum0,
-                                               float2& sum1, uint32_t s_addr) {
-  uint32_t pk[BN / 2];
-#pragma unroll
-  for (int i = 0; i < BN / 2; i += 2) {
-    const float2 x0 = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), cs2, nm2);
-    const float2 x1 = __ffma2_rn(make_float2(s[2 * i + 2], s[2 * i + 3]), cs2, nm2);
-    const float2 p0 = make_float2(ex2_approx(x0.x), ex2_approx(x0.y));
-    const float2 p1 = make_float2(ex2_approx(x1.x), ex2_approx(x1.y));
-    sum0 = __fadd2_rn(sum0, p0);
-    sum1 = __fadd2_rn(sum1, p1);
-    pk[i] = pack16<BF16>(p0.x, p0.y);
-    pk[i + 1] = pack16<BF16>(p1.x, p1.y);
-  }
-#pragma unroll
-  for (int c = 0; c < BN / 64; ++c) tmem_st32(s_addr + c * 32, *reinterpret_cast<const uint32_t(*)[32]>(&pk[c * 32]));
-}
 
 // The same with a multiplier per probability applied after it has been added to the row sum
 // (dropout): dmul(i) is the multiplier of score column i.
@@ -874,21 +830,32 @@ EncodeTiledFn encode_fn() {
 
 }  // namespace
 
-// [B, L, H, Dim] row-major 16-bit tensor, box = 64 elements x 1 head x `rows` tokens.
-int make_tmap_blhd(CUtensorMap* m, const void* base, int dtype, int B, int L, int H, int Dim, int rows) {
+// 16-bit tensor of `rank` dimensions, innermost first (dense; `strides` in bytes from the second on), boxes in the 128-byte swizzle.
+int make_tmap_16bit(CUtensorMap* m, const void* base, int dtype, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box) {
   const int rcb = bind_context();
   if (rcb) return rcb;
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(PJX_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-  cuuint64_t dims[4] = {(cuuint64_t)Dim, (cuuint64_t)H, (cuuint64_t)L, (cuuint64_t)B};
-  cuuint64_t strides[3] = {(cuuint64_t)Dim * 2, (cuuint64_t)H * Dim * 2, (cuuint64_t)L * H * Dim * 2};
-  cuuint32_t box[4] = {64, 1, (cuuint32_t)rows, 1};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult r = fn(m, dtype == PJX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-                  const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  cuuint64_t d[5], st[4];
+  cuuint32_t bx[5], estr[5] = {1, 1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    bx[i] = box[i];
+    if (i) st[i - 1] = strides[i - 1];
+  }
+  CUresult r = fn(m, dtype == PJX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank,
+                  const_cast<void*>(base), d, st, bx, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(PJX_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
   return PJX_OK;
+}
+
+// [B, L, H, Dim] row-major 16-bit tensor, box = 64 elements x 1 head x `rows` tokens.
+int make_tmap_blhd(CUtensorMap* m, const void* base, int dtype, int B, int L, int H, int Dim, int rows) {
+  const uint64_t dims[4] = {(uint64_t)Dim, (uint64_t)H, (uint64_t)L, (uint64_t)B};
+  const uint64_t strides[3] = {(uint64_t)Dim * 2, (uint64_t)H * Dim * 2, (uint64_t)L * H * Dim * 2};
+  const uint32_t box[4] = {64, 1, (uint32_t)rows, 1};
+  return make_tmap_16bit(m, base, dtype, 4, dims, strides, box);
 }
 
 namespace {

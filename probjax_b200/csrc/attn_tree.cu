@@ -293,14 +293,6 @@ void plan_splits(TreeParams& p) {
 
 }  // namespace
 
-#ifndef PJX_TREE_SM100
-bool tree_sm100_supported(const TreeParams&, int, const char** why) {
-  if (why) *why = "not built";
-  return false;
-}
-int launch_tree_sm100(const TreeParams&, int, cudaStream_t) { return fail(PJX_ERR_UNSUPPORTED, "tree"); }
-#endif
-
 }  // namespace pjx
 
 extern "C" {

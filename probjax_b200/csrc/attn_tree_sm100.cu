@@ -1,0 +1,567 @@
+// Tree attention on the tensor cores: up to 128 query rows (t, g) of a KV head's group per tile, the keys of a split streamed
+// through shared memory by TMA, both products as tcgen05 MMAs with accumulators in tensor memory.
+//
+//   o_i = sum_j softmax_j(sm_scale q_i . k_j) v_j over the cached prefix and i's ancestors among the drafts
+//
+// With few rows the call is bound by HBM (every K and V byte once); 256 rows per KV head do as much arithmetic per byte as the
+// tensor cores can take.  One CTA per SM:
+//
+//   warp 0       TMA producer: the Q tile(s), then a K ring and a V ring of 128-key tiles; pages are fetched in boxes that never
+//                straddle one
+//   warp 1       MMA issuer: S = Q.K^T, O += P.V with P read from tensor memory
+//   warps 2-5, 6-9   two softmax groups, one thread per row
+//   warp 10      clears the values of keys that nobody sees (behind the prefix, absent drafts): 0 x NaN is not 0
+//
+// One row tile (ROWS = 1): the groups take the even and the odd key tiles, each with a running (max, sum, O) of its own, so that
+// one group's softmax runs beside the other's MMAs; they are merged at the end.  Two row tiles (ROWS = 2): a group per row tile, and
+// both use every key tile.  A draft's ancestors are found by walking the parents, only in the (at most two) tiles that hold
+// drafts: 128 keep bits per row and tile.
+//
+// Every barrier wait is bounded: on expiry the role raises the CTA's abort flag, all roles drain, tensor memory is freed and the
+// status word gets PJX_ERR_DEVICE_TIMEOUT.
+#include "sm100_softmax.cuh"
+#include "tree_plan.cuh"
+
+namespace pjx {
+
+int make_tmap_blhd(CUtensorMap* m, const void* base, int dtype, int B, int L, int H, int Dim, int rows);
+int make_tmap_16bit(CUtensorMap* m, const void* base, int dtype, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box);
+
+namespace {
+
+using namespace sm100;
+
+constexpr int BN = kTreeTile;
+constexpr int NTHREADS = 352;
+
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, int c2, int c3, int c4) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%3, %4, %5, %6, %7}], [%2];\n" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+      : "memory");
+}
+__device__ __forceinline__ void st_shared4(uint32_t addr, float a, float b, float c, float d) {
+  asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+}
+__device__ __forceinline__ float4 ld_shared4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+template <int HD, int ROWS>
+struct Cfg {
+  static constexpr int SUB = HD / 64;
+  static constexpr int TILE_BYTES = SUB * 128 * 128;  // 128 rows of Q, K or V
+  static constexpr int KST = HD == 128 ? (ROWS == 1 ? 3 : 2) : 6;
+  static constexpr int VST = HD == 128 ? 3 : 6;
+  static constexpr int OFF_Q = 0;
+  static constexpr int OFF_K = OFF_Q + ROWS * TILE_BYTES;
+  static constexpr int OFF_V = OFF_K + KST * TILE_BYTES;
+  static constexpr int OFF_PAR = OFF_V + VST * TILE_BYTES;
+  static constexpr int OFF_ML = OFF_PAR + kTreeMaxNodes * 2;  // (max, sum) of the second group's rows
+  static constexpr int OFF_BAR = OFF_ML + 128 * 8;
+  static constexpr int CLEAN = 3;  // tiles that can hold keys nobody sees: the end of the prefix and two tiles of drafts
+  static constexpr int N_BAR = 1 + 2 * KST + 2 * VST + 2 + 2 + 2 * CLEAN + 1;
+  static constexpr int SMEM_BYTES = OFF_BAR + N_BAR * 8 + 16 + 1024;  // + alignment slack
+  static constexpr int TMEM_COLS = 512;
+  static_assert(2 * BN + 2 * HD <= TMEM_COLS, "tensor memory has 512 columns");
+  static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
+  static_assert(2 * 128 * HD * 4 <= (KST + VST) * TILE_BYTES, "the output is staged over the rings");
+};
+
+struct TreeGeometry {
+  int tokens;     // query tokens of a row tile
+  int row_tiles;  // CTAs that share a split and a KV head
+  int box_rows;   // keys per TMA box of the cache
+};
+
+template <int HD, bool BF16, int ROWS>
+__global__ void __launch_bounds__(NTHREADS, 1)
+attn_tree_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_kn,
+                       const __grid_constant__ CUtensorMap tm_vn, const TreeParams p, const TreeGeometry geo) {
+  using C = Cfg<HD, ROWS>;
+  extern __shared__ unsigned char smem_unaligned[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_unaligned) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = uniform(smem_u32(smem));
+  auto BAR = [&](int i) { return sbase + C::OFF_BAR + 8u * i; };
+  constexpr int Q_FULL = 0;
+  constexpr int K_FULL = 1, K_EMPTY = K_FULL + C::KST;
+  constexpr int V_FULL = K_EMPTY + C::KST, V_EMPTY = V_FULL + C::VST;
+  constexpr int S_FULL = V_EMPTY + C::VST;  // [2]
+  constexpr int P_FULL = S_FULL + 2;        // [2] 128 arrivals
+  constexpr int V_CLEAN = P_FULL + 2;       // [3] 32 arrivals: the values of keys nobody sees are cleared
+  constexpr int V_LANDED = V_CLEAN + C::CLEAN;  // [3] and may be
+  constexpr int O_DONE = V_LANDED + C::CLEAN;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_BAR + C::N_BAR * 8);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int16_t* par = reinterpret_cast<int16_t*>(smem + C::OFF_PAR);
+
+  const int warp = uniform(static_cast<int>(threadIdx.x >> 5)), lane = threadIdx.x & 31;
+  // KV heads of a split run side by side: a token's heads are neighbours in memory
+  const int x = blockIdx.x / (geo.row_tiles * p.Hkv), rem = blockIdx.x - x * (geo.row_tiles * p.Hkv);
+  const int hk = rem / geo.row_tiles, t0 = (rem - hk * geo.row_tiles) * ROWS * geo.tokens;
+  const TreeSplit sp = tree_split(p, x);
+  // The combine may be resident early; it waits for this grid.
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  if (sp.b < 0) return;  // (the whole CTA; the combine never reads this split)
+  const int b = uniform(sp.b), prefix = uniform(sp.prefix), first = uniform(sp.first), n = uniform(sp.end - sp.first);
+  const int prefix_tiles = (prefix + BN - 1) / BN;
+  const int clean0 = max(0, prefix / BN - first);  // first tile of the loop that may hold a key nobody sees
+  const int G = p.Hq / p.Hkv;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::N_BAR; ++i)
+      mbar_init(BAR(i), i >= P_FULL && i < P_FULL + 2 ? 128u : i >= V_CLEAN && i < V_CLEAN + C::CLEAN ? 32u : 1u);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  load_tree(p, b, par, threadIdx.x, NTHREADS);  // (only its loads; the barrier below covers them)
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = uniform(*tmem_slot);
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    // (converged: every lane runs the loop, one issues)
+    const uint32_t leader = elect_leader();
+    if (leader) {
+      prefetch_tmap(&tm_q);
+      prefetch_tmap(&tm_k);
+      prefetch_tmap(&tm_v);
+      const uint32_t rows_bytes = (uint32_t)(geo.tokens * G) * 128u;
+      mbar_arrive_expect_tx(BAR(Q_FULL), ROWS * C::SUB * rows_bytes);
+#pragma unroll
+      for (int t = 0; t < ROWS; ++t)
+#pragma unroll
+        for (int s = 0; s < C::SUB; ++s)
+          tma_load_5d(sbase + C::OFF_Q + t * C::TILE_BYTES + s * 128 * 128, &tm_q, BAR(Q_FULL), s * 64, 0, hk, t0 + t * geo.tokens, b);
+    }
+    const int boxes = BN / geo.box_rows;  // per tile: 1, 2, 4 or 8
+    int page_row = 0;                     // lane i: pool row of box i of the current tile
+    for (int j = 0; j < n; ++j) {
+      const int tile = first + j;
+      const bool drafts = tile >= prefix_tiles;
+      const int key0 = tile * BN;
+      if (p.block_table && !drafts) {
+        page_row = p.num_pages * p.page_size;  // outside the pool: zeros
+        const int key = key0 + lane * geo.box_rows;
+        if (lane < boxes && key < prefix) {
+          const int page = p.block_table[(int64_t)b * p.max_pages + key / p.page_size];
+          if (page >= 0 && page < p.num_pages) page_row = page * p.page_size + key % p.page_size;
+        }
+      }
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        constexpr int ST[2] = {C::KST, C::VST}, OFF[2] = {C::OFF_K, C::OFF_V}, FULL[2] = {K_FULL, V_FULL}, EMPTY[2] = {K_EMPTY, V_EMPTY};
+        const int st = j % ST[kv];
+        const bool ok = mbar_wait_all(BAR(EMPTY[kv] + st), ((j / ST[kv]) & 1) ^ 1, abort_flag);
+        if (!ok) {
+          j = n;
+          break;
+        }
+        const uint32_t bar = BAR(FULL[kv] + st), dst = sbase + OFF[kv] + st * C::TILE_BYTES;
+        if (leader) mbar_arrive_expect_tx(bar, C::TILE_BYTES);
+        if (drafts) {
+          if (leader) {
+#pragma unroll
+            for (int s = 0; s < C::SUB; ++s)
+              tma_load_4d(dst + s * 128 * 128, kv ? &tm_vn : &tm_kn, bar, s * 64, hk, (tile - prefix_tiles) * BN, b);
+          }
+        } else if (!p.block_table) {
+          if (leader) {
+#pragma unroll
+            for (int s = 0; s < C::SUB; ++s) tma_load_4d(dst + s * 128 * 128, kv ? &tm_v : &tm_k, bar, s * 64, hk, key0, b);
+          }
+        } else {
+          for (int i = 0; i < boxes; ++i) {
+            const int row = __shfl_sync(0xffffffffu, page_row, i);
+            if (leader) {
+#pragma unroll
+              for (int s = 0; s < C::SUB; ++s)
+                tma_load_4d(dst + s * 128 * 128 + i * geo.box_rows * 128, kv ? &tm_v : &tm_k, bar, s * 64, hk, row, 0);
+            }
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // -------------------------------------------------------------- MMA issuer
+    const uint32_t leader = elect_leader();
+    constexpr uint32_t idesc_s = make_idesc(128, BN, BF16, false, false);
+    constexpr uint32_t idesc_o = make_idesc(128, HD, BF16, false, true);
+    auto issue_s = [&](int t, int j) {  // scores of key tile j into buffer t
+      const uint32_t qa = sbase + C::OFF_Q + (ROWS == 2 ? t : 0) * C::TILE_BYTES;
+      const uint32_t ka = sbase + C::OFF_K + (j % C::KST) * C::TILE_BYTES;
+#pragma unroll
+      for (int s = 0; s < C::SUB; ++s)
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          mma_ss(tmem + t * BN, make_smem_desc(qa + s * 128 * 128 + kk * 32, 16, 1024),
+                 make_smem_desc(ka + s * 128 * 128 + kk * 32, 16, 1024), idesc_s, (s | kk) != 0, leader);
+    };
+    auto issue_pv = [&](int t, int j, bool fresh) {
+      const uint32_t va = sbase + C::OFF_V + (j % C::VST) * C::TILE_BYTES;
+#pragma unroll
+      for (int kk = 0; kk < BN / 16; ++kk)
+        mma_ts(tmem + 2 * BN + t * HD, tmem + t * BN + kk * 8, make_smem_desc(va + kk * 2048, 128 * 128, 1024), idesc_o,
+               !fresh || kk != 0, leader);
+    };
+    auto wait_k = [&](int j) { return mbar_wait_all(BAR(K_FULL + j % C::KST), (j / C::KST) & 1, abort_flag); };
+    auto wait_v = [&](int j) {
+      bool ok = mbar_wait_all(BAR(V_FULL + j % C::VST), (j / C::VST) & 1, abort_flag);
+      if (ok && j >= clean0) {
+        if (leader) mbar_arrive(BAR(V_LANDED + j - clean0));
+        ok = mbar_wait_all(BAR(V_CLEAN + j - clean0), 0, abort_flag);
+      }
+      return ok;
+    };
+    bool ok = mbar_wait_all(BAR(Q_FULL), 0, abort_flag);
+    if constexpr (ROWS == 1) {
+      for (int j = 0; ok && j < min(2, n); ++j) {
+        ok = wait_k(j);
+        if (!ok) break;
+        tc_fence_after();
+        issue_s(j, j);
+        mma_commit(BAR(S_FULL + j), leader);
+        mma_commit(BAR(K_EMPTY + j % C::KST), leader);
+      }
+      for (int j = 0; ok && j < n; ++j) {
+        const int t = j & 1;
+        ok = wait_v(j) && mbar_wait_all(BAR(P_FULL + t), (j >> 1) & 1, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        issue_pv(t, j, j < 2);
+        mma_commit(BAR(V_EMPTY + j % C::VST), leader);
+        if (j == n - 1) mma_commit(BAR(O_DONE), leader);
+        if (j + 2 < n) {
+          ok = wait_k(j + 2);
+          if (!ok) break;
+          tc_fence_after();
+          issue_s(t, j + 2);
+          mma_commit(BAR(S_FULL + t), leader);
+          mma_commit(BAR(K_EMPTY + (j + 2) % C::KST), leader);
+        }
+      }
+    } else {
+      if (ok) ok = wait_k(0);
+      if (ok) {
+        tc_fence_after();
+        issue_s(0, 0);
+        mma_commit(BAR(S_FULL), leader);
+        issue_s(1, 0);
+        mma_commit(BAR(S_FULL + 1), leader);
+        mma_commit(BAR(K_EMPTY), leader);
+      }
+      for (int j = 0; ok && j < n; ++j) {
+        const bool more = j + 1 < n;
+        ok = wait_v(j) && (!more || wait_k(j + 1));
+        if (!ok) break;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          ok = ok && mbar_wait_all(BAR(P_FULL + t), j & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          issue_pv(t, j, j == 0);
+          if (more) {
+            issue_s(t, j + 1);
+            mma_commit(BAR(S_FULL + t), leader);
+          }
+        }
+        if (!ok) break;
+        mma_commit(BAR(V_EMPTY + j % C::VST), leader);
+        if (more)
+          mma_commit(BAR(K_EMPTY + (j + 1) % C::KST), leader);
+        else
+          mma_commit(BAR(O_DONE), leader);
+      }
+    }
+  } else if (warp == 10) {
+    // ------------------------------------------- values of keys that nobody sees
+    // (told by the issuer, which follows the V ring: a wait for one late phase of V_FULL alone would pass at once)
+    for (int j = clean0; j < n; ++j) {
+      const int tile = first + j, st = j % C::VST;
+      if (mbar_wait(BAR(V_LANDED + j - clean0), 0, abort_flag)) {
+        bool wrote = false;
+        for (int r = lane; r < BN; r += 32) {
+          const int node = (tile - prefix_tiles) * BN + r;  // (drafts past the last one arrive as zeros)
+          const bool seen = tile < prefix_tiles ? tile * BN + r < prefix : node >= p.N || tree_present(par, node);
+          if (seen) continue;
+          wrote = true;
+          const uint32_t row = sbase + C::OFF_V + st * C::TILE_BYTES + r * 128;
+#pragma unroll
+          for (int s = 0; s < C::SUB; ++s)
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(row + s * 128 * 128 + u * 16), "r"(0) : "memory");
+        }
+        if (wrote) fence_proxy_async();
+      }
+      mbar_arrive(BAR(V_CLEAN + j - clean0));
+    }
+  } else {
+    // ------------------------------------------------------------ softmax warps
+    const int t = (warp - 2) >> 2;
+    const int quarter = warp & 3;  // tensor-memory lane quarter this warp may access
+    const int r_in = quarter * 32 + lane;
+    const int node = t0 + (ROWS == 2 ? t * geo.tokens : 0) + r_in / G;
+    const bool there = r_in < geo.tokens * G && node < p.N && tree_present(par, node);
+    const uint32_t lane_sel = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t s_addr = tmem + lane_sel + t * BN;
+    const uint32_t o_addr = tmem + lane_sel + 2 * BN + t * HD;
+    const float c1 = p.sm_scale * kLog2e;
+    constexpr int STEP = ROWS == 1 ? 2 : 1;
+    float m_ref = -INFINITY, l = 0.f;
+    bool ok = true;
+    int it = 0;
+    for (int j = ROWS == 1 ? t : 0; j < n; j += STEP, ++it) {
+      ok = mbar_wait(BAR(S_FULL + t), it & 1, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      float s[BN];
+#pragma unroll
+      for (int c = 0; c < BN / 32; ++c) tmem_ld32f(s_addr + c * 32, &s[c * 32]);
+      tmem_wait_ld();
+      const int tile = first + j;
+      if (j >= clean0) {  // keep bits of the tile's 128 keys
+        uint32_t bits[4];
+        if (tile < prefix_tiles) {
+          const int valid = prefix - tile * BN;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int k = valid - 32 * c;
+            bits[c] = k >= 32 ? 0xffffffffu : k <= 0 ? 0u : (1u << k) - 1u;
+          }
+        } else {
+          const int node0 = (tile - prefix_tiles) * BN;
+          uint32_t b0 = 0, b1 = 0, b2 = 0, b3 = 0;
+          if (there) {
+            for (int i = node; i >= node0; i = par[i]) {
+              const int k = i - node0;
+              const uint32_t bit = 1u << (k & 31);
+              if (k < 32) b0 |= bit;
+              else if (k < 64) b1 |= bit;
+              else if (k < 96) b2 |= bit;
+              else if (k < 128) b3 |= bit;
+            }
+          }
+          bits[0] = b0; bits[1] = b1; bits[2] = b2; bits[3] = b3;
+        }
+#pragma unroll
+        for (int i = 0; i < BN; ++i) s[i] = (bits[i / 32] >> (i % 32)) & 1u ? s[i] : -INFINITY;
+      }
+      float mx;
+      {
+        float m[8];  // independent chains
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m[i] = fmaxf(s[2 * i], s[2 * i + 1]);
+#pragma unroll
+        for (int i = 1; i < BN / 16; ++i)
+#pragma unroll
+          for (int u = 0; u < 8; ++u) m[u] = fmax3(m[u], s[16 * i + 2 * u], s[16 * i + 2 * u + 1]);
+        mx = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), fmaxf(fmaxf(m[4], m[5]), fmaxf(m[6], m[7])));
+      }
+      mx *= c1;  // c1 > 0
+      // lazy running maximum: advance only when it grew by more than 8 (base 2)
+      const bool need = (mx > m_ref + 8.f) || (m_ref == -INFINITY && mx > -INFINITY);
+      const bool rescale = __any_sync(0xffffffffu, need);
+      float corr = 1.f;
+      if (rescale) {
+        const float m_new = fmaxf(m_ref, mx);
+        corr = (m_new == -INFINITY) ? 1.f : exp2f(m_ref - m_new);
+        m_ref = m_new;
+        l *= corr;
+      }
+      const float neg_m = (m_ref == -INFINITY) ? 0.f : -m_ref;
+      float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
+      exp_pack_store<BN, BF16>(s, make_float2(c1, c1), make_float2(neg_m, neg_m), sum0, sum1, s_addr);
+      const float lsum = (sum0.x + sum0.y) + (sum1.x + sum1.y);
+      // the group's previous P.V completed before these scores became visible
+      if (rescale && it > 0) {
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) {
+          float o[32];
+          tmem_ld32f(o_addr + c * 32, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] *= corr;
+          tmem_st32f(o_addr + c * 32, o);
+        }
+      }
+      l += lsum;
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(BAR(P_FULL + t));
+    }
+    ok = ok && mbar_wait(BAR(O_DONE), 0, abort_flag);
+    ok = __all_sync(0xffffffffu, ok);
+    tc_fence_after();
+    // All products are done and all loads have landed: the rings are free.  The rows leave through shared memory, 16-byte units
+    // swizzled by row, so that whole rows are written.
+    const int rows = p.N * G;
+    const int64_t part = ((int64_t)hk * p.splits + x) * rows;
+    const int token0 = t0 + (ROWS == 2 ? t * geo.tokens : 0);
+    const int n_rows = min(geo.tokens, p.N - token0) * G;  // rows of the tile that exist (may be none)
+    const uint32_t stage = sbase + C::OFF_K + (ROWS == 2 ? t : 0) * (128 * HD * 4);
+    const uint32_t my_row = stage + r_in * (HD * 4);
+    const bool mine = ROWS == 2 || t == 0;
+    float* ml = reinterpret_cast<float*>(smem + C::OFF_ML);
+    if constexpr (ROWS == 1) {
+      if (t == 1) {  // the odd tiles' state
+        ml[2 * r_in] = m_ref;
+        ml[2 * r_in + 1] = l;
+        if (it > 0 && ok) {
+#pragma unroll
+          for (int c = 0; c < HD / 32; ++c) {
+            float o[32];
+            tmem_ld32f(o_addr + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              st_shared4(my_row + (((c * 8 + i) ^ (r_in & 7)) << 4), o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          }
+        }
+      }
+      asm volatile("bar.sync 1, 256;\n" ::: "memory");
+    }
+    if (mine && ok) {
+      float wa = 1.f, wb = 0.f, m = m_ref, lsum = l;
+      if constexpr (ROWS == 1) {
+        const float m1 = ml[2 * r_in], l1 = ml[2 * r_in + 1];
+        m = fmaxf(m_ref, m1);
+        wa = m_ref == -INFINITY ? 0.f : exp2f(m_ref - m);
+        wb = m1 == -INFINITY ? 0.f : exp2f(m1 - m);
+        lsum = l * wa + l1 * wb;
+      }
+      const bool keep = there && lsum > 0.f;
+      const float inv = keep ? 1.f / lsum : 0.f;
+#pragma unroll
+      for (int c = 0; c < HD / 32; ++c) {
+        float o[32];
+        tmem_ld32f(o_addr + c * 32, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t at = my_row + (((c * 8 + i) ^ (r_in & 7)) << 4);
+          float4 v = make_float4(o[4 * i] * wa, o[4 * i + 1] * wa, o[4 * i + 2] * wa, o[4 * i + 3] * wa);
+          if (ROWS == 1 && wb != 0.f) {
+            const float4 w = ld_shared4(at);
+            v = make_float4(fmaf(w.x, wb, v.x), fmaf(w.y, wb, v.y), fmaf(w.z, wb, v.z), fmaf(w.w, wb, v.w));
+          }
+          if (keep)
+            st_shared4(at, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+          else
+            st_shared4(at, 0.f, 0.f, 0.f, 0.f);
+        }
+      }
+      if (r_in < n_rows) p.lse_part[part + (int64_t)token0 * G + r_in] = keep ? m + log2f(lsum) : -INFINITY;
+    }
+    if constexpr (ROWS == 1)
+      asm volatile("bar.sync 1, 256;\n" ::: "memory");
+    else if (t == 0)
+      asm volatile("bar.sync 1, 128;\n" ::: "memory");
+    else
+      asm volatile("bar.sync 2, 128;\n" ::: "memory");
+    if (ok) {
+      constexpr int UNITS = HD / 4, THREADS = ROWS == 1 ? 256 : 128;
+      const int tid = ROWS == 1 ? t * 128 + (warp - 2 - 4 * t) * 32 + lane : (warp - 2 - 4 * t) * 32 + lane;
+      float* out = p.o_part + (part + (int64_t)token0 * G) * HD;
+      for (int i = tid; i < n_rows * UNITS; i += THREADS) {
+        const int r = i / UNITS, u = i % UNITS;
+        const float4 v = ld_shared4(stage + r * (HD * 4) + ((u ^ (r & 7)) << 4));
+        *reinterpret_cast<float4*>(out + (int64_t)r * HD + u * 4) = v;
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tmem_dealloc(tmem, C::TMEM_COLS);
+    if (lane == 0 && *abort_flag && p.status) atomicExch(p.status, (int)PJX_ERR_DEVICE_TIMEOUT);
+  }
+}
+
+template <int HD, bool BF16, int ROWS>
+int launch_t(const TreeParams& p, int dtype, cudaStream_t stream) {
+  using C = Cfg<HD, ROWS>;
+  const int G = p.Hq / p.Hkv;
+  TreeGeometry geo;
+  geo.tokens = 128 / G < p.N ? 128 / G : p.N;
+  geo.row_tiles = (p.N + ROWS * geo.tokens - 1) / (ROWS * geo.tokens);
+  geo.box_rows = BN;
+  while (p.block_table && p.page_size % geo.box_rows) geo.box_rows /= 2;
+  int rc = bind_context();
+  if (rc) return rc;
+  CUtensorMap tq, tk, tv, tkn, tvn;
+  // (the stride of a dimension of one entry means nothing, but has to be one)
+  auto token = [&](int64_t s, int heads) { return (uint64_t)(p.N > 1 ? s : (int64_t)heads * HD) * 2; };
+  auto sequence = [&](int64_t s, int heads) { return (uint64_t)(p.B > 1 ? s : (int64_t)p.N * heads * HD) * 2; };
+  {
+    const uint64_t dims[5] = {(uint64_t)HD, (uint64_t)G, (uint64_t)p.Hkv, (uint64_t)p.N, (uint64_t)p.B};
+    const uint64_t strides[4] = {(uint64_t)HD * 2, (uint64_t)G * HD * 2, token(p.q_ts, p.Hq), sequence(p.q_bs, p.Hq)};
+    const uint32_t box[5] = {64, (uint32_t)G, 1, (uint32_t)geo.tokens, 1};
+    if ((rc = make_tmap_16bit(&tq, p.q, dtype, 5, dims, strides, box))) return rc;
+  }
+  for (int kv = 0; kv < 2; ++kv) {
+    const uint64_t dims[4] = {(uint64_t)HD, (uint64_t)p.Hkv, (uint64_t)p.N, (uint64_t)p.B};
+    const uint64_t strides[3] = {(uint64_t)HD * 2, token(kv ? p.vn_ts : p.kn_ts, p.Hkv), sequence(kv ? p.vn_bs : p.kn_bs, p.Hkv)};
+    const uint32_t box[4] = {64, 1, BN, 1};
+    if ((rc = make_tmap_16bit(kv ? &tvn : &tkn, kv ? p.v_new : p.k_new, dtype, 4, dims, strides, box))) return rc;
+    const void* base = kv ? p.v : p.k;
+    CUtensorMap* m = kv ? &tv : &tk;
+    const int rows = p.block_table ? p.num_pages * p.page_size : p.capacity;
+    if (rows == 0)
+      *m = kv ? tvn : tkn;  // no cache: never used
+    else if ((rc = make_tmap_blhd(m, base, dtype, p.block_table ? 1 : p.B, rows, p.Hkv, HD, geo.box_rows)))
+      return rc;
+  }
+  auto kern = attn_tree_sm100_kernel<HD, BF16, ROWS>;
+  if ((rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES), "cudaFuncSetAttribute(tree)")))
+    return rc;
+  kern<<<(unsigned)((int64_t)p.splits * p.Hkv * geo.row_tiles), NTHREADS, C::SMEM_BYTES, stream>>>(tq, tk, tv, tkn, tvn, p, geo);
+  count_launch();
+  return check_cuda(cudaGetLastError(), "tree attention launch");
+}
+
+template <int HD, bool BF16>
+int launch_rows(const TreeParams& p, int dtype, cudaStream_t stream) {
+  const int G = p.Hq / p.Hkv;
+  return p.N > 128 / G ? launch_t<HD, BF16, 2>(p, dtype, stream) : launch_t<HD, BF16, 1>(p, dtype, stream);
+}
+
+}  // namespace
+
+bool tree_sm100_supported(const TreeParams& p, int dtype, const char** why) {
+  const char* w = nullptr;
+  const int64_t units = p.q_bs | p.q_ts | p.kn_bs | p.kn_ts | p.vn_bs | p.vn_ts;
+  if (dtype != PJX_BF16 && dtype != PJX_F16) w = "dtype must be bf16 or fp16";
+  else if (p.D != p.Dv || (p.D != 64 && p.D != 128)) w = "head widths must be (64, 64) or (128, 128)";
+  else if (p.Hq / p.Hkv > 128) w = "at most 128 query heads a KV head";
+  else if (!(p.sm_scale > 0.f)) w = "sm_scale must be positive";
+  else if (units % 8) w = "strides must be whole 16 bytes";
+  else if ((p.B > 1 && (p.q_bs == 0 || p.kn_bs == 0 || p.vn_bs == 0)) || (p.N > 1 && (p.q_ts == 0 || p.kn_ts == 0 || p.vn_ts == 0)))
+    w = "rows must not share memory";
+  else if ((reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) |
+            reinterpret_cast<uintptr_t>(p.k_new) | reinterpret_cast<uintptr_t>(p.v_new)) & 15)
+    w = "addresses must be 16-byte aligned";
+  else if (p.block_table && (int64_t)p.num_pages * p.page_size >= 0x7fffffff) w = "a pool of fewer than 2^31 rows";
+  else if ((int64_t)p.splits * p.Hkv * p.N > 0x7fffffffLL) w = "grid too large";
+  if (why) *why = w;
+  return w == nullptr;
+}
+
+int launch_tree_sm100(const TreeParams& p, int dtype, cudaStream_t stream) {
+  if (dtype == PJX_BF16) return p.D == 128 ? launch_rows<128, true>(p, dtype, stream) : launch_rows<64, true>(p, dtype, stream);
+  return p.D == 128 ? launch_rows<128, false>(p, dtype, stream) : launch_rows<64, false>(p, dtype, stream);
+}
+
+}  // namespace pjx
