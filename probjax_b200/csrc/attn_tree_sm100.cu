@@ -17,6 +17,10 @@
 // both use every key tile.  A draft's ancestors are found by walking the parents, only in the (at most two) tiles that hold
 // drafts: 128 keep bits per row and tile.
 //
+// A CTA's run of the work (tree_plan.cuh) is a few segments, each a stretch of one sequence's keys; barriers and rings run on
+// through all of them, and since the output leaves through the Q tile's shared memory, the next segment's keys are
+// fetched meanwhile.
+//
 // Every barrier wait is bounded: on expiry the role raises the CTA's abort flag, all roles drain, tensor memory is freed and the
 // status word gets PJX_ERR_DEVICE_TIMEOUT.
 #include "sm100_softmax.cuh"
@@ -59,22 +63,19 @@ struct Cfg {
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_K = OFF_Q + ROWS * TILE_BYTES;
   static constexpr int OFF_V = OFF_K + KST * TILE_BYTES;
-  static constexpr int OFF_PAR = OFF_V + VST * TILE_BYTES;
-  static constexpr int OFF_ML = OFF_PAR + kTreeMaxNodes * 2;  // (max, sum) of the second group's rows
-  static constexpr int OFF_BAR = OFF_ML + 128 * 8;
-  static constexpr int CLEAN = 3;  // tiles that can hold keys nobody sees: the end of the prefix and two tiles of drafts
-  static constexpr int N_BAR = 1 + 2 * KST + 2 * VST + 2 + 2 + 2 * CLEAN + 1;
+  static constexpr int OFF_ML = OFF_V + VST * TILE_BYTES;  // (max, sum) of the second group's rows
+  static constexpr int OFF_WORK = OFF_ML + 128 * 8;        // the softmax warps' segments
+  static constexpr int OFF_BAR = OFF_WORK + 8 * 64;
+  static constexpr int N_BAR = 2 + 2 * KST + 2 * VST + 2 + 2 + 2 + 1 + 2;
   static constexpr int SMEM_BYTES = OFF_BAR + N_BAR * 8 + 16 + 1024;  // + alignment slack
   static constexpr int TMEM_COLS = 512;
   static_assert(2 * BN + 2 * HD <= TMEM_COLS, "tensor memory has 512 columns");
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
-  static_assert(2 * 128 * HD * 4 <= (KST + VST) * TILE_BYTES, "the output is staged over the rings");
 };
 
 struct TreeGeometry {
-  int tokens;     // query tokens of a row tile
-  int row_tiles;  // CTAs that share a split and a KV head
-  int box_rows;   // keys per TMA box of the cache
+  int tokens;    // query tokens of a row tile
+  int box_rows;  // keys per TMA box of the cache
 };
 
 template <int HD, bool BF16, int ROWS>
@@ -87,34 +88,49 @@ attn_tree_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_unaligned) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = uniform(smem_u32(smem));
   auto BAR = [&](int i) { return sbase + C::OFF_BAR + 8u * i; };
-  constexpr int Q_FULL = 0;
-  constexpr int K_FULL = 1, K_EMPTY = K_FULL + C::KST;
+  constexpr int Q_FULL = 0, Q_FREE = 1;  // Q_FREE: 256 arrivals, the output staged over Q has left
+  constexpr int K_FULL = 2, K_EMPTY = K_FULL + C::KST;
   constexpr int V_FULL = K_EMPTY + C::KST, V_EMPTY = V_FULL + C::VST;
   constexpr int S_FULL = V_EMPTY + C::VST;  // [2]
   constexpr int P_FULL = S_FULL + 2;        // [2] 128 arrivals
-  constexpr int V_CLEAN = P_FULL + 2;       // [3] 32 arrivals: the values of keys nobody sees are cleared
-  constexpr int V_LANDED = V_CLEAN + C::CLEAN;  // [3] and may be
-  constexpr int O_DONE = V_LANDED + C::CLEAN;
+  constexpr int V_LANDED = P_FULL + 2;      // a tile that may hold keys nobody sees is there
+  constexpr int V_CLEAN = V_LANDED + 1;     // 32 arrivals: their values are cleared
+  constexpr int O_DONE = V_CLEAN + 1;
+  constexpr int MEET = O_DONE + 1;          // [2] the softmax threads that stage a tile meet here (bounded, unlike a named barrier)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_BAR + C::N_BAR * 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int16_t* par = reinterpret_cast<int16_t*>(smem + C::OFF_PAR);
 
   const int warp = uniform(static_cast<int>(threadIdx.x >> 5)), lane = threadIdx.x & 31;
-  // KV heads of a split run side by side: a token's heads are neighbours in memory
-  const int x = blockIdx.x / (geo.row_tiles * p.Hkv), rem = blockIdx.x - x * (geo.row_tiles * p.Hkv);
-  const int hk = rem / geo.row_tiles, t0 = (rem - hk * geo.row_tiles) * ROWS * geo.tokens;
-  const TreeSplit sp = tree_split(p, x);
+  const TreeLine line = tree_line(p);
   // The combine may be resident early; it waits for this grid.
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-  if (sp.b < 0) return;  // (the whole CTA; the combine never reads this split)
-  const int b = uniform(sp.b), prefix = uniform(sp.prefix), first = uniform(sp.first), n = uniform(sp.end - sp.first);
-  const int prefix_tiles = (prefix + BN - 1) / BN;
-  const int clean0 = max(0, prefix / BN - first);  // first tile of the loop that may hold a key nobody sees
-  const int G = p.Hq / p.Hkv;
+  if ((int)blockIdx.x >= line.ctas) return;
+  const int64_t start = tree_run(line, blockIdx.x), stop = tree_run(line, blockIdx.x + 1);
+  const int G = p.Hq / p.Hkv, row_tiles = p.columns / p.Hkv;
+  // What the roles need of a segment; every warp walks the same segments.
+  struct Work {
+    int b, hk, t0, first, n, prefix, prefix_tiles, clean0;
+    int64_t slot;
+  };
+  auto next = [&](int64_t& pos, Work& w) {
+    if (pos >= stop) return false;
+    const TreeSegment sg = tree_segment(p, line, blockIdx.x, pos, stop);
+    w.b = uniform(sg.b);
+    w.prefix = uniform(sg.prefix);
+    w.first = uniform(sg.first);
+    w.n = uniform(sg.end - sg.first);
+    w.slot = sg.slot;
+    w.hk = uniform(sg.column / row_tiles);
+    w.t0 = uniform((sg.column - w.hk * row_tiles) * ROWS * geo.tokens);
+    w.prefix_tiles = (w.prefix + BN - 1) / BN;
+    w.clean0 = max(0, w.prefix / BN - w.first);  // first tile of the segment that may hold a key nobody sees
+    pos += w.n;
+    return true;
+  };
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::N_BAR; ++i)
-      mbar_init(BAR(i), i >= P_FULL && i < P_FULL + 2 ? 128u : i >= V_CLEAN && i < V_CLEAN + C::CLEAN ? 32u : 1u);
+      mbar_init(BAR(i), i == Q_FREE ? 256u : i >= P_FULL && i < P_FULL + 2 ? 128u : i == V_CLEAN ? 32u : i >= MEET ? (ROWS == 1 ? 256u : 128u) : 1u);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -122,7 +138,6 @@ attn_tree_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
     tmem_relinquish();
   }
-  load_tree(p, b, par, threadIdx.x, NTHREADS);  // (only its loads; the barrier below covers them)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -136,163 +151,174 @@ attn_tree_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       prefetch_tmap(&tm_q);
       prefetch_tmap(&tm_k);
       prefetch_tmap(&tm_v);
-      const uint32_t rows_bytes = (uint32_t)(geo.tokens * G) * 128u;
-      mbar_arrive_expect_tx(BAR(Q_FULL), ROWS * C::SUB * rows_bytes);
+    }
+    const int boxes = BN / geo.box_rows;  // per tile: 1, 2, 4 or 8
+    int g = 0, seg = 0;                   // tiles loaded so far, segments
+    bool ok = true;
+    Work w = {};
+    auto load_q = [&] {
+      ok = mbar_wait_all(BAR(Q_FREE), (seg & 1) ^ 1, abort_flag);
+      if (!ok || !leader) return;
+      mbar_arrive_expect_tx(BAR(Q_FULL), ROWS * C::SUB * (uint32_t)(geo.tokens * G) * 128u);
 #pragma unroll
       for (int t = 0; t < ROWS; ++t)
 #pragma unroll
         for (int s = 0; s < C::SUB; ++s)
-          tma_load_5d(sbase + C::OFF_Q + t * C::TILE_BYTES + s * 128 * 128, &tm_q, BAR(Q_FULL), s * 64, 0, hk, t0 + t * geo.tokens, b);
-    }
-    const int boxes = BN / geo.box_rows;  // per tile: 1, 2, 4 or 8
-    int page_row = 0;                     // lane i: pool row of box i of the current tile
-    for (int j = 0; j < n; ++j) {
-      const int tile = first + j;
-      const bool drafts = tile >= prefix_tiles;
-      const int key0 = tile * BN;
-      if (p.block_table && !drafts) {
-        page_row = p.num_pages * p.page_size;  // outside the pool: zeros
-        const int key = key0 + lane * geo.box_rows;
-        if (lane < boxes && key < prefix) {
-          const int page = p.block_table[(int64_t)b * p.max_pages + key / p.page_size];
-          if (page >= 0 && page < p.num_pages) page_row = page * p.page_size + key % p.page_size;
-        }
-      }
-#pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        constexpr int ST[2] = {C::KST, C::VST}, OFF[2] = {C::OFF_K, C::OFF_V}, FULL[2] = {K_FULL, V_FULL}, EMPTY[2] = {K_EMPTY, V_EMPTY};
-        const int st = j % ST[kv];
-        const bool ok = mbar_wait_all(BAR(EMPTY[kv] + st), ((j / ST[kv]) & 1) ^ 1, abort_flag);
-        if (!ok) {
-          j = n;
-          break;
-        }
-        const uint32_t bar = BAR(FULL[kv] + st), dst = sbase + OFF[kv] + st * C::TILE_BYTES;
-        if (leader) mbar_arrive_expect_tx(bar, C::TILE_BYTES);
-        if (drafts) {
-          if (leader) {
-#pragma unroll
-            for (int s = 0; s < C::SUB; ++s)
-              tma_load_4d(dst + s * 128 * 128, kv ? &tm_vn : &tm_kn, bar, s * 64, hk, (tile - prefix_tiles) * BN, b);
+          tma_load_5d(sbase + C::OFF_Q + t * C::TILE_BYTES + s * 128 * 128, &tm_q, BAR(Q_FULL), s * 64, 0, w.hk, w.t0 + t * geo.tokens, w.b);
+    };
+    for (int64_t pos = start; ok && next(pos, w); ++seg) {
+      // The first key tiles of a later segment are fetched before its queries, whose place is still in use.
+      const int ahead = seg == 0 ? 0 : min(w.n, min(C::KST, C::VST));
+      for (int j = 0; ok && j < w.n; ++j, ++g) {
+        if (j == ahead) load_q();
+        const int tile = w.first + j;
+        const bool drafts = tile >= w.prefix_tiles;
+        const int key0 = tile * BN;
+        int page_row = p.num_pages * p.page_size;  // lane i: pool row of box i of the tile; past the pool: zeros
+        if (p.block_table && !drafts) {
+          const int key = key0 + lane * geo.box_rows;
+          if (lane < boxes && key < w.prefix) {
+            const int page = p.block_table[(int64_t)w.b * p.max_pages + key / p.page_size];
+            if (page >= 0 && page < p.num_pages) page_row = page * p.page_size + key % p.page_size;
           }
-        } else if (!p.block_table) {
-          if (leader) {
+        }
 #pragma unroll
-            for (int s = 0; s < C::SUB; ++s) tma_load_4d(dst + s * 128 * 128, kv ? &tm_v : &tm_k, bar, s * 64, hk, key0, b);
-          }
-        } else {
-          for (int i = 0; i < boxes; ++i) {
-            const int row = __shfl_sync(0xffffffffu, page_row, i);
+        for (int kv = 0; kv < 2; ++kv) {
+          constexpr int ST[2] = {C::KST, C::VST}, OFF[2] = {C::OFF_K, C::OFF_V}, FULL[2] = {K_FULL, V_FULL}, EMPTY[2] = {K_EMPTY, V_EMPTY};
+          const int st = g % ST[kv];
+          ok = ok && mbar_wait_all(BAR(EMPTY[kv] + st), ((g / ST[kv]) & 1) ^ 1, abort_flag);
+          if (!ok) break;
+          const uint32_t bar = BAR(FULL[kv] + st), dst = sbase + OFF[kv] + st * C::TILE_BYTES;
+          if (leader) mbar_arrive_expect_tx(bar, C::TILE_BYTES);
+          if (drafts) {
             if (leader) {
 #pragma unroll
               for (int s = 0; s < C::SUB; ++s)
-                tma_load_4d(dst + s * 128 * 128 + i * geo.box_rows * 128, kv ? &tm_v : &tm_k, bar, s * 64, hk, row, 0);
+                tma_load_4d(dst + s * 128 * 128, kv ? &tm_vn : &tm_kn, bar, s * 64, w.hk, (tile - w.prefix_tiles) * BN, w.b);
+            }
+          } else if (!p.block_table) {
+            if (leader) {
+#pragma unroll
+              for (int s = 0; s < C::SUB; ++s) tma_load_4d(dst + s * 128 * 128, kv ? &tm_v : &tm_k, bar, s * 64, w.hk, key0, w.b);
+            }
+          } else {
+            for (int i = 0; i < boxes; ++i) {
+              const int row = __shfl_sync(0xffffffffu, page_row, i);
+              if (leader) {
+#pragma unroll
+                for (int s = 0; s < C::SUB; ++s)
+                  tma_load_4d(dst + s * 128 * 128 + i * geo.box_rows * 128, kv ? &tm_v : &tm_k, bar, s * 64, w.hk, row, 0);
+              }
             }
           }
         }
       }
+      if (ok && ahead == w.n) load_q();  // (a short segment: its keys went first)
     }
   } else if (warp == 1) {
     // -------------------------------------------------------------- MMA issuer
     const uint32_t leader = elect_leader();
     constexpr uint32_t idesc_s = make_idesc(128, BN, BF16, false, false);
     constexpr uint32_t idesc_o = make_idesc(128, HD, BF16, false, true);
-    auto issue_s = [&](int t, int j) {  // scores of key tile j into buffer t
+    int g = 0, seg = 0, cleaned = 0;  // tiles before this segment, segments, tiles handed to the clearing warp
+    int p_done[2] = {0, 0};           // P tiles of each group so far
+    bool ok = true;
+    Work w = {};
+    auto issue_s = [&](int t, int j) {  // scores of the segment's key tile j into buffer t
       const uint32_t qa = sbase + C::OFF_Q + (ROWS == 2 ? t : 0) * C::TILE_BYTES;
-      const uint32_t ka = sbase + C::OFF_K + (j % C::KST) * C::TILE_BYTES;
+      const uint32_t ka = sbase + C::OFF_K + ((g + j) % C::KST) * C::TILE_BYTES;
 #pragma unroll
       for (int s = 0; s < C::SUB; ++s)
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
           mma_ss(tmem + t * BN, make_smem_desc(qa + s * 128 * 128 + kk * 32, 16, 1024),
                  make_smem_desc(ka + s * 128 * 128 + kk * 32, 16, 1024), idesc_s, (s | kk) != 0, leader);
+      mma_commit(BAR(S_FULL + t), leader);
     };
     auto issue_pv = [&](int t, int j, bool fresh) {
-      const uint32_t va = sbase + C::OFF_V + (j % C::VST) * C::TILE_BYTES;
+      const uint32_t va = sbase + C::OFF_V + ((g + j) % C::VST) * C::TILE_BYTES;
 #pragma unroll
       for (int kk = 0; kk < BN / 16; ++kk)
         mma_ts(tmem + 2 * BN + t * HD, tmem + t * BN + kk * 8, make_smem_desc(va + kk * 2048, 128 * 128, 1024), idesc_o,
                !fresh || kk != 0, leader);
     };
-    auto wait_k = [&](int j) { return mbar_wait_all(BAR(K_FULL + j % C::KST), (j / C::KST) & 1, abort_flag); };
-    auto wait_v = [&](int j) {
-      bool ok = mbar_wait_all(BAR(V_FULL + j % C::VST), (j / C::VST) & 1, abort_flag);
-      if (ok && j >= clean0) {
-        if (leader) mbar_arrive(BAR(V_LANDED + j - clean0));
-        ok = mbar_wait_all(BAR(V_CLEAN + j - clean0), 0, abort_flag);
-      }
-      return ok;
+    auto wait_k = [&](int j) {
+      const bool there = mbar_wait_all(BAR(K_FULL + (g + j) % C::KST), ((g + j) / C::KST) & 1, abort_flag);
+      tc_fence_after();
+      return there;
     };
-    bool ok = mbar_wait_all(BAR(Q_FULL), 0, abort_flag);
-    if constexpr (ROWS == 1) {
-      for (int j = 0; ok && j < min(2, n); ++j) {
-        ok = wait_k(j);
-        if (!ok) break;
-        tc_fence_after();
-        issue_s(j, j);
-        mma_commit(BAR(S_FULL + j), leader);
-        mma_commit(BAR(K_EMPTY + j % C::KST), leader);
+    auto free_k = [&](int j) { mma_commit(BAR(K_EMPTY + (g + j) % C::KST), leader); };
+    auto wait_v = [&](int j) {
+      bool there = mbar_wait_all(BAR(V_FULL + (g + j) % C::VST), ((g + j) / C::VST) & 1, abort_flag);
+      if (there && j >= w.clean0) {
+        if (leader) mbar_arrive(BAR(V_LANDED));
+        there = mbar_wait_all(BAR(V_CLEAN), cleaned++ & 1, abort_flag);
       }
-      for (int j = 0; ok && j < n; ++j) {
-        const int t = j & 1;
-        ok = wait_v(j) && mbar_wait_all(BAR(P_FULL + t), (j >> 1) & 1, abort_flag);
-        if (!ok) break;
-        tc_fence_after();
-        issue_pv(t, j, j < 2);
-        mma_commit(BAR(V_EMPTY + j % C::VST), leader);
-        if (j == n - 1) mma_commit(BAR(O_DONE), leader);
-        if (j + 2 < n) {
-          ok = wait_k(j + 2);
-          if (!ok) break;
-          tc_fence_after();
-          issue_s(t, j + 2);
-          mma_commit(BAR(S_FULL + t), leader);
-          mma_commit(BAR(K_EMPTY + (j + 2) % C::KST), leader);
+      return there;
+    };
+    auto wait_p = [&](int t) {
+      const bool there = mbar_wait_all(BAR(P_FULL + t), p_done[t]++ & 1, abort_flag);
+      tc_fence_after();
+      return there;
+    };
+    for (int64_t pos = start; ok && next(pos, w); ++seg, g += w.n) {
+      const int n = w.n;
+      ok = mbar_wait_all(BAR(Q_FULL), seg & 1, abort_flag);
+      if constexpr (ROWS == 1) {
+        for (int j = 0; ok && j < min(2, n); ++j) {
+          if (!(ok = wait_k(j))) break;
+          issue_s(j, j);
+          free_k(j);
         }
-      }
-    } else {
-      if (ok) ok = wait_k(0);
-      if (ok) {
-        tc_fence_after();
-        issue_s(0, 0);
-        mma_commit(BAR(S_FULL), leader);
-        issue_s(1, 0);
-        mma_commit(BAR(S_FULL + 1), leader);
-        mma_commit(BAR(K_EMPTY), leader);
-      }
-      for (int j = 0; ok && j < n; ++j) {
-        const bool more = j + 1 < n;
-        ok = wait_v(j) && (!more || wait_k(j + 1));
-        if (!ok) break;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          ok = ok && mbar_wait_all(BAR(P_FULL + t), j & 1, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          issue_pv(t, j, j == 0);
-          if (more) {
-            issue_s(t, j + 1);
-            mma_commit(BAR(S_FULL + t), leader);
+        for (int j = 0; ok && j < n; ++j) {
+          const int t = j & 1;
+          if (!(ok = wait_v(j) && wait_p(t))) break;
+          issue_pv(t, j, j < 2);
+          mma_commit(BAR(V_EMPTY + (g + j) % C::VST), leader);
+          if (j + 2 < n) {
+            if (!(ok = wait_k(j + 2))) break;
+            issue_s(t, j + 2);
+            free_k(j + 2);
           }
         }
-        if (!ok) break;
-        mma_commit(BAR(V_EMPTY + j % C::VST), leader);
-        if (more)
-          mma_commit(BAR(K_EMPTY + (j + 1) % C::KST), leader);
-        else
-          mma_commit(BAR(O_DONE), leader);
+      } else {
+        if (ok && (ok = wait_k(0))) {
+          issue_s(0, 0);
+          issue_s(1, 0);
+          free_k(0);
+        }
+        for (int j = 0; ok && j < n; ++j) {
+          const bool more = j + 1 < n;
+          if (!(ok = wait_v(j) && (!more || wait_k(j + 1)))) break;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (!(ok = ok && wait_p(t))) break;
+            issue_pv(t, j, j == 0);
+            if (more) issue_s(t, j + 1);
+          }
+          if (!ok) break;
+          mma_commit(BAR(V_EMPTY + (g + j) % C::VST), leader);
+          if (more) free_k(j + 1);
+        }
       }
+      if (ok) mma_commit(BAR(O_DONE), leader);
     }
   } else if (warp == 10) {
     // ------------------------------------------- values of keys that nobody sees
-    // (told by the issuer, which follows the V ring: a wait for one late phase of V_FULL alone would pass at once)
-    for (int j = clean0; j < n; ++j) {
-      const int tile = first + j, st = j % C::VST;
-      if (mbar_wait(BAR(V_LANDED + j - clean0), 0, abort_flag)) {
+    // (told by the issuer, which follows the V ring; the two take turns)
+    int g = 0, cleaned = 0;
+    bool ok = true;
+    Work w = {};
+    for (int64_t pos = start; ok && next(pos, w); g += w.n) {
+      const int32_t* parents = p.parents + w.b * p.parents_bs;
+      for (int j = w.clean0; ok && j < w.n; ++j, ++cleaned) {
+        const int tile = w.first + j, st = (g + j) % C::VST;
+        ok = mbar_wait_all(BAR(V_LANDED), cleaned & 1, abort_flag);
+        if (!ok) break;
         bool wrote = false;
         for (int r = lane; r < BN; r += 32) {
-          const int node = (tile - prefix_tiles) * BN + r;  // (drafts past the last one arrive as zeros)
-          const bool seen = tile < prefix_tiles ? tile * BN + r < prefix : node >= p.N || tree_present(par, node);
+          const int node = (tile - w.prefix_tiles) * BN + r;  // (drafts past the last one arrive as zeros)
+          const bool seen = tile < w.prefix_tiles ? tile * BN + r < w.prefix : node >= p.N || tree_present(parents, node);
           if (seen) continue;
           wrote = true;
           const uint32_t row = sbase + C::OFF_V + st * C::TILE_BYTES + r * 128;
@@ -303,182 +329,221 @@ attn_tree_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
               asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(row + s * 128 * 128 + u * 16), "r"(0) : "memory");
         }
         if (wrote) fence_proxy_async();
+        mbar_arrive(BAR(V_CLEAN));
       }
-      mbar_arrive(BAR(V_CLEAN + j - clean0));
     }
   } else {
     // ------------------------------------------------------------ softmax warps
     const int t = (warp - 2) >> 2;
     const int quarter = warp & 3;  // tensor-memory lane quarter this warp may access
     const int r_in = quarter * 32 + lane;
-    const int node = t0 + (ROWS == 2 ? t * geo.tokens : 0) + r_in / G;
-    const bool there = r_in < geo.tokens * G && node < p.N && tree_present(par, node);
     const uint32_t lane_sel = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_addr = tmem + lane_sel + t * BN;
     const uint32_t o_addr = tmem + lane_sel + 2 * BN + t * HD;
     const float c1 = p.sm_scale * kLog2e;
     constexpr int STEP = ROWS == 1 ? 2 : 1;
-    float m_ref = -INFINITY, l = 0.f;
+    // The segment lives in shared memory: the registers hold the scores of a row and little else.
+    struct Held {
+      int b, t0, first, prefix, prefix_tiles;
+      int64_t slot, pos;
+    };
+    static_assert(sizeof(Held) <= 64, "a warp's slot");
+    volatile Held* held = reinterpret_cast<volatile Held*>(smem + C::OFF_WORK + (warp - 2) * 64);
+    int it = 0, seg = 0, met = 0;  // score tiles of this group so far, segments, meetings
     bool ok = true;
-    int it = 0;
-    for (int j = ROWS == 1 ? t : 0; j < n; j += STEP, ++it) {
-      ok = mbar_wait(BAR(S_FULL + t), it & 1, abort_flag);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      tc_fence_after();
-      float s[BN];
+    auto meet = [&] {
+      const uint32_t bar = BAR(MEET + (ROWS == 1 ? 0 : t));
+      mbar_arrive(bar);
+      const bool there = mbar_wait(bar, met++ & 1, abort_flag);
+      ok = __all_sync(0xffffffffu, there) && ok;
+    };
+    auto next_held = [&](int& n, int& clean0) {
+      Work w;
+      int64_t pos = seg == 0 ? start : held->pos;
+      if (!next(pos, w)) return false;
+      __syncwarp();
+      if (lane == 0) {
+        held->b = w.b;
+        held->t0 = w.t0;
+        held->first = w.first;
+        held->prefix = w.prefix;
+        held->prefix_tiles = w.prefix_tiles;
+        held->slot = w.slot;
+        held->pos = pos;
+      }
+      __syncwarp();
+      n = w.n;
+      clean0 = w.clean0;
+      return true;
+    };
+    int n, clean0;
+    for (; ok && next_held(n, clean0); ++seg) {
+      float m_ref = -INFINITY, l = 0.f;
+      bool any = false;  // this group has accumulated a tile of the segment
+      for (int j = ROWS == 1 ? t : 0; j < n; j += STEP, ++it) {
+        ok = mbar_wait(BAR(S_FULL + t), it & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        float s[BN];
 #pragma unroll
-      for (int c = 0; c < BN / 32; ++c) tmem_ld32f(s_addr + c * 32, &s[c * 32]);
-      tmem_wait_ld();
-      const int tile = first + j;
-      if (j >= clean0) {  // keep bits of the tile's 128 keys
-        uint32_t bits[4];
-        if (tile < prefix_tiles) {
-          const int valid = prefix - tile * BN;
+        for (int c = 0; c < BN / 32; ++c) tmem_ld32f(s_addr + c * 32, &s[c * 32]);
+        tmem_wait_ld();
+        if (j >= clean0) {  // keep bits of the tile's 128 keys
+          const int tile = held->first + j;
+          uint32_t bits[4];
+          if (tile < held->prefix_tiles) {
+            const int valid = held->prefix - tile * BN;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int k = valid - 32 * c;
-            bits[c] = k >= 32 ? 0xffffffffu : k <= 0 ? 0u : (1u << k) - 1u;
-          }
-        } else {
-          const int node0 = (tile - prefix_tiles) * BN;
-          uint32_t b0 = 0, b1 = 0, b2 = 0, b3 = 0;
-          if (there) {
-            for (int i = node; i >= node0; i = par[i]) {
+            for (int c = 0; c < 4; ++c) {
+              const int k = valid - 32 * c;
+              bits[c] = k >= 32 ? 0xffffffffu : k <= 0 ? 0u : (1u << k) - 1u;
+            }
+          } else {
+            const int node0 = (tile - held->prefix_tiles) * BN;
+            const int32_t* parents = p.parents + held->b * p.parents_bs;
+            uint32_t b0 = 0, b1 = 0, b2 = 0, b3 = 0;
+            const int node = held->t0 + (ROWS == 2 ? t * geo.tokens : 0) + r_in / G;
+            int i = r_in < geo.tokens * G && node < p.N ? node : -1;
+            while (i >= 0) {
               const int k = i - node0;
               const uint32_t bit = 1u << (k & 31);
-              if (k < 32) b0 |= bit;
-              else if (k < 64) b1 |= bit;
-              else if (k < 96) b2 |= bit;
-              else if (k < 128) b3 |= bit;
+              b0 |= k >= 0 && k < 32 ? bit : 0u;
+              b1 |= k >= 32 && k < 64 ? bit : 0u;
+              b2 |= k >= 64 && k < 96 ? bit : 0u;
+              b3 |= k >= 96 && k < 128 ? bit : 0u;
+              i = tree_parent(parents, i);
             }
+            if (i != -1) b0 = b1 = b2 = b3 = 0;  // absent: sees nothing (and the combine drops its row)
+            bits[0] = b0; bits[1] = b1; bits[2] = b2; bits[3] = b3;
           }
-          bits[0] = b0; bits[1] = b1; bits[2] = b2; bits[3] = b3;
+#pragma unroll
+          for (int i = 0; i < BN; ++i) s[i] = (bits[i / 32] >> (i % 32)) & 1u ? s[i] : -INFINITY;
         }
+        float mx;
+        {
+          float m[8];  // independent chains
 #pragma unroll
-        for (int i = 0; i < BN; ++i) s[i] = (bits[i / 32] >> (i % 32)) & 1u ? s[i] : -INFINITY;
-      }
-      float mx;
-      {
-        float m[8];  // independent chains
+          for (int i = 0; i < 8; ++i) m[i] = fmaxf(s[2 * i], s[2 * i + 1]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m[i] = fmaxf(s[2 * i], s[2 * i + 1]);
+          for (int i = 1; i < BN / 16; ++i)
 #pragma unroll
-        for (int i = 1; i < BN / 16; ++i)
-#pragma unroll
-          for (int u = 0; u < 8; ++u) m[u] = fmax3(m[u], s[16 * i + 2 * u], s[16 * i + 2 * u + 1]);
-        mx = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), fmaxf(fmaxf(m[4], m[5]), fmaxf(m[6], m[7])));
-      }
-      mx *= c1;  // c1 > 0
-      // lazy running maximum: advance only when it grew by more than 8 (base 2)
-      const bool need = (mx > m_ref + 8.f) || (m_ref == -INFINITY && mx > -INFINITY);
-      const bool rescale = __any_sync(0xffffffffu, need);
-      float corr = 1.f;
-      if (rescale) {
-        const float m_new = fmaxf(m_ref, mx);
-        corr = (m_new == -INFINITY) ? 1.f : exp2f(m_ref - m_new);
-        m_ref = m_new;
-        l *= corr;
-      }
-      const float neg_m = (m_ref == -INFINITY) ? 0.f : -m_ref;
-      float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
-      exp_pack_store<BN, BF16>(s, make_float2(c1, c1), make_float2(neg_m, neg_m), sum0, sum1, s_addr);
-      const float lsum = (sum0.x + sum0.y) + (sum1.x + sum1.y);
-      // the group's previous P.V completed before these scores became visible
-      if (rescale && it > 0) {
-#pragma unroll
-        for (int c = 0; c < HD / 32; ++c) {
-          float o[32];
-          tmem_ld32f(o_addr + c * 32, o);
-          tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] *= corr;
-          tmem_st32f(o_addr + c * 32, o);
+            for (int u = 0; u < 8; ++u) m[u] = fmax3(m[u], s[16 * i + 2 * u], s[16 * i + 2 * u + 1]);
+          mx = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), fmaxf(fmaxf(m[4], m[5]), fmaxf(m[6], m[7])));
         }
-      }
-      l += lsum;
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(BAR(P_FULL + t));
-    }
-    ok = ok && mbar_wait(BAR(O_DONE), 0, abort_flag);
-    ok = __all_sync(0xffffffffu, ok);
-    tc_fence_after();
-    // All products are done and all loads have landed: the rings are free.  The rows leave through shared memory, 16-byte units
-    // swizzled by row, so that whole rows are written.
-    const int rows = p.N * G;
-    const int64_t part = ((int64_t)hk * p.splits + x) * rows;
-    const int token0 = t0 + (ROWS == 2 ? t * geo.tokens : 0);
-    const int n_rows = min(geo.tokens, p.N - token0) * G;  // rows of the tile that exist (may be none)
-    const uint32_t stage = sbase + C::OFF_K + (ROWS == 2 ? t : 0) * (128 * HD * 4);
-    const uint32_t my_row = stage + r_in * (HD * 4);
-    const bool mine = ROWS == 2 || t == 0;
-    float* ml = reinterpret_cast<float*>(smem + C::OFF_ML);
-    if constexpr (ROWS == 1) {
-      if (t == 1) {  // the odd tiles' state
-        ml[2 * r_in] = m_ref;
-        ml[2 * r_in + 1] = l;
-        if (it > 0 && ok) {
+        mx *= c1;  // c1 > 0
+        // lazy running maximum: advance only when it grew by more than 8 (base 2)
+        const bool need = (mx > m_ref + 8.f) || (m_ref == -INFINITY && mx > -INFINITY);
+        const bool rescale = __any_sync(0xffffffffu, need);
+        float corr = 1.f;
+        if (rescale) {
+          const float m_new = fmaxf(m_ref, mx);
+          corr = (m_new == -INFINITY) ? 1.f : exp2f(m_ref - m_new);
+          m_ref = m_new;
+          l *= corr;
+        }
+        const float neg_m = (m_ref == -INFINITY) ? 0.f : -m_ref;
+        float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
+        exp_pack_store<BN, BF16>(s, make_float2(c1, c1), make_float2(neg_m, neg_m), sum0, sum1, s_addr);
+        const float lsum = (sum0.x + sum0.y) + (sum1.x + sum1.y);
+        // the group's previous P.V completed before these scores became visible
+        if (rescale && any) {
 #pragma unroll
           for (int c = 0; c < HD / 32; ++c) {
             float o[32];
             tmem_ld32f(o_addr + c * 32, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              st_shared4(my_row + (((c * 8 + i) ^ (r_in & 7)) << 4), o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            for (int i = 0; i < 32; ++i) o[i] *= corr;
+            tmem_st32f(o_addr + c * 32, o);
           }
         }
+        l += lsum;
+        any = true;
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(BAR(P_FULL + t));
       }
-      asm volatile("bar.sync 1, 256;\n" ::: "memory");
-    }
-    if (mine && ok) {
-      float wa = 1.f, wb = 0.f, m = m_ref, lsum = l;
-      if constexpr (ROWS == 1) {
-        const float m1 = ml[2 * r_in], l1 = ml[2 * r_in + 1];
-        m = fmaxf(m_ref, m1);
-        wa = m_ref == -INFINITY ? 0.f : exp2f(m_ref - m);
-        wb = m1 == -INFINITY ? 0.f : exp2f(m1 - m);
-        lsum = l * wa + l1 * wb;
+      ok = ok && mbar_wait(BAR(O_DONE), seg & 1, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+      // All products of the segment are done and Q is dead.  The rows leave through Q's shared memory, half a row (HD / 2 floats) at a
+      // time, 16-byte units swizzled by row, so that whole lines are written; the rings go on loading.
+      constexpr int HALF = HD / 2, UNITS = HALF / 4;
+      const int tile_rows = geo.tokens * G;
+      const int token0 = held->t0 + (ROWS == 2 ? t * geo.tokens : 0);
+      const int n_rows = min(geo.tokens, p.N - token0) * G;  // rows of the tile that exist (may be none)
+      const int64_t part = held->slot * p.column_rows + (ROWS == 2 ? t * tile_rows : 0);
+      const uint32_t stage = sbase + C::OFF_Q + (ROWS == 2 ? t : 0) * C::TILE_BYTES;
+      const uint32_t my_row = stage + r_in * (HALF * 4);
+      const bool writer = ROWS == 2 || t == 0;
+      float* ml = reinterpret_cast<float*>(smem + C::OFF_ML);
+      if (ROWS == 1 && t == 1) {  // the odd tiles' state
+        ml[2 * r_in] = m_ref;
+        ml[2 * r_in + 1] = l;
       }
-      const bool keep = there && lsum > 0.f;
-      const float inv = keep ? 1.f / lsum : 0.f;
+      float wa = 1.f, wb = 0.f, inv = 0.f;
 #pragma unroll
-      for (int c = 0; c < HD / 32; ++c) {
-        float o[32];
-        tmem_ld32f(o_addr + c * 32, o);
-        tmem_wait_ld();
+      for (int half = 0; half < 2; ++half) {
+        if constexpr (ROWS == 1) {
+          if (t == 1 && any && ok) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t at = my_row + (((c * 8 + i) ^ (r_in & 7)) << 4);
-          float4 v = make_float4(o[4 * i] * wa, o[4 * i + 1] * wa, o[4 * i + 2] * wa, o[4 * i + 3] * wa);
-          if (ROWS == 1 && wb != 0.f) {
-            const float4 w = ld_shared4(at);
-            v = make_float4(fmaf(w.x, wb, v.x), fmaf(w.y, wb, v.y), fmaf(w.z, wb, v.z), fmaf(w.w, wb, v.w));
+            for (int c = 0; c < HALF / 32; ++c) {
+              float o[32];
+              tmem_ld32f(o_addr + half * HALF + c * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                st_shared4(my_row + (((c * 8 + i) ^ (r_in & 7)) << 4), o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            }
           }
-          if (keep)
-            st_shared4(at, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-          else
-            st_shared4(at, 0.f, 0.f, 0.f, 0.f);
+          meet();
         }
+        if (writer && ok) {
+          if (half == 0) {
+            float m = m_ref, lsum = l;
+            if constexpr (ROWS == 1) {
+              const float m1 = ml[2 * r_in], l1 = ml[2 * r_in + 1];
+              m = fmaxf(m_ref, m1);
+              wa = m_ref == -INFINITY ? 0.f : exp2f(m_ref - m);
+              wb = m1 == -INFINITY ? 0.f : exp2f(m1 - m);
+              lsum = l * wa + l1 * wb;
+            }
+            inv = lsum > 0.f ? 1.f / lsum : 0.f;
+            if (r_in < n_rows) p.lse_part[part + r_in] = lsum > 0.f ? m + log2f(lsum) : -INFINITY;
+          }
+#pragma unroll
+          for (int c = 0; c < HALF / 32; ++c) {
+            float o[32];
+            tmem_ld32f(o_addr + half * HALF + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const uint32_t at = my_row + (((c * 8 + i) ^ (r_in & 7)) << 4);
+              float4 v = make_float4(o[4 * i] * wa, o[4 * i + 1] * wa, o[4 * i + 2] * wa, o[4 * i + 3] * wa);
+              if (ROWS == 1 && wb != 0.f) {
+                const float4 u = ld_shared4(at);
+                v = make_float4(fmaf(u.x, wb, v.x), fmaf(u.y, wb, v.y), fmaf(u.z, wb, v.z), fmaf(u.w, wb, v.w));
+              }
+              st_shared4(at, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+            }
+          }
+        }
+        meet();
+        if (ok) {
+          constexpr int THREADS = ROWS == 1 ? 256 : 128;
+          const int tid = (ROWS == 1 ? t * 128 : 0) + r_in;
+          float* out = p.o_part + part * HD + half * HALF;
+          for (int i = tid; i < n_rows * UNITS; i += THREADS) {
+            const int r = i / UNITS, u = i % UNITS;
+            *reinterpret_cast<float4*>(out + (int64_t)r * HD + u * 4) = ld_shared4(stage + r * (HALF * 4) + ((u ^ (r & 7)) << 4));
+          }
+        }
+        if (half == 0) meet();  // (the second half goes where the first one lay)
       }
-      if (r_in < n_rows) p.lse_part[part + (int64_t)token0 * G + r_in] = keep ? m + log2f(lsum) : -INFINITY;
-    }
-    if constexpr (ROWS == 1)
-      asm volatile("bar.sync 1, 256;\n" ::: "memory");
-    else if (t == 0)
-      asm volatile("bar.sync 1, 128;\n" ::: "memory");
-    else
-      asm volatile("bar.sync 2, 128;\n" ::: "memory");
-    if (ok) {
-      constexpr int UNITS = HD / 4, THREADS = ROWS == 1 ? 256 : 128;
-      const int tid = ROWS == 1 ? t * 128 + (warp - 2 - 4 * t) * 32 + lane : (warp - 2 - 4 * t) * 32 + lane;
-      float* out = p.o_part + (part + (int64_t)token0 * G) * HD;
-      for (int i = tid; i < n_rows * UNITS; i += THREADS) {
-        const int r = i / UNITS, u = i % UNITS;
-        const float4 v = ld_shared4(stage + r * (HD * 4) + ((u ^ (r & 7)) << 4));
-        *reinterpret_cast<float4*>(out + (int64_t)r * HD + u * 4) = v;
-      }
+      fence_proxy_async();  // the queries of the next segment are written here by TMA
+      tc_fence_before();
+      mbar_arrive(BAR(Q_FREE));
     }
   }
 
@@ -490,13 +555,18 @@ attn_tree_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   }
 }
 
+// Query tokens of a row tile.
+int tree_tokens(const TreeParams& p) {
+  const int most = 128 / (p.Hq / p.Hkv);
+  return most < p.N ? most : p.N;
+}
+
 template <int HD, bool BF16, int ROWS>
 int launch_t(const TreeParams& p, int dtype, cudaStream_t stream) {
   using C = Cfg<HD, ROWS>;
   const int G = p.Hq / p.Hkv;
   TreeGeometry geo;
-  geo.tokens = 128 / G < p.N ? 128 / G : p.N;
-  geo.row_tiles = (p.N + ROWS * geo.tokens - 1) / (ROWS * geo.tokens);
+  geo.tokens = tree_tokens(p);
   geo.box_rows = BN;
   while (p.block_table && p.page_size % geo.box_rows) geo.box_rows /= 2;
   int rc = bind_context();
@@ -527,15 +597,14 @@ int launch_t(const TreeParams& p, int dtype, cudaStream_t stream) {
   auto kern = attn_tree_sm100_kernel<HD, BF16, ROWS>;
   if ((rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES), "cudaFuncSetAttribute(tree)")))
     return rc;
-  kern<<<(unsigned)((int64_t)p.splits * p.Hkv * geo.row_tiles), NTHREADS, C::SMEM_BYTES, stream>>>(tq, tk, tv, tkn, tvn, p, geo);
+  kern<<<p.ctas, NTHREADS, C::SMEM_BYTES, stream>>>(tq, tk, tv, tkn, tvn, p, geo);
   count_launch();
   return check_cuda(cudaGetLastError(), "tree attention launch");
 }
 
 template <int HD, bool BF16>
 int launch_rows(const TreeParams& p, int dtype, cudaStream_t stream) {
-  const int G = p.Hq / p.Hkv;
-  return p.N > 128 / G ? launch_t<HD, BF16, 2>(p, dtype, stream) : launch_t<HD, BF16, 1>(p, dtype, stream);
+  return p.N > tree_tokens(p) ? launch_t<HD, BF16, 2>(p, dtype, stream) : launch_t<HD, BF16, 1>(p, dtype, stream);
 }
 
 }  // namespace
@@ -554,9 +623,15 @@ bool tree_sm100_supported(const TreeParams& p, int dtype, const char** why) {
             reinterpret_cast<uintptr_t>(p.k_new) | reinterpret_cast<uintptr_t>(p.v_new)) & 15)
     w = "addresses must be 16-byte aligned";
   else if (p.block_table && (int64_t)p.num_pages * p.page_size >= 0x7fffffff) w = "a pool of fewer than 2^31 rows";
-  else if ((int64_t)p.splits * p.Hkv * p.N > 0x7fffffffLL) w = "grid too large";
   if (why) *why = w;
   return w == nullptr;
+}
+
+void tree_sm100_geometry(TreeParams& p) {
+  const int tokens = tree_tokens(p), rows = p.N > tokens ? 2 : 1;
+  p.column_rows = rows * tokens * (p.Hq / p.Hkv);
+  p.columns = p.Hkv * ((p.N + rows * tokens - 1) / (rows * tokens));
+  p.ctas = 148;  // one CTA per SM
 }
 
 int launch_tree_sm100(const TreeParams& p, int dtype, cudaStream_t stream) {

@@ -309,11 +309,11 @@ struct TreeParams {
   int page_size, max_pages, num_pages;
   void* o;            // [B, N, Hq, Dv]
   float* lse;         // [B, Hq, N] or null
-  float* o_part;      // [Hkv, splits, N * G, Dv] fp32, rows (t, g)
-  float* lse_part;    // [Hkv, splits, N * G] base 2, -inf for a split without keys
+  float* o_part;      // [slots, column_rows, Dv] fp32, normalised by the segment's own sum
+  float* lse_part;    // [slots, column_rows] base 2, -inf where the segment holds no key of the row
   int B, N, Hq, Hkv, D, Dv, capacity;
-  int splits;         // splits of the whole batch (grid x)
-  int per_seq;        // > 0: that many splits for every sequence; 0: dealt out on the device from the lengths
+  // A column is a tile of `column_rows` packed rows (t, g) of one KV head; see tree_plan.cuh.
+  int column_rows, columns, ctas;
   float sm_scale;
   int32_t* status;
 };

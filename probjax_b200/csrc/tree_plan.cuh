@@ -1,24 +1,19 @@
-// What the kernels of the tree attention share: the drafts' tree, and how the tiles of a ragged batch are dealt to CTAs.
+// What the kernels of the tree attention share: the drafts' tree, and how the work of a ragged batch is dealt to the CTAs.
 #pragma once
 
 #include "pjx_common.cuh"
 
 namespace pjx {
 
-// Parents of the drafts into `par` [N]: -1 hangs on the context, 0 <= parent < own index on a draft; everything else is absent
-// (-2).  All threads of the CTA take part; one barrier.
-__device__ __forceinline__ void load_tree(const TreeParams& p, int b, int16_t* par, int tid, int n_threads) {
-  const int32_t* src = p.parents + b * p.parents_bs;
-  for (int i = tid; i < p.N; i += n_threads) {
-    const int v = src[i];
-    par[i] = (int16_t)(v >= -1 && v < i ? v : -2);
-  }
-  __syncthreads();
+// Parent of draft i: -1 hangs on the context, 0 <= parent < i on that draft, everything else is absent (-2).
+__device__ __forceinline__ int tree_parent(const int32_t* parents, int i) {
+  const int v = __ldg(parents + i);
+  return v >= -1 && v < i ? v : -2;
 }
 // Whether draft i hangs on the context: what hangs on an absent draft is absent too.  Parents come before their children, so the
 // walk ends.
-__device__ __forceinline__ bool tree_present(const int16_t* par, int i) {
-  while (i >= 0) i = par[i];
+__device__ __forceinline__ bool tree_present(const int32_t* parents, int i) {
+  while (i >= 0) i = tree_parent(parents, i);
   return i == -1;
 }
 
@@ -27,105 +22,68 @@ __device__ __forceinline__ int tree_tiles(const TreeParams& p, int prefix) {
   return (prefix + kTreeTile - 1) / kTreeTile + (p.N + kTreeTile - 1) / kTreeTile;
 }
 
-// Splits of the batch: every split is a run of at most `unit` tiles of one sequence, numbered through the batch.  With per_seq > 0 every
-// sequence has that many; otherwise `unit` is the smallest (up to a sixteenth) with which the batch has no more than p.splits.
-// Computed by whole warps.
-constexpr int kTreePlanSeqs = 128;  // sequences that are dealt out on the device: four per lane
-struct TreeSplit {
-  int b;          // sequence, -1: none
-  int prefix;     // its cached keys
-  int first, end; // tiles
+// The work is a line: for every column (a tile of query rows of one KV head) all key tiles of all sequences.  It is cut into
+// equal runs, one per CTA, so that a ragged batch balances without knowing the lengths on the host, and a CTA's run falls into segments
+// of one column and sequence.  Every segment leaves a partial result in a slot of its own: from one segment to the next on the line
+// either the CTA or the (column, sequence) pair moves on by one, so their sum numbers the slots.
+// All functions are computed by whole warps.
+struct TreeLine {
+  int tiles;       // key tiles of the batch
+  int64_t length;  // tiles of all columns
+  int ctas;        // CTAs that have work
 };
-struct TreePlan {
-  int unit;
-  int n[kTreePlanSeqs / 32], first[kTreePlanSeqs / 32];
-};
-__device__ __forceinline__ TreePlan tree_plan(const TreeParams& p) {
-  constexpr int PER = kTreePlanSeqs / 32;
+__device__ __forceinline__ TreeLine tree_line(const TreeParams& p) {
   const int lane = threadIdx.x & 31;
-  TreePlan r;
-  int tiles[PER], total = 0;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int b = lane + 32 * i;
-    tiles[i] = b < p.B ? tree_tiles(p, tree_prefix(p, b)) : 0;
-    total += tiles[i];
-  }
-  total = __reduce_add_sync(0xffffffffu, total);
-  r.unit = max(1, (total + p.splits - 1) / p.splits);
-  while (true) {  // ends: p.splits >= B, and the longest sequence's tiles as the unit give one split each
-    int cnt = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      r.n[i] = (tiles[i] + r.unit - 1) / r.unit;
-      cnt += r.n[i];
-    }
-    if (static_cast<int>(__reduce_add_sync(0xffffffffu, cnt)) <= p.splits) break;
-    r.unit += max(1, r.unit / 16);
-  }
-  int before = 0;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    int incl = r.n[i];
+  int sum = 0;
+  for (int b = lane; b < p.B; b += 32) sum += tree_tiles(p, tree_prefix(p, b));
+  TreeLine l;
+  l.tiles = __reduce_add_sync(0xffffffffu, sum);
+  l.length = (int64_t)l.tiles * p.columns;
+  l.ctas = (int)min((int64_t)p.ctas, l.length);
+  return l;
+}
+struct TreeSegment {
+  int b, prefix;   // sequence, its cached keys
+  int column;
+  int first, end;  // tiles of the sequence
+  int64_t slot;
+};
+// The segment at `pos` of CTA `cta`, whose run ends at `stop`.
+__device__ __forceinline__ TreeSegment tree_segment(const TreeParams& p, const TreeLine& l, int cta, int64_t pos, int64_t stop) {
+  const int lane = threadIdx.x & 31;
+  TreeSegment s;
+  s.column = (int)(pos / l.tiles);
+  int at = (int)(pos - (int64_t)s.column * l.tiles);
+  s.b = s.prefix = s.first = s.end = 0;
+  for (int base = 0; base < p.B; base += 32) {
+    const int prefix = base + lane < p.B ? tree_prefix(p, base + lane) : 0;
+    const int tiles = base + lane < p.B ? tree_tiles(p, prefix) : 0;
+    int incl = tiles;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
       const int up = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += up;
     }
-    r.first[i] = before + incl - r.n[i];
-    before += __shfl_sync(0xffffffffu, incl, 31);
-  }
-  return r;
-}
-// What split x of the batch is.
-__device__ __forceinline__ TreeSplit tree_split(const TreeParams& p, int x) {
-  TreeSplit s = {-1, 0, 0, 0};
-  int unit;
-  int index = 0;
-  if (p.per_seq > 0) {
-    s.b = x / p.per_seq;
-    index = x - s.b * p.per_seq;
-  } else {
-    const TreePlan plan = tree_plan(p);
-    unit = plan.unit;
-#pragma unroll
-    for (int i = 0; i < kTreePlanSeqs / 32; ++i) {
-      const unsigned mine = __ballot_sync(0xffffffffu, x >= plan.first[i] && x < plan.first[i] + plan.n[i]);
-      if (mine) {
-        s.b = __ffs(mine) - 1 + 32 * i;
-        index = x - __shfl_sync(0xffffffffu, plan.first[i], __ffs(mine) - 1);
-      }
+    const unsigned past = __ballot_sync(0xffffffffu, at < incl);
+    if (past) {
+      const int src = __ffs(past) - 1;
+      s.b = base + src;
+      s.prefix = __shfl_sync(0xffffffffu, prefix, src);
+      s.end = __shfl_sync(0xffffffffu, tiles, src);
+      s.first = at - (__shfl_sync(0xffffffffu, incl, src) - s.end);
+      break;
     }
-    if (s.b < 0) return s;
+    at -= __shfl_sync(0xffffffffu, incl, 31);
   }
-  s.prefix = tree_prefix(p, s.b);
-  const int tiles = tree_tiles(p, s.prefix);
-  if (p.per_seq > 0) unit = (tiles + p.per_seq - 1) / p.per_seq;
-  s.first = index * unit;
-  s.end = min(tiles, s.first + unit);
-  if (s.first >= s.end) s.b = -1;
+  s.end = (int)min((int64_t)s.end, s.first + (stop - pos));
+  s.slot = (int64_t)cta + (int64_t)s.column * p.B + s.b;
   return s;
 }
-// The splits of sequence b: their number and the first one's.
-__device__ __forceinline__ void tree_splits_of(const TreeParams& p, int b, int& first, int& n) {
-  if (p.per_seq > 0) {
-    const int tiles = tree_tiles(p, tree_prefix(p, b));
-    const int unit = (tiles + p.per_seq - 1) / p.per_seq;
-    first = b * p.per_seq;
-    n = (tiles + unit - 1) / unit;
-    return;
-  }
-  const TreePlan plan = tree_plan(p);
-  first = n = 0;
-#pragma unroll
-  for (int i = 0; i < kTreePlanSeqs / 32; ++i)
-    if (b / 32 == i) {
-      first = __shfl_sync(0xffffffffu, plan.first[i], b & 31);
-      n = __shfl_sync(0xffffffffu, plan.n[i], b & 31);
-    }
-}
+__device__ __forceinline__ int64_t tree_run(const TreeLine& l, int cta) { return l.length * cta / l.ctas; }
 
 bool tree_sm100_supported(const TreeParams& p, int dtype, const char** why);
+// Geometry of the tensor-core kernel: rows of a column, columns, CTAs.
+void tree_sm100_geometry(TreeParams& p);
 int launch_tree_sm100(const TreeParams& p, int dtype, cudaStream_t stream);
 
 }  // namespace pjx
