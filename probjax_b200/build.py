@@ -31,6 +31,7 @@ SOURCES = [
     "attn_tree.cu",
     "attn_tree_sm100.cu",
     "key_weights.cu",
+    "key_weights_sm100.cu",
     "kv_cache.cu",
     "kv_compact.cu",
     "rope.cu",

@@ -107,7 +107,7 @@ int launch_t(const KeyWeightsParams& p, cudaStream_t stream) {
 int launch_key_weights(const KeyWeightsParams& p, int dtype, int impl, cudaStream_t stream) {
   if (impl != PJX_IMPL_GENERIC && key_weights_sm100_supported(p, dtype)) return launch_key_weights_sm100(p, dtype, stream);
   if (impl == PJX_IMPL_SM100)
-    return fail(PJX_ERR_UNSUPPORTED, "the tcgen05 key weights take bf16/fp16, D in {64, 128}, at most 256 query heads a KV head and 16-byte aligned q / k");
+    return fail(PJX_ERR_UNSUPPORTED, "the tcgen05 key weights take bf16/fp16, D in {64, 128}, at most 128 query heads a KV head and 16-byte aligned q / k");
   if (p.D > 256) return fail(PJX_ERR_UNSUPPORTED, "key weights: head width up to 256 (got %d)", p.D);
   switch (dtype) {
     case PJX_F32: return launch_t<float>(p, stream);
@@ -115,10 +115,6 @@ int launch_key_weights(const KeyWeightsParams& p, int dtype, int impl, cudaStrea
     default: return launch_t<__half>(p, stream);
   }
 }
-
-// (tensor-core form: not built yet)
-bool key_weights_sm100_supported(const KeyWeightsParams&, int) { return false; }
-int launch_key_weights_sm100(const KeyWeightsParams&, int, cudaStream_t) { return fail(PJX_ERR_UNSUPPORTED, "key weights"); }
 
 }  // namespace pjx
 
