@@ -2,16 +2,21 @@
 // that a key's sum over all query rows is one thread's: w_j += sum_r exp2(c q_r.k_j - lse2_r), no exchange between threads.
 //
 // With few rows the call is bound by HBM (K once), from some 160 rows per KV head on by the exponentials (16 per clock and SM).
-// 256 keys a step, as two 128-key tiles with a group of 128 threads each; rows (t, g) in chunks of up to 128; every chunk of
-// scores is double-buffered in tensor memory (2 tiles x 2 x 128 columns), so the MMAs run ahead of the exponentials.
+// 128 keys a step, the even and the odd steps with groups of threads and two score buffers (128 columns each) of their own, so that the
+// MMAs run ahead of the exponentials; rows (t, g) in chunks of up to 128.  The log-sum-exp of a row is subtracted by the MMAs too: one
+// more step of 16 columns multiplies -lse2 / c, split into three 16-bit numbers (24 bits and more), with a constant; read per column and
+// thread out of shared memory it cost as much of that memory's bandwidth as all MMA operands.
 //
-//   warp 0       TMA producer: pairs of key tiles (two stages), chunks of Q and their log-sum-exps (QST stages)
+//   warp 0       producer: key tiles (KST stages) and chunks of Q (QST stages) by TMA, the chunks' log-sum-exp columns
 //   warp 1       MMA issuer
-//   warps 2-5, 6-9   the two groups: one thread per key
+//   warps 2-17   four groups of 128 threads, two per parity: a key has a thread for the first 64 rows of a chunk and one for the
+//                others (with one thread per key, 2.5 warps per scheduler, the kernel waits for latencies: 259 us against xx)
 //
 // RESIDENT: all rows fit into the stages, stay there while the CTA walks the keys of one (sequence, head), and the key steps are dealt
 // in contiguous runs; otherwise the rows stream past every key step out of L2 and the steps are dealt in turn, which balances a
 // causal mask.  Every wait is bounded as in the other tcgen05 kernels.
+#include <type_traits>
+
 #include "sm100_softmax.cuh"
 
 namespace pjx {
@@ -24,8 +29,12 @@ namespace {
 using namespace sm100;
 
 constexpr int BT = 128;          // keys of a tile, rows of a chunk
-constexpr int STEP = 2 * BT;     // keys of a step
-constexpr int NTHREADS = 320;
+constexpr int STEP = BT;         // keys of a step
+constexpr int NTHREADS = 576;
+#ifndef POLY
+#define POLY 3
+#endif
+constexpr int kPolyEvery = POLY;
 
 __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, int c2, int c3, int c4) {
   asm volatile(
@@ -35,19 +44,43 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* m, 
       : "memory");
 }
 
+// 2^x for two numbers on the FMA pipe: x = i + f with i the nearest integer (adding and taking away 1.5 * 2^23 + 127 rounds, and leaves i + 127
+// in the low bits), 2^f on [-1/2, 1/2] by the polynomial of degree 5 with the least largest relative error, 7.5e-8 (found by
+// exchange, in float64).  x is held to [-127, 128], where the result is 0 and infinite; NaN stays NaN.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-127.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-127.f));
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(128.f));
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(128.f));
+  constexpr float kRound = 12582912.f + 127.f;
+  const float2 t = __fadd2_rn(x, make_float2(kRound, kRound));
+  const float2 r = __fadd2_rn(t, make_float2(-kRound, -kRound));
+  const float2 f = __fadd2_rn(x, make_float2(-r.x, -r.y));
+  constexpr float c[6] = {1.0000001192092896f, 0.6931469440460205f, 0.24022120237350464f, 0.05550713092088699f, 0.009675540961325169f, 0.0013276472454890609f};
+  float2 y = make_float2(c[5], c[5]);
+#pragma unroll
+  for (int i = 4; i >= 0; --i) y = __ffma2_rn(y, f, make_float2(c[i], c[i]));
+  return __fmul2_rn(y, make_float2(__int_as_float(__float_as_int(t.x) << 23), __int_as_float(__float_as_int(t.y) << 23)));
+}
+
 template <int HD>
 struct Cfg {
   static constexpr int SUB = HD / 64;
   static constexpr int TILE_BYTES = SUB * BT * 128;
-  static constexpr int QST = HD == 128 ? 3 : 6;
-  static constexpr int OFF_K = 0;                              // [2 stages][2 tiles]
-  static constexpr int OFF_Q = OFF_K + 4 * TILE_BYTES;         // [QST]
-  static constexpr int OFF_LSE = OFF_Q + QST * TILE_BYTES;     // [QST][BT] minus the base-2 log-sum-exp
-  static constexpr int OFF_BAR = OFF_LSE + QST * BT * 4;
-  static constexpr int N_BAR = 4 + 2 * QST + 8;
+  static constexpr int QST = HD == 128 ? 2 : 3;
+  static constexpr int KST = HD == 128 ? 4 : 6;
+  static constexpr int OFF_K = 0;                              // [KST]
+  static constexpr int OFF_Q = OFF_K + KST * TILE_BYTES;       // [QST]
+  static constexpr int OFF_EXT = OFF_Q + QST * TILE_BYTES;     // 128 rows of 4 x 16 columns: the QST stages' log-sum-exps, then the constant
+  static constexpr int OFF_SUM = OFF_EXT + BT * 128;           // [4 steps][2 parities][BT] sums of the second halves
+  static constexpr int OFF_BAR = OFF_SUM + 8 * BT * 4;
+  static constexpr int N_BAR = 2 * KST + 2 * QST + 8 + 32;
   static constexpr int SMEM_BYTES = OFF_BAR + N_BAR * 8 + 16 + 1024;
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
+  static_assert(QST <= 3, "the constant takes the last of the four column groups");
 };
+// -lse2 / c = 4096 a + 64 b + c': in fp16 that reaches to 2.6 * 10^8 and down to 6 * 10^-8.
+constexpr float kExt0 = 4096.f, kExt1 = 64.f;
 
 struct KeyGeometry {
   int tokens;  // query tokens of a chunk
@@ -103,18 +136,26 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_unaligned) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = uniform(smem_u32(smem));
   auto BAR = [&](int i) { return sbase + C::OFF_BAR + 8u * i; };
-  constexpr int K_FULL = 0, K_EMPTY = 2, Q_FULL = 4, Q_EMPTY = Q_FULL + C::QST, S_FULL = Q_EMPTY + C::QST, S_FREE = S_FULL + 4;
+  constexpr int K_FULL = 0, K_EMPTY = C::KST, Q_FULL = 2 * C::KST, Q_EMPTY = Q_FULL + C::QST, S_FULL = Q_EMPTY + C::QST, S_FREE = S_FULL + 4,
+                SUM = S_FREE + 4;  // [4 steps][2 parities][4 warps] the second half's sums are there
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_BAR + C::N_BAR * 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float* lse_s = reinterpret_cast<float*>(smem + C::OFF_LSE);
   const int warp = uniform(static_cast<int>(threadIdx.x >> 5)), lane = threadIdx.x & 31;
   const int G = p.Hq / p.Hkv;
   const int per_head = key_line(p);
   const int64_t total = (int64_t)per_head * p.Hkv;
   // this CTA's steps: pos = start, start + stride, .. below stop
-  const int64_t start = RESIDENT ? total * blockIdx.x / gridDim.x : blockIdx.x;
-  const int64_t stop = RESIDENT ? total * (blockIdx.x + 1) / gridDim.x : total;
+  const int head = blockIdx.x % p.Hkv, part = blockIdx.x / p.Hkv, parts = gridDim.x / p.Hkv;
+  const int64_t start = RESIDENT ? (int64_t)head * per_head + (int64_t)per_head * part / parts : blockIdx.x;
+  const int64_t stop = RESIDENT ? (int64_t)head * per_head + (int64_t)per_head * (part + 1) / parts : total;
   const int64_t stride = RESIDENT ? 1 : gridDim.x;
+  // The step at `pos`: the next one of the same rows where it follows on.
+  auto advance = [&](KeyStep& s, int64_t pos) {
+    if (RESIDENT && pos != start && s.k0 + STEP < s.len)
+      s.k0 += STEP;
+    else
+      s = key_step(p, per_head, pos);
+  };
   // chunks whose tokens see a key of the step
   auto chunk_range = [&](const KeyStep& s, int& c0, int& c1) {
     const int t_first = (int)max((int64_t)0, (int64_t)s.k0 - p.band_hi);
@@ -129,7 +170,7 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::N_BAR; ++i)
-      mbar_init(BAR(i), i >= Q_FULL && i < Q_EMPTY ? 33u : i >= Q_EMPTY && i < S_FULL ? 257u : i >= S_FREE ? 128u : 1u);
+      mbar_init(BAR(i), i >= Q_FULL && i < Q_EMPTY ? 2u : i >= S_FREE && i < SUM ? 8u : 1u);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -148,6 +189,13 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
       prefetch_tmap(&tm_k);
       prefetch_tmap(&tm_q);
     }
+    using T = std::conditional_t<BF16, __nv_bfloat16, __half>;
+    auto write_ext = [&](int row, int group, uint32_t first, uint32_t second) {  // 16 columns of a 128-byte-swizzled row: three numbers
+      const uint32_t at = sbase + C::OFF_EXT + row * 128;
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %3};\n" ::"r"(at + (((2 * group) ^ (row & 7)) << 4)), "r"(first), "r"(second), "r"(0) : "memory");
+      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(at + (((2 * group + 1) ^ (row & 7)) << 4)), "r"(0) : "memory");
+    };
+    for (int i = lane; i < BT; i += 32) write_ext(i, 3, pack16<BF16>(kExt0, kExt1), pack16<BF16>(1.f, 0.f));  // (fenced with the first chunk)
     bool ok = true;
     int step = 0, fill = 0, held_b = -1, held_hk = -1;  // steps, Q stages filled so far, whose rows they hold
     auto load_chunk = [&](const KeyStep& s, int c) {
@@ -157,30 +205,35 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
       ++fill;
       for (int i = lane; i < BT; i += 32) {
         const int t = c * geo.tokens + i / G, h = s.hk * G + i % G;
-        float l = INFINITY;  // rows that are not there, and rows without keys, add nothing
+        float l = INFINITY;  // rows without keys add nothing
         if (i < geo.tokens * G && t < p.Lq) l = p.lse[((int64_t)s.b * p.Hq + h) * p.Lq + t] * kLog2e;
-        lse_s[st * BT + i] = -l;
+        const float x = -l / (p.sm_scale * kLog2e);
+        const float hi = Elem<T>::round(x / kExt0), rest = fmaf(-kExt0, hi, x);
+        const float mid = Elem<T>::round(rest / kExt1), lo = fmaf(-kExt1, mid, rest);
+        const bool finite = fabsf(hi) < INFINITY;
+        write_ext(i, st, pack16<BF16>(hi, finite ? mid : 0.f), pack16<BF16>(finite ? lo : 0.f, 0.f));
       }
-      mbar_arrive(BAR(Q_FULL + st));
+      fence_proxy_async();
+      __syncwarp();
       if (leader) {
+        mbar_arrive(BAR(Q_FULL + st));
         mbar_arrive_expect_tx(BAR(Q_FULL + st), C::SUB * (uint32_t)(geo.tokens * G) * 128u);
 #pragma unroll
         for (int u = 0; u < C::SUB; ++u)
           tma_load_5d(sbase + C::OFF_Q + st * C::TILE_BYTES + u * BT * 128, &tm_q, BAR(Q_FULL + st), u * 64, 0, s.hk, c * geo.tokens, s.b);
       }
     };
+    KeyStep s = {};
     for (int64_t pos = start; ok && pos < stop; pos += stride, ++step) {
-      const KeyStep s = key_step(p, per_head, pos);
-      const int ks = step & 1;
-      ok = mbar_wait_all(BAR(K_EMPTY + ks), ((step >> 1) & 1) ^ 1, abort_flag);
+      advance(s, pos);
+      const int ks = step % C::KST;
+      ok = mbar_wait_all(BAR(K_EMPTY + ks), ((step / C::KST) & 1) ^ 1, abort_flag);
       if (!ok) break;
       if (leader) {
-        mbar_arrive_expect_tx(BAR(K_FULL + ks), 2 * C::TILE_BYTES);
+        mbar_arrive_expect_tx(BAR(K_FULL + ks), C::TILE_BYTES);
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int u = 0; u < C::SUB; ++u)
-            tma_load_4d(sbase + C::OFF_K + (ks * 2 + t) * C::TILE_BYTES + u * BT * 128, &tm_k, BAR(K_FULL + ks), u * 64, s.hk, s.k0 + t * BT, s.b);
+        for (int u = 0; u < C::SUB; ++u)
+          tma_load_4d(sbase + C::OFF_K + ks * C::TILE_BYTES + u * BT * 128, &tm_k, BAR(K_FULL + ks), u * 64, s.hk, s.k0, s.b);
       }
       int c0, c1;
       chunk_range(s, c0, c1);
@@ -192,48 +245,57 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
   } else if (warp == 1) {
     const uint32_t leader = elect_leader();
     constexpr uint32_t idesc = make_idesc(BT, BT, BF16, false, false);
+    // (descriptors differ in the address field, in units of 16 bytes)
+    const uint64_t k_desc = make_smem_desc(sbase + C::OFF_K, 16, 1024), q_desc = make_smem_desc(sbase + C::OFF_Q, 16, 1024);
+    const uint64_t ext_desc = make_smem_desc(sbase + C::OFF_EXT, 16, 1024);
     bool ok = true;
-    int step = 0, used = 0, base = 0, n_s = 0, held_b = -1, held_hk = -1;  // Q stages used, the first of the resident ones, score tiles
+    int step = 0, used = 0, base = 0, held_b = -1, held_hk = -1;  // Q stages used, the first of the resident ones
+    int n_s[2] = {0, 0};                                          // score tiles of either parity
+    KeyStep s = {};
     for (int64_t pos = start; ok && pos < stop; pos += stride, ++step) {
-      const KeyStep s = key_step(p, per_head, pos);
+      advance(s, pos);
       int c0, c1;
       chunk_range(s, c0, c1);
       const bool fresh = !RESIDENT || s.b != held_b || s.hk != held_hk;
-      const KeyStep after = RESIDENT && pos + 1 < stop ? key_step(p, per_head, pos + 1) : s;
-      const bool last = RESIDENT && pos + 1 < stop && (after.b != s.b || after.hk != s.hk);  // the rows are done with this step
+      const bool last = RESIDENT && s.k0 + STEP >= s.len;  // the rows are done with this step
       held_b = s.b;
       held_hk = s.hk;
       if (RESIDENT && fresh) {
         base = used;
         used += geo.chunks;
       }
-      ok = mbar_wait_all(BAR(K_FULL + (step & 1)), (step >> 1) & 1, abort_flag);
-      for (int c = c0; ok && c < c1; ++c, ++n_s) {
+      const int ks = step % C::KST, t = step & 1;
+      ok = mbar_wait_all(BAR(K_FULL + ks), (step / C::KST) & 1, abort_flag);
+      for (int c = c0; ok && c < c1; ++c) {
         const int f = RESIDENT ? base + c : used++;
         const int st = f % C::QST;
         if (fresh) ok = mbar_wait_all(BAR(Q_FULL + st), (f / C::QST) & 1, abort_flag);
+        const int n = t ? n_s[1]++ : n_s[0]++, buf = t * 2 + (n & 1);
+        ok = ok && mbar_wait_all(BAR(S_FREE + buf), ((n >> 1) & 1) ^ 1, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t ka = k_desc + ks * (C::TILE_BYTES / 16), qa = q_desc + st * (C::TILE_BYTES / 16);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int buf = t * 2 + (n_s & 1);
-          ok = ok && mbar_wait_all(BAR(S_FREE + buf), ((n_s >> 1) & 1) ^ 1, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t ka = sbase + C::OFF_K + ((step & 1) * 2 + t) * C::TILE_BYTES, qa = sbase + C::OFF_Q + st * C::TILE_BYTES;
+        for (int u = 0; u < C::SUB; ++u)
 #pragma unroll
-          for (int u = 0; u < C::SUB; ++u)
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              mma_ss(tmem + buf * BT, make_smem_desc(ka + u * BT * 128 + kk * 32, 16, 1024),
-                     make_smem_desc(qa + u * BT * 128 + kk * 32, 16, 1024), idesc, (u | kk) != 0, leader);
-          mma_commit(BAR(S_FULL + buf), leader);
-        }
-        if (ok && (!RESIDENT || last)) mma_commit(BAR(Q_EMPTY + st), leader);
+          for (int kk = 0; kk < 4; ++kk)
+            mma_ss(tmem + buf * BT, ka + (u * BT * 128 + kk * 32) / 16, qa + (u * BT * 128 + kk * 32) / 16, idesc, (u | kk) != 0, leader);
+        // (last: one more rounding at the size of the result)
+        mma_ss(tmem + buf * BT, ext_desc + 3 * 2, ext_desc + st * 2, idesc, true, leader);
+        mma_commit(BAR(S_FULL + buf), leader);
+        if (!RESIDENT || last) mma_commit(BAR(Q_EMPTY + st), leader);
       }
-      if (ok) mma_commit(BAR(K_EMPTY + (step & 1)), leader);
+      if (ok) mma_commit(BAR(K_EMPTY + ks), leader);
     }
   } else {
-    const int t = (warp - 2) >> 2;
+    const int t = ((warp - 2) >> 2) & 1, half = (warp - 2) >> 3;
     const int key_in = (warp & 3) * 32 + lane;  // tensor-memory lane
+    // The first half's thread adds the second's sum one step later, when it has long been there.
+    float* sums = reinterpret_cast<float*>(smem + C::OFF_SUM) + t * BT + key_in;
+    auto sum_bar = [&](int m) { return BAR(SUM + ((m & 3) * 2 + t) * 4 + (warp & 3)); };
+    float held_part = 0.f;
+    int64_t held_at = -1;  // where the sum of the step before goes
+    bool holds = false;
     const uint32_t lane_sel = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const float c1 = p.sm_scale * kLog2e;
     const float2 cc = make_float2(c1, c1);
@@ -241,75 +303,84 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
       const int tid = threadIdx.x - 64;
       for (int64_t row = blockIdx.x; row < (int64_t)p.B * p.Hkv; row += gridDim.x) {
         const int len = key_len(p, (int)(row / p.Hkv));
-        for (int j = len + tid; j < p.Lkv; j += 256) p.weights_out[row * p.Lkv + j] = p.weights_in ? p.weights_in[row * p.Lkv + j] : 0.f;
+        for (int j = len + tid; j < p.Lkv; j += NTHREADS - 64) p.weights_out[row * p.Lkv + j] = p.weights_in ? p.weights_in[row * p.Lkv + j] : 0.f;
       }
     }
     bool ok = true;
-    int step = 0, used = 0, base = 0, n_s = 0, held_b = -1, held_hk = -1;
+    auto finish = [&](int m) {
+      ok = ok && mbar_wait(sum_bar(m), (m >> 2) & 1, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok && held_at >= 0) p.weights_out[held_at] = (p.weights_in ? p.weights_in[held_at] : 0.f) + (held_part + sums[(m & 3) * 2 * BT]);
+    };
+    int step = 0, n_s = 0, mine = 0;  // steps, score tiles and steps of this parity
+    KeyStep s = {};
     for (int64_t pos = start; ok && pos < stop; pos += stride, ++step) {
-      const KeyStep s = key_step(p, per_head, pos);
+      advance(s, pos);
+      if ((step & 1) != t) continue;  // the other parity's
       int c_first, c_last;
       chunk_range(s, c_first, c_last);
-      const bool fresh = !RESIDENT || s.b != held_b || s.hk != held_hk;
-      const KeyStep after = RESIDENT && pos + 1 < stop ? key_step(p, per_head, pos + 1) : s;
-      const bool last = RESIDENT && pos + 1 < stop && (after.b != s.b || after.hk != s.hk);
-      held_b = s.b;
-      held_hk = s.hk;
-      if (RESIDENT && fresh) {
-        base = used;
-        used += geo.chunks;
-      }
-      const int first_key = s.k0 + t * BT, key = first_key + key_in;
-      float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
+      const int key = s.k0 + key_in;
+      const bool all = s.k0 + BT <= s.len && s.k0 >= (int64_t)p.Lq - 1 + p.band_lo && s.k0 + BT - 1 <= p.band_hi;  // every row sees every key
+      float2 sum[4] = {};
       for (int c = c_first; ok && c < c_last; ++c, ++n_s) {
-        const int f = RESIDENT ? base + c : used++;
-        const int st = f % C::QST, buf = t * 2 + (n_s & 1);
-        if (fresh) ok = mbar_wait(BAR(Q_FULL + st), (f / C::QST) & 1, abort_flag);
-        ok = ok && mbar_wait(BAR(S_FULL + buf), (n_s >> 1) & 1, abort_flag);
+        const int buf = t * 2 + (n_s & 1);
+        ok = mbar_wait(BAR(S_FULL + buf), (n_s >> 1) & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        const int t0 = c * geo.tokens, toks = min(geo.tokens, p.Lq - t0);
-        const int cols = toks * G;
-        // rows of the chunk that see this key: [lo, hi)
-        int lo = 0, hi = cols;
-        const bool whole = first_key + BT <= s.len && first_key >= (int64_t)t0 + toks - 1 + p.band_lo && first_key + BT - 1 <= (int64_t)t0 + p.band_hi;
-        if (!whole) {
+        const int t0 = c * geo.tokens, cols = min(geo.tokens, p.Lq - t0) * G;
+        int lo = 0, hi = cols;  // rows of the chunk that see this key
+        if (!all) {
           const int64_t a = ((int64_t)key - p.band_hi - t0) * G, e = ((int64_t)key - p.band_lo - t0 + 1) * G;
           lo = (int)max((int64_t)0, min((int64_t)cols, a));
           hi = key < s.len ? (int)max((int64_t)0, min((int64_t)cols, e)) : 0;
         }
-        const float4* nl = reinterpret_cast<const float4*>(lse_s + st * BT);
-        for (int c32 = 0; c32 * 32 < cols; ++c32) {
+        const uint32_t s_addr = tmem + lane_sel + buf * BT;
+        const int end = min((cols + 31) / 32, 2 * half + 2);
+        for (int c32 = 2 * half; c32 < end; ++c32) {
           float x[32];
-          tmem_ld32f(tmem + lane_sel + buf * BT + c32 * 32, x);
+          tmem_ld32f(s_addr + c32 * 32, x);
           tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float4 l4 = nl[c32 * 8 + i];
-            const float2 a = __ffma2_rn(make_float2(x[4 * i], x[4 * i + 1]), cc, make_float2(l4.x, l4.y));
-            const float2 e = __ffma2_rn(make_float2(x[4 * i + 2], x[4 * i + 3]), cc, make_float2(l4.z, l4.w));
-            x[4 * i] = a.x; x[4 * i + 1] = a.y; x[4 * i + 2] = e.x; x[4 * i + 3] = e.y;
+          for (int i = 0; i < 16; ++i) {
+            const float2 a = __fmul2_rn(make_float2(x[2 * i], x[2 * i + 1]), cc);
+            x[2 * i] = a.x; x[2 * i + 1] = a.y;
           }
-          if (!whole || c32 * 32 + 32 > cols) {  // (columns past the rows hold anything)
+          if (!all || c32 * 32 + 32 > cols) {  // (columns past the rows hold anything)
 #pragma unroll
             for (int i = 0; i < 32; ++i) x[i] = c32 * 32 + i >= lo && c32 * 32 + i < hi ? x[i] : -INFINITY;
           }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            sum0 = __fadd2_rn(sum0, make_float2(ex2_approx(x[4 * i]), ex2_approx(x[4 * i + 1])));
-            sum1 = __fadd2_rn(sum1, make_float2(ex2_approx(x[4 * i + 2]), ex2_approx(x[4 * i + 3])));
+          for (int i = 0; i < 16; ++i) {
+            const float2 v = make_float2(x[2 * i], x[2 * i + 1]);
+            const float2 e = i % kPolyEvery == kPolyEvery - 1 ? exp2_poly(v) : make_float2(ex2_approx(v.x), ex2_approx(v.y));
+            sum[i & 3] = __fadd2_rn(sum[i & 3], e);
           }
         }
         tc_fence_before();
-        mbar_arrive(BAR(S_FREE + buf));
-        if (!RESIDENT || last) mbar_arrive(BAR(Q_EMPTY + st));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(BAR(S_FREE + buf));  // (an arrival per warp: 256 on one word took as long as the MMAs)
       }
-      if (ok && key < s.len) {
-        const int64_t at = ((int64_t)s.b * p.Hkv + s.hk) * p.Lkv + key;
-        p.weights_out[at] = (p.weights_in ? p.weights_in[at] : 0.f) + ((sum0.x + sum0.y) + (sum1.x + sum1.y));
+      const float2 s01 = __fadd2_rn(sum[0], sum[1]), s23 = __fadd2_rn(sum[2], sum[3]);
+      const float part = (s01.x + s01.y) + (s23.x + s23.y);
+      const int64_t at = key < s.len ? ((int64_t)s.b * p.Hkv + s.hk) * p.Lkv + key : -1;
+      if (c_first == c_last) {  // no row sees a key of the step
+        if (half == 0 && at >= 0) p.weights_out[at] = p.weights_in ? p.weights_in[at] : 0.f;
+        continue;
       }
+      if (half == 1) {
+        sums[(mine & 3) * 2 * BT] = part;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(sum_bar(mine));
+      } else {
+        if (holds) finish(mine - 1);
+        held_part = part;
+        held_at = at;
+        holds = true;
+      }
+      ++mine;
     }
+    if (half == 0 && holds && ok) finish(mine - 1);
   }
 
   tc_fence_before();
@@ -338,7 +409,7 @@ int launch_t(const KeyWeightsParams& p, int dtype, cudaStream_t stream) {
   auto kern = resident ? key_weights_sm100_kernel<HD, BF16, true> : key_weights_sm100_kernel<HD, BF16, false>;
   if ((rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES), "cudaFuncSetAttribute(key weights)")))
     return rc;
-  kern<<<148, NTHREADS, C::SMEM_BYTES, stream>>>(tk, tq, p, geo);
+  kern<<<resident ? p.Hkv * (148 / p.Hkv) : 148, NTHREADS, C::SMEM_BYTES, stream>>>(tk, tq, p, geo);
   count_launch();
   return check_cuda(cudaGetLastError(), "key weights launch");
 }
@@ -349,6 +420,7 @@ bool key_weights_sm100_supported(const KeyWeightsParams& p, int dtype) {
   if (dtype != PJX_BF16 && dtype != PJX_F16) return false;
   if (p.D != 64 && p.D != 128) return false;
   if (p.Hq / p.Hkv > BT || p.Lq < 1) return false;
+  if (!(fabsf(p.sm_scale) >= 1e-4f && fabsf(p.sm_scale) <= 1e4f)) return false;  // (-lse2 / c stays in range)
   return ((reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k)) & 15) == 0;
 }
 
