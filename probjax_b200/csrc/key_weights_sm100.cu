@@ -10,7 +10,12 @@
 //   warp 0       producer: key tiles (KST stages) and chunks of Q (QST stages) by TMA, the chunks' log-sum-exp columns
 //   warp 1       MMA issuer
 //   warps 2-17   four groups of 128 threads, two per parity: a key has a thread for the first 64 rows of a chunk and one for the
-//                others (with one thread per key, 2.5 warps per scheduler, the kernel waits for latencies: 259 us against xx)
+//                others (with one thread per key, 2.5 warps per scheduler, the kernel waits for latencies)
+//
+// 8 prompts of 32k keys, 8 KV heads of 128 (537 MB of keys), us: 4 rows per KV head 105, 64 rows 107, 128 rows 114 (4.7 TB/s), 256 rows
+// 183, where the exponentials alone take 131.  Steps at 256 rows: a thread per key 259, two threads 224, log-sum-exps inside the
+// MMAs 198, sums of the second half added a step later and short loops around the MMAs 183.  A part of the exponentials as a
+// polynomial on the FMA pipe (a quarter, a third, a half) is no faster: 187, 185, 209.
 //
 // RESIDENT: all rows fit into the stages, stay there while the CTA walks the keys of one (sequence, head), and the key steps are dealt
 // in contiguous runs; otherwise the rows stream past every key step out of L2 and the steps are dealt in turn, which balances a
@@ -31,10 +36,6 @@ using namespace sm100;
 constexpr int BT = 128;          // keys of a tile, rows of a chunk
 constexpr int STEP = BT;         // keys of a step
 constexpr int NTHREADS = 576;
-#ifndef POLY
-#define POLY 3
-#endif
-constexpr int kPolyEvery = POLY;
 
 __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, int c2, int c3, int c4) {
   asm volatile(
@@ -42,25 +43,6 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* m, 
       "[%0], [%1, {%3, %4, %5, %6, %7}], [%2];\n" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
       : "memory");
-}
-
-// 2^x for two numbers on the FMA pipe: x = i + f with i the nearest integer (adding and taking away 1.5 * 2^23 + 127 rounds, and leaves i + 127
-// in the low bits), 2^f on [-1/2, 1/2] by the polynomial of degree 5 with the least largest relative error, 7.5e-8 (found by
-// exchange, in float64).  x is held to [-127, 128], where the result is 0 and infinite; NaN stays NaN.
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-127.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-127.f));
-  asm("min.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(128.f));
-  asm("min.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(128.f));
-  constexpr float kRound = 12582912.f + 127.f;
-  const float2 t = __fadd2_rn(x, make_float2(kRound, kRound));
-  const float2 r = __fadd2_rn(t, make_float2(-kRound, -kRound));
-  const float2 f = __fadd2_rn(x, make_float2(-r.x, -r.y));
-  constexpr float c[6] = {1.0000001192092896f, 0.6931469440460205f, 0.24022120237350464f, 0.05550713092088699f, 0.009675540961325169f, 0.0013276472454890609f};
-  float2 y = make_float2(c[5], c[5]);
-#pragma unroll
-  for (int i = 4; i >= 0; --i) y = __ffma2_rn(y, f, make_float2(c[i], c[i]));
-  return __fmul2_rn(y, make_float2(__int_as_float(__float_as_int(t.x) << 23), __int_as_float(__float_as_int(t.y) << 23)));
 }
 
 template <int HD>
@@ -98,6 +80,7 @@ __device__ __forceinline__ int key_line(const KeyWeightsParams& p) {
 }
 struct KeyStep {
   int b, hk, len, k0;
+  int n;  // steps of a run that follow on, with the same rows
 };
 __device__ __forceinline__ KeyStep key_step(const KeyWeightsParams& p, int per_head, int64_t pos) {
   const int lane = threadIdx.x & 31;
@@ -105,6 +88,7 @@ __device__ __forceinline__ KeyStep key_step(const KeyWeightsParams& p, int per_h
   s.hk = (int)(pos / per_head);
   int at = (int)(pos - (int64_t)s.hk * per_head);
   s.b = s.len = s.k0 = 0;
+  s.n = 1;
   for (int base = 0; base < p.B; base += 32) {
     const int len = base + lane < p.B ? key_len(p, base + lane) : 0;
     const int steps = (len + STEP - 1) / STEP;
@@ -148,14 +132,18 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
   const int head = blockIdx.x % p.Hkv, part = blockIdx.x / p.Hkv, parts = gridDim.x / p.Hkv;
   const int64_t start = RESIDENT ? (int64_t)head * per_head + (int64_t)per_head * part / parts : blockIdx.x;
   const int64_t stop = RESIDENT ? (int64_t)head * per_head + (int64_t)per_head * (part + 1) / parts : total;
-  const int64_t stride = RESIDENT ? 1 : gridDim.x;
-  // The step at `pos`: the next one of the same rows where it follows on.
-  auto advance = [&](KeyStep& s, int64_t pos) {
-    if (RESIDENT && pos != start && s.k0 + STEP < s.len)
-      s.k0 += STEP;
-    else
-      s = key_step(p, per_head, pos);
+  // The run of steps at `pos` (one step where the rows stream).
+  auto run_at = [&](int64_t pos) {
+    KeyStep s = key_step(p, per_head, pos);
+    if constexpr (RESIDENT) s.n = (int)min((int64_t)(s.len - s.k0 + STEP - 1) / STEP, stop - pos);
+    s.b = uniform(s.b);
+    s.hk = uniform(s.hk);
+    s.len = uniform(s.len);
+    s.k0 = uniform(s.k0);
+    s.n = uniform(s.n);
+    return s;
   };
+  const int64_t stride = RESIDENT ? 1 : gridDim.x;
   // chunks whose tokens see a key of the step
   auto chunk_range = [&](const KeyStep& s, int& c0, int& c1) {
     const int t_first = (int)max((int64_t)0, (int64_t)s.k0 - p.band_hi);
@@ -197,7 +185,7 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
     };
     for (int i = lane; i < BT; i += 32) write_ext(i, 3, pack16<BF16>(kExt0, kExt1), pack16<BF16>(1.f, 0.f));  // (fenced with the first chunk)
     bool ok = true;
-    int step = 0, fill = 0, held_b = -1, held_hk = -1;  // steps, Q stages filled so far, whose rows they hold
+    int fill = 0, ks = 0, kp = 1;  // Q stages filled so far; K stage and the parity its freedom is waited with
     auto load_chunk = [&](const KeyStep& s, int c) {
       const int st = fill % C::QST;
       ok = ok && mbar_wait_all(BAR(Q_EMPTY + st), ((fill / C::QST) & 1) ^ 1, abort_flag);
@@ -223,24 +211,26 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
           tma_load_5d(sbase + C::OFF_Q + st * C::TILE_BYTES + u * BT * 128, &tm_q, BAR(Q_FULL + st), u * 64, 0, s.hk, c * geo.tokens, s.b);
       }
     };
-    KeyStep s = {};
-    for (int64_t pos = start; ok && pos < stop; pos += stride, ++step) {
-      advance(s, pos);
-      const int ks = step % C::KST;
-      ok = mbar_wait_all(BAR(K_EMPTY + ks), ((step / C::KST) & 1) ^ 1, abort_flag);
-      if (!ok) break;
-      if (leader) {
-        mbar_arrive_expect_tx(BAR(K_FULL + ks), C::TILE_BYTES);
-#pragma unroll
-        for (int u = 0; u < C::SUB; ++u)
-          tma_load_4d(sbase + C::OFF_K + ks * C::TILE_BYTES + u * BT * 128, &tm_k, BAR(K_FULL + ks), u * 64, s.hk, s.k0, s.b);
-      }
+    for (int64_t pos = start; ok && pos < stop;) {
+      const KeyStep s = run_at(pos);
       int c0, c1;
       chunk_range(s, c0, c1);
-      if (RESIDENT && s.b == held_b && s.hk == held_hk) continue;
-      for (int c = c0; ok && c < c1; ++c) load_chunk(s, c);
-      held_b = s.b;
-      held_hk = s.hk;
+      for (int j = 0; ok && j < s.n; ++j) {
+        if (!(ok = mbar_wait_all(BAR(K_EMPTY + ks), kp, abort_flag))) break;
+        if (leader) {
+          mbar_arrive_expect_tx(BAR(K_FULL + ks), C::TILE_BYTES);
+#pragma unroll
+          for (int u = 0; u < C::SUB; ++u)
+            tma_load_4d(sbase + C::OFF_K + ks * C::TILE_BYTES + u * BT * 128, &tm_k, BAR(K_FULL + ks), u * 64, s.hk, s.k0 + j * STEP, s.b);
+        }
+        if (++ks == C::KST) {
+          ks = 0;
+          kp ^= 1;
+        }
+        if (j == 0)
+          for (int c = c0; ok && c < c1; ++c) load_chunk(s, c);
+      }
+      pos += RESIDENT ? s.n : stride;
     }
   } else if (warp == 1) {
     const uint32_t leader = elect_leader();
@@ -248,54 +238,49 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
     // (descriptors differ in the address field, in units of 16 bytes)
     const uint64_t k_desc = make_smem_desc(sbase + C::OFF_K, 16, 1024), q_desc = make_smem_desc(sbase + C::OFF_Q, 16, 1024);
     const uint64_t ext_desc = make_smem_desc(sbase + C::OFF_EXT, 16, 1024);
+    // (Few instructions between the MMAs: this warp shares its scheduler with compute warps, and a slow step here is one for all.)
     bool ok = true;
-    int step = 0, used = 0, base = 0, held_b = -1, held_hk = -1;  // Q stages used, the first of the resident ones
-    int n_s[2] = {0, 0};                                          // score tiles of either parity
-    KeyStep s = {};
-    for (int64_t pos = start; ok && pos < stop; pos += stride, ++step) {
-      advance(s, pos);
+    int used = 0, ks = 0, kp = 0, step = 0;  // Q stages used; K stage and parity; steps
+    uint32_t n_s = 0x0000;                   // score tiles of either parity, mod 4: bits 0-1 and 2-3
+    for (int64_t pos = start; ok && pos < stop;) {
+      const KeyStep s = run_at(pos);
       int c0, c1;
       chunk_range(s, c0, c1);
-      const bool fresh = !RESIDENT || s.b != held_b || s.hk != held_hk;
-      const bool last = RESIDENT && s.k0 + STEP >= s.len;  // the rows are done with this step
-      held_b = s.b;
-      held_hk = s.hk;
-      if (RESIDENT && fresh) {
-        base = used;
-        used += geo.chunks;
-      }
-      const int ks = step % C::KST, t = step & 1;
-      ok = mbar_wait_all(BAR(K_FULL + ks), (step / C::KST) & 1, abort_flag);
-      for (int c = c0; ok && c < c1; ++c) {
-        const int f = RESIDENT ? base + c : used++;
-        const int st = f % C::QST;
-        if (fresh) ok = mbar_wait_all(BAR(Q_FULL + st), (f / C::QST) & 1, abort_flag);
-        const int n = t ? n_s[1]++ : n_s[0]++, buf = t * 2 + (n & 1);
-        ok = ok && mbar_wait_all(BAR(S_FREE + buf), ((n >> 1) & 1) ^ 1, abort_flag);
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t ka = k_desc + ks * (C::TILE_BYTES / 16), qa = q_desc + st * (C::TILE_BYTES / 16);
+      for (int j = 0; ok && j < s.n; ++j, ++step) {
+        const int t = step & 1;
+        if (!(ok = mbar_wait_all(BAR(K_FULL + ks), kp, abort_flag))) break;
+        const uint64_t ka = k_desc + ks * (C::TILE_BYTES / 16);
+        const bool last = !RESIDENT || j == s.n - 1;
+        for (int c = c0; c < c1; ++c) {
+          const int f = used + c - c0, st = f % C::QST;
+          if (j == 0 && !(ok = mbar_wait_all(BAR(Q_FULL + st), (f / C::QST) & 1, abort_flag))) break;
+          const uint32_t n = (n_s >> (2 * t)) & 3u, buf = t * 2 + (n & 1);
+          if (!(ok = mbar_wait_all(BAR(S_FREE + buf), (n >> 1) ^ 1, abort_flag))) break;
+          n_s = (n_s & ~(3u << (2 * t))) | (((n + 1) & 3u) << (2 * t));
+          tc_fence_after();
+          const uint64_t qa = q_desc + st * (C::TILE_BYTES / 16);
 #pragma unroll
-        for (int u = 0; u < C::SUB; ++u)
+          for (int u = 0; u < C::SUB; ++u)
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_ss(tmem + buf * BT, ka + (u * BT * 128 + kk * 32) / 16, qa + (u * BT * 128 + kk * 32) / 16, idesc, (u | kk) != 0, leader);
-        // (last: one more rounding at the size of the result)
-        mma_ss(tmem + buf * BT, ext_desc + 3 * 2, ext_desc + st * 2, idesc, true, leader);
-        mma_commit(BAR(S_FULL + buf), leader);
-        if (!RESIDENT || last) mma_commit(BAR(Q_EMPTY + st), leader);
+            for (int kk = 0; kk < 4; ++kk)
+              mma_ss(tmem + buf * BT, ka + (u * BT * 128 + kk * 32) / 16, qa + (u * BT * 128 + kk * 32) / 16, idesc, (u | kk) != 0, leader);
+          // (last: one more rounding at the size of the result)
+          mma_ss(tmem + buf * BT, ext_desc + 3 * 2, ext_desc + st * 2, idesc, true, leader);
+          mma_commit(BAR(S_FULL + buf), leader);
+          if (last) mma_commit(BAR(Q_EMPTY + st), leader);
+        }
+        if (ok) mma_commit(BAR(K_EMPTY + ks), leader);
+        if (++ks == C::KST) {
+          ks = 0;
+          kp ^= 1;
+        }
       }
-      if (ok) mma_commit(BAR(K_EMPTY + ks), leader);
+      used += c1 - c0;
+      pos += RESIDENT ? s.n : stride;
     }
   } else {
     const int t = ((warp - 2) >> 2) & 1, half = (warp - 2) >> 3;
     const int key_in = (warp & 3) * 32 + lane;  // tensor-memory lane
-    // The first half's thread adds the second's sum one step later, when it has long been there.
-    float* sums = reinterpret_cast<float*>(smem + C::OFF_SUM) + t * BT + key_in;
-    auto sum_bar = [&](int m) { return BAR(SUM + ((m & 3) * 2 + t) * 4 + (warp & 3)); };
-    float held_part = 0.f;
-    int64_t held_at = -1;  // where the sum of the step before goes
-    bool holds = false;
     const uint32_t lane_sel = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const float c1 = p.sm_scale * kLog2e;
     const float2 cc = make_float2(c1, c1);
@@ -306,79 +291,91 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
         for (int j = len + tid; j < p.Lkv; j += NTHREADS - 64) p.weights_out[row * p.Lkv + j] = p.weights_in ? p.weights_in[row * p.Lkv + j] : 0.f;
       }
     }
-    bool ok = true;
+    // The first half's thread adds the second's sum one step later, when it has long been there.
+    float* sums = reinterpret_cast<float*>(smem + C::OFF_SUM) + t * BT + key_in;
+    auto sum_bar = [&](int m) { return BAR(SUM + ((m & 3) * 2 + t) * 4 + (warp & 3)); };
+    float held_part = 0.f;
+    float* held_out = nullptr;  // where the sum of the step before goes
+    const float* held_in = nullptr;
+    bool ok = true, holds = false;
     auto finish = [&](int m) {
       ok = ok && mbar_wait(sum_bar(m), (m >> 2) & 1, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
-      if (ok && held_at >= 0) p.weights_out[held_at] = (p.weights_in ? p.weights_in[held_at] : 0.f) + (held_part + sums[(m & 3) * 2 * BT]);
+      if (ok && held_out) *held_out = (held_in ? *held_in : 0.f) + (held_part + sums[(m & 3) * 2 * BT]);
     };
     int step = 0, n_s = 0, mine = 0;  // steps, score tiles and steps of this parity
-    KeyStep s = {};
-    for (int64_t pos = start; ok && pos < stop; pos += stride, ++step) {
-      advance(s, pos);
-      if ((step & 1) != t) continue;  // the other parity's
+    for (int64_t pos = start; ok && pos < stop;) {
+      const KeyStep s = run_at(pos);
       int c_first, c_last;
       chunk_range(s, c_first, c_last);
-      const int key = s.k0 + key_in;
-      const bool all = s.k0 + BT <= s.len && s.k0 >= (int64_t)p.Lq - 1 + p.band_lo && s.k0 + BT - 1 <= p.band_hi;  // every row sees every key
-      float2 sum[4] = {};
-      for (int c = c_first; ok && c < c_last; ++c, ++n_s) {
-        const int buf = t * 2 + (n_s & 1);
-        ok = mbar_wait(BAR(S_FULL + buf), (n_s >> 1) & 1, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc_fence_after();
-        const int t0 = c * geo.tokens, cols = min(geo.tokens, p.Lq - t0) * G;
-        int lo = 0, hi = cols;  // rows of the chunk that see this key
-        if (!all) {
-          const int64_t a = ((int64_t)key - p.band_hi - t0) * G, e = ((int64_t)key - p.band_lo - t0 + 1) * G;
-          lo = (int)max((int64_t)0, min((int64_t)cols, a));
-          hi = key < s.len ? (int)max((int64_t)0, min((int64_t)cols, e)) : 0;
+      const int64_t row = ((int64_t)s.b * p.Hkv + s.hk) * p.Lkv;
+      float* out = p.weights_out + row;
+      const float* in = p.weights_in ? p.weights_in + row : nullptr;
+      const int open_from = p.Lq - 1 + p.band_lo, open_to = p.band_hi;  // keys that every row sees
+      const int first = (step & 1) == t ? 0 : 1;                        // this parity's steps of the run
+      step += s.n;
+      pos += RESIDENT ? s.n : stride;
+      for (int j = first; ok && j < s.n; j += 2) {
+        const int k0 = s.k0 + j * STEP, key = k0 + key_in;
+        const bool all = k0 + BT <= s.len && k0 >= open_from && k0 + BT - 1 <= open_to;  // every row sees every key of the step
+        float2 sum[4] = {};
+        for (int c = c_first; ok && c < c_last; ++c, ++n_s) {
+          const int buf = t * 2 + (n_s & 1);
+          ok = mbar_wait(BAR(S_FULL + buf), (n_s >> 1) & 1, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          const int t0 = c * geo.tokens, cols = min(geo.tokens, p.Lq - t0) * G;
+          int lo = 0, hi = cols;  // rows of the chunk that see this key
+          if (!all) {
+            const int64_t a = ((int64_t)key - p.band_hi - t0) * G, e = ((int64_t)key - p.band_lo - t0 + 1) * G;
+            lo = (int)max((int64_t)0, min((int64_t)cols, a));
+            hi = key < s.len ? (int)max((int64_t)0, min((int64_t)cols, e)) : 0;
+          }
+          const uint32_t s_addr = tmem + lane_sel + buf * BT;
+          const int end = min((cols + 31) / 32, 2 * half + 2);
+          for (int c32 = 2 * half; c32 < end; ++c32) {
+            float x[32];
+            tmem_ld32f(s_addr + c32 * 32, x);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float2 a = __fmul2_rn(make_float2(x[2 * i], x[2 * i + 1]), cc);
+              x[2 * i] = a.x; x[2 * i + 1] = a.y;
+            }
+            if (!all || c32 * 32 + 32 > cols) {  // (columns past the rows hold anything)
+#pragma unroll
+              for (int i = 0; i < 32; ++i) x[i] = c32 * 32 + i >= lo && c32 * 32 + i < hi ? x[i] : -INFINITY;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float2 v = make_float2(x[2 * i], x[2 * i + 1]);
+              sum[i & 3] = __fadd2_rn(sum[i & 3], make_float2(ex2_approx(x[2 * i]), ex2_approx(x[2 * i + 1])));
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(BAR(S_FREE + buf));  // (an arrival per warp: 256 on one word took as long as the MMAs)
         }
-        const uint32_t s_addr = tmem + lane_sel + buf * BT;
-        const int end = min((cols + 31) / 32, 2 * half + 2);
-        for (int c32 = 2 * half; c32 < end; ++c32) {
-          float x[32];
-          tmem_ld32f(s_addr + c32 * 32, x);
-          tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 a = __fmul2_rn(make_float2(x[2 * i], x[2 * i + 1]), cc);
-            x[2 * i] = a.x; x[2 * i + 1] = a.y;
-          }
-          if (!all || c32 * 32 + 32 > cols) {  // (columns past the rows hold anything)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = c32 * 32 + i >= lo && c32 * 32 + i < hi ? x[i] : -INFINITY;
-          }
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 v = make_float2(x[2 * i], x[2 * i + 1]);
-            const float2 e = i % kPolyEvery == kPolyEvery - 1 ? exp2_poly(v) : make_float2(ex2_approx(v.x), ex2_approx(v.y));
-            sum[i & 3] = __fadd2_rn(sum[i & 3], e);
-          }
+        const float2 s01 = __fadd2_rn(sum[0], sum[1]), s23 = __fadd2_rn(sum[2], sum[3]);
+        const float part = (s01.x + s01.y) + (s23.x + s23.y);
+        if (c_first == c_last) {  // no row sees a key of the step
+          if (half == 0 && key < s.len) out[key] = in ? in[key] : 0.f;
+          continue;
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(BAR(S_FREE + buf));  // (an arrival per warp: 256 on one word took as long as the MMAs)
+        if (half == 1) {
+          sums[(mine & 3) * 2 * BT] = part;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sum_bar(mine));
+        } else {
+          if (holds) finish(mine - 1);
+          held_part = part;
+          held_out = key < s.len ? out + key : nullptr;
+          held_in = in ? in + key : nullptr;
+          holds = true;
+        }
+        ++mine;
       }
-      const float2 s01 = __fadd2_rn(sum[0], sum[1]), s23 = __fadd2_rn(sum[2], sum[3]);
-      const float part = (s01.x + s01.y) + (s23.x + s23.y);
-      const int64_t at = key < s.len ? ((int64_t)s.b * p.Hkv + s.hk) * p.Lkv + key : -1;
-      if (c_first == c_last) {  // no row sees a key of the step
-        if (half == 0 && at >= 0) p.weights_out[at] = p.weights_in ? p.weights_in[at] : 0.f;
-        continue;
-      }
-      if (half == 1) {
-        sums[(mine & 3) * 2 * BT] = part;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(sum_bar(mine));
-      } else {
-        if (holds) finish(mine - 1);
-        held_part = part;
-        held_at = at;
-        holds = true;
-      }
-      ++mine;
     }
     if (half == 0 && holds && ok) finish(mine - 1);
   }
