@@ -76,6 +76,17 @@ def _scratch_bytes(device, tag: str, nbytes: int) -> torch.Tensor:
     return buf
 
 
+def _launch(index: int, fn, *args) -> None:
+    """One library call on device ``index``, made current for it where it is not, with its status checked."""
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args)
+    if rc:
+        _lib.check(rc)
+
+
 def _workspace(device, tag: str, nbytes: int) -> torch.Tensor:
     """:func:`_scratch_bytes`, but memory of its own while a graph is captured: graphs captured on one stream may replay on
     several at once, and a cached buffer must not outlive the graph whose pool it came from."""

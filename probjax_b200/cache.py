@@ -13,12 +13,13 @@ kernel with ``kv_lengths = positions``.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
 
 from . import _lib
-from .attention import _DTYPES, _IMPL, _ptr, _require_gpu, _scratch_bytes, _status_word, _stream, _wants_grad, mha
+from .attention import _DTYPES, _IMPL, _launch, _ptr, _require_gpu, _scratch_bytes, _status_word, _stream, _wants_grad, mha
 from .drafts import accept_drafts, decode_tree
 from .eviction import decode_weights, evict, key_weights
 from .masks import CausalFromBottomRightMask, KVLenMask
@@ -170,13 +171,15 @@ def _rope_axes_call(x, positions, sections, base, shared, interleaved, inverse, 
     if (x.stride(3) != 1 and D > 1) or (x.stride(2) != D and H > 1):
         x = x.contiguous()
     y = torch.empty((B, T, H, D), dtype=x.dtype, device=x.device) if out is None else out
-    with torch.cuda.device(x.device):
-        rc = _lib.lib().pjx_rope_axes(_ptr(x), x.stride(0) if B > 1 else 0, x.stride(1) if T > 1 else 0, _ptr(y), _ptr(positions),
-                                      _POSITION_TYPES[positions.dtype], 0 if positions.shape[0] == 1 else positions.stride(0), len(sections),
-                                      (ctypes.c_int32 * len(sections))(*sections), B, T, H, D, int(shared), int(interleaved), int(inverse),
-                                      float(base), _DTYPES[x.dtype], _stream(x.device))
-    _lib.check(rc)
+    _launch(x.get_device(), _lib.lib().pjx_rope_axes, _ptr(x), x.stride(0) if B > 1 else 0, x.stride(1) if T > 1 else 0, _ptr(y), _ptr(positions),
+            _POSITION_TYPES[positions.dtype], 0 if positions.shape[0] == 1 else positions.stride(0), len(sections), _section_array(sections), B, T,
+            H, D, int(shared), int(interleaved), int(inverse), float(base), _DTYPES[x.dtype], _stream(x.device))
     return y
+
+
+@functools.lru_cache(maxsize=64)
+def _section_array(sections):
+    return (ctypes.c_int32 * len(sections))(*sections)
 
 
 class _RopeAxesFunction(torch.autograd.Function):
@@ -213,16 +216,17 @@ def rope_axes(x: torch.Tensor, positions, sections, *, base: float = 10_000.0, s
     sections = tuple(int(s) for s in sections)
     T, H, D = x.shape[-3:]
     lead = tuple(x.shape[:-3])
-    pos = torch.as_tensor(positions)
+    pos = positions if isinstance(positions, torch.Tensor) else torch.as_tensor(positions)
     if pos.dtype not in _POSITION_TYPES:
         if pos.is_complex() or pos.dtype == torch.bool:
             raise ValueError(f"positions must be numbers, got {pos.dtype}")
         pos = pos.to(torch.float32 if pos.is_floating_point() else torch.int64)
-    pos = pos.to(x.device)
-    if tuple(pos.shape) == (T, len(sections)):
+    if pos.device != x.device:
+        pos = pos.to(x.device)
+    if pos.shape == (T, len(sections)):
         pos = pos[None].contiguous()
-    elif tuple(pos.shape) == lead + (T, len(sections)):
-        pos = pos.reshape(-1, T, len(sections)).contiguous()
+    elif pos.shape == lead + (T, len(sections)):
+        pos = (pos if pos.dim() == 3 else pos.reshape(-1, T, len(sections))).contiguous()
     else:
         raise ValueError(f"positions must be [T={T}, axes={len(sections)}] or [..., T, axes] with the leading dimensions {list(lead)}, "
                          f"got {tuple(pos.shape)}")
@@ -240,7 +244,8 @@ def rope_axes(x: torch.Tensor, positions, sections, *, base: float = 10_000.0, s
             first, last = x.data_ptr(), x.data_ptr() + (sum((d - 1) * s for d, s in zip(x.shape, x.stride())) + 1) * x.element_size()
             if first < out.data_ptr() + n and out.data_ptr() < last:
                 raise ValueError("rope_axes: out overlaps x without being it")
-    return _rope_axes_call(x4, pos, sections, base, shared, interleaved, False, out).reshape(x.shape)
+    y = _rope_axes_call(x4, pos, sections, base, shared, interleaved, False, out)
+    return y if x.dim() == 4 else y.reshape(x.shape)
 
 
 def _check_layers(x, *weights) -> None:

@@ -10,18 +10,21 @@ decode branch for a ragged batch.
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
 
 from . import _lib
-from .attention import _DTYPES, _IMPL, _ptr, _require_gpu, _status_word, _stream, _workspace
+from .attention import _DTYPES, _IMPL, _launch, _ptr, _require_gpu, _status_word, _stream, _workspace
 
 
 def _token_rows(t: torch.Tensor):
     """``(tensor, sequence stride, token stride)`` of a ``[B, N, H, D]`` tensor whose heads are dense, in elements: a slice
     of a fused projection is taken as it is, anything the kernels cannot address is copied."""
     B, N, H, D = t.shape
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t, N * H * D, H * D
     es = t.element_size()
     bs, ts = t.stride(0), t.stride(1)
     dense = (t.stride(3) == 1 or D == 1) and (t.stride(2) == D or H == 1)
@@ -35,6 +38,8 @@ def _token_rows(t: torch.Tensor):
 
 
 def _int32(x, device, shape, what):
+    if isinstance(x, torch.Tensor) and x.dtype is torch.int32 and x.shape == shape and x.device == device and x.is_contiguous():
+        return x
     t = torch.as_tensor(x)
     if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
         raise ValueError(f"{what} must hold integers, got {t.dtype}")
@@ -46,30 +51,36 @@ def _int32(x, device, shape, what):
 
 def _check_cache(name, k_new, v_new, k_cache, v_cache, block_table):
     """Shapes, types and devices of drafts beside a cache: ``(B, N, Hkv, D, Dv, capacity, page_size, max_pages, num_pages, table)``."""
+    dtype = getattr(k_new, "dtype", None)
     for what, t in (("k_new", k_new), ("v_new", v_new), ("k_cache", k_cache), ("v_cache", v_cache)):
         if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() != 4:
             raise ValueError(f"{name} takes rank-4 CUDA tensors; {what} is not one")
-        if t.dtype != k_new.dtype or t.device != k_new.device:
+        if t.dtype is not dtype or t.get_device() != k_new.get_device():
             raise ValueError(f"{name}: all tensors must share a dtype and a device")
-    if k_new.dtype not in _DTYPES:
-        raise ValueError(f"unsupported dtype {k_new.dtype}; expected float32, bfloat16 or float16")
+    if dtype not in _DTYPES:
+        raise ValueError(f"unsupported dtype {dtype}; expected float32, bfloat16 or float16")
     B, N, Hkv, D = k_new.shape
-    Dv = v_new.shape[3]
-    if tuple(v_new.shape[:3]) != (B, N, Hkv):
+    vb, vn, vh, Dv = v_new.shape
+    if (vb, vn, vh) != (B, N, Hkv):
         raise ValueError(f"{name}: v_new must be [B={B}, N={N}, Hkv={Hkv}, Dv], got {tuple(v_new.shape)}")
-    if k_cache.shape[2:] != (Hkv, D) or v_cache.shape[2:] != (Hkv, Dv) or v_cache.shape[:2] != k_cache.shape[:2]:
+    rows, cap, kh, kd = k_cache.shape
+    if (kh, kd) != (Hkv, D) or v_cache.shape != (rows, cap, Hkv, Dv):
         raise ValueError(f"{name}: caches must be [.., .., Hkv={Hkv}, D={D}] and [.., .., Hkv={Hkv}, Dv={Dv}] alike, got "
                          f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
     if block_table is None:
-        if k_cache.shape[0] != B:
-            raise ValueError(f"{name}: the cache holds {k_cache.shape[0]} sequences, the drafts {B}")
-        return B, N, Hkv, D, Dv, k_cache.shape[1], 0, 0, 0, None
+        if rows != B:
+            raise ValueError(f"{name}: the cache holds {rows} sequences, the drafts {B}")
+        return B, N, Hkv, D, Dv, cap, 0, 0, 0, None
     table = torch.as_tensor(block_table)
     if table.dim() != 2 or table.shape[0] != B:
         raise ValueError(f"block_table must be [B={B}, max_pages], got {tuple(table.shape)}")
     table = _int32(table, k_new.device, table.shape, "block_table")
-    page = k_cache.shape[1]
-    return B, N, Hkv, D, Dv, table.shape[1] * page, page, table.shape[1], k_cache.shape[0], table
+    return B, N, Hkv, D, Dv, table.shape[1] * cap, cap, table.shape[1], rows, table
+
+
+@functools.lru_cache(maxsize=256)
+def _tree_workspace(*sizes) -> int:
+    return _lib.lib().pjx_attn_decode_tree_workspace_bytes(*sizes)
 
 
 def decode_tree(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, parents, *,
@@ -89,15 +100,16 @@ def decode_tree(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_cac
         raise ValueError(f"implementation must be None or one of {sorted(k for k in _IMPL if k)}")
     B, N, Hkv, D, Dv, cap, page, max_pages, num_pages, table = _check_cache("decode_tree", k_new, v_new, k_cache, v_cache, block_table)
     dev = k_new.device
-    if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.device != dev or q.dtype != k_new.dtype:
+    if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.device != dev or q.dtype is not k_new.dtype:
         raise ValueError("decode_tree: q must be a rank-4 tensor of the drafts' dtype and device")
     Hq = q.shape[2]
-    if tuple(q.shape) != (B, N, Hq, D):
+    if q.shape != (B, N, Hq, D):
         raise ValueError(f"decode_tree: q must be [B={B}, N={N}, Hq, D={D}], got {tuple(q.shape)}")
     if Hq < 1 or Hkv < 1 or Hq % Hkv != 0:
         raise ValueError(f"query heads ({Hq}) must be a multiple of key/value heads ({Hkv})")
     lengths = _int32(kv_lengths, dev, (B,), "kv_lengths")
-    parents = torch.as_tensor(parents)
+    if not isinstance(parents, torch.Tensor):
+        parents = torch.as_tensor(parents)
     tree = _int32(parents, dev, (N,) if parents.dim() == 1 else (B, N), "parents")
     q, qb, qt = _token_rows(q)
     k_new, kb, kt = _token_rows(k_new)
@@ -105,15 +117,11 @@ def decode_tree(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_cac
     k_cache, v_cache = k_cache.contiguous(), v_cache.contiguous()
     o = torch.empty((B, N, Hq, Dv), dtype=q.dtype, device=dev)
     lse = torch.empty((B, Hq, N), dtype=torch.float32, device=dev) if return_lse else None
-    L = _lib.lib()
-    ws = _workspace(dev, "tree", L.pjx_attn_decode_tree_workspace_bytes(B, N, Hq, Hkv, Dv, cap))
-    with torch.cuda.device(dev):
-        rc = L.pjx_attn_decode_tree(_ptr(q), qb, qt, _ptr(k_new), kb, kt, _ptr(v_new), vb, vt, _ptr(k_cache), _ptr(v_cache), _ptr(tree),
-                                    0 if tree.dim() == 1 else N, _ptr(lengths), _ptr(table), _ptr(o), _ptr(lse), B, N, Hq, Hkv, D, Dv,
-                                    cap, page, max_pages, num_pages, _DTYPES[q.dtype],
-                                    1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), _IMPL[implementation], _ptr(ws),
-                                    ws.numel(), _ptr(_status_word(dev)), _stream(dev))
-    _lib.check(rc)
+    ws = _workspace(dev, "tree", _tree_workspace(B, N, Hq, Hkv, Dv, cap))
+    _launch(dev.index, _lib.lib().pjx_attn_decode_tree, _ptr(q), qb, qt, _ptr(k_new), kb, kt, _ptr(v_new), vb, vt, _ptr(k_cache),
+            _ptr(v_cache), _ptr(tree), 0 if tree.dim() == 1 else N, _ptr(lengths), _ptr(table), _ptr(o), _ptr(lse), B, N, Hq, Hkv, D, Dv, cap,
+            page, max_pages, num_pages, _DTYPES[q.dtype], 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), _IMPL[implementation],
+            _ptr(ws), ws.numel(), _ptr(_status_word(dev)), _stream(dev))
     return (o, lse) if return_lse else o
 
 
@@ -129,21 +137,21 @@ def accept_drafts(k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Tenso
     if not k_cache.is_contiguous() or not v_cache.is_contiguous():
         raise ValueError("accept_drafts writes the caches in place: they must be contiguous")
     lengths = _int32(kv_lengths, dev, (B,), "kv_lengths")
-    path = torch.as_tensor(path)
+    if not isinstance(path, torch.Tensor):
+        path = torch.as_tensor(path)
     if path.dim() != 2:
         raise ValueError(f"path must be [B={B}, P], got {tuple(path.shape)}")
     path = _int32(path, dev, (B, path.shape[1]), "path")
     counts = _int32(counts, dev, (B,), "counts")
+    given = out
     if out is None:
-        out = torch.empty((B,), dtype=torch.int32, device=dev)
-    for what, t, n in (("out", out, B), ("overflow", overflow, 1)):
+        out = torch.empty_like(lengths)
+    for what, t, n in (("out", given, B), ("overflow", overflow, 1)):
         if t is not None and (tuple(t.shape) != (n,) or t.dtype != torch.int32 or t.device != dev or not t.is_contiguous()):
             raise ValueError(f"accept_drafts: {what} must be a contiguous int32 [{n}] on {dev}")
     k_new, kb, kt = _token_rows(k_new)
     v_new, vb, vt = _token_rows(v_new)
-    with torch.cuda.device(dev):
-        rc = _lib.lib().pjx_kv_cache_accept(_ptr(k_cache), _ptr(v_cache), _ptr(k_new), kb, kt, _ptr(v_new), vb, vt, _ptr(lengths), _ptr(path),
-                                            _ptr(counts), _ptr(table), B, N, path.shape[1], Hkv, D, Dv, cap, page, max_pages, num_pages,
-                                            _DTYPES[k_new.dtype], _ptr(out), _ptr(overflow), _stream(dev))
-    _lib.check(rc)
+    _launch(dev.index, _lib.lib().pjx_kv_cache_accept, _ptr(k_cache), _ptr(v_cache), _ptr(k_new), kb, kt, _ptr(v_new), vb, vt, _ptr(lengths),
+            _ptr(path), _ptr(counts), _ptr(table), B, N, path.shape[1], Hkv, D, Dv, cap, page, max_pages, num_pages, _DTYPES[k_new.dtype],
+            _ptr(out), _ptr(overflow), _stream(dev))
     return out

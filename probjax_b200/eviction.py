@@ -9,12 +9,13 @@ The reference's cache only grows (probjax/nn/layers/attention.py:631-643, 727-75
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
 
 from . import _lib
-from .attention import (_DTYPES, _IMPL, _as_tensor, _band_args, _check_call, _ptr, _require_gpu, _status_word, _stream, _workspace)
+from .attention import (_DTYPES, _IMPL, _as_tensor, _band_args, _check_call, _launch, _ptr, _require_gpu, _status_word, _stream, _workspace)
 from .drafts import _int32
 from .masks import AttentionMask, split_mask
 
@@ -22,7 +23,7 @@ from .masks import AttentionMask, split_mask
 def _weights_args(what, weights, out, shape, dev):
     """``(weights, out)`` as float32 tensors of ``shape``; ``out`` is made where it is not given."""
     for name, t in (("weights", weights), ("out", out)):
-        if t is not None and (tuple(t.shape) != shape or t.dtype != torch.float32 or t.device != dev):
+        if t is not None and (t.shape != shape or t.dtype is not torch.float32 or t.device != dev):
             raise ValueError(f"{what}: {name} must be float32 {list(shape)} on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     if out is None:
         out = torch.empty(shape, dtype=torch.float32, device=dev)
@@ -36,6 +37,11 @@ def _weights_args(what, weights, out, shape, dev):
     elif weights is not None and not weights.is_contiguous():
         raise ValueError(f"{what}: weights that are also the result must be contiguous")
     return weights, out
+
+
+@functools.lru_cache(maxsize=256)
+def _decode_workspace(*sizes) -> int:
+    return _lib.lib().pjx_attn_decode_weights_workspace_bytes(*sizes)
 
 
 def decode_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor | None = None, *, kv_lengths=None,
@@ -61,13 +67,10 @@ def decode_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         elif weights.data_ptr() != out.data_ptr():
             out.copy_(weights)
         return (o, lse, out) if return_lse else (o, out)
-    L = _lib.lib()
-    ws = _workspace(dev, "decode_weights", L.pjx_attn_decode_weights_workspace_bytes(B, Lq, Hq, Hkv, Dv, cap, int(split_len)))
-    with torch.cuda.device(dev):
-        rc = L.pjx_attn_decode_weights(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(lengths), _ptr(weights), _ptr(out), _ptr(o), _ptr(lse),
-                                       B, Lq, Hq, Hkv, D, Dv, cap, _DTYPES[q.dtype], 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale),
-                                       int(split_len), _ptr(ws), ws.numel(), _ptr(_status_word(dev)), _stream(dev))
-    _lib.check(rc)
+    ws = _workspace(dev, "decode_weights", _decode_workspace(B, Lq, Hq, Hkv, Dv, cap, int(split_len)))
+    _launch(dev.index, _lib.lib().pjx_attn_decode_weights, _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(lengths), _ptr(weights), _ptr(out),
+            _ptr(o), _ptr(lse), B, Lq, Hq, Hkv, D, Dv, cap, _DTYPES[q.dtype], 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale),
+            int(split_len), _ptr(ws), ws.numel(), _ptr(_status_word(dev)), _stream(dev))
     return (o, lse, out) if return_lse else (o, out)
 
 
@@ -96,11 +99,9 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, weights:
     weights, out = _weights_args("key_weights", weights, out, (B, Hkv, Lkv), dev)
     q, k, lse = q.contiguous(), k.contiguous(), lse.contiguous()
     band_lo, band_hi = _band_args(False, lm.band)
-    with torch.cuda.device(dev):
-        rc = _lib.lib().pjx_attn_key_weights(_ptr(q), _ptr(k), _ptr(lse), _ptr(weights), _ptr(out), _ptr(lengths), B, Lq, Lkv, Hq, Hkv, D,
-                                             _DTYPES[q.dtype], band_lo, band_hi, 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale),
-                                             _IMPL[implementation], _ptr(_status_word(dev)), _stream(dev))
-    _lib.check(rc)
+    _launch(dev.index, _lib.lib().pjx_attn_key_weights, _ptr(q), _ptr(k), _ptr(lse), _ptr(weights), _ptr(out), _ptr(lengths), B, Lq, Lkv, Hq,
+            Hkv, D, _DTYPES[q.dtype], band_lo, band_hi, 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), _IMPL[implementation],
+            _ptr(_status_word(dev)), _stream(dev))
     return out
 
 
@@ -122,29 +123,26 @@ def evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor, k
         raise ValueError(f"unsupported dtype {k_cache.dtype}; expected float32, bfloat16 or float16")
     B, cap, Hkv, D = k_cache.shape
     Dv = v_cache.shape[3]
-    if tuple(v_cache.shape[:3]) != (B, cap, Hkv) or v_cache.dtype != k_cache.dtype or v_cache.device != dev:
+    if v_cache.shape[:3] != (B, cap, Hkv) or v_cache.dtype is not k_cache.dtype or v_cache.device != dev:
         raise ValueError(f"evict: v_cache must be [B={B}, capacity={cap}, Hkv={Hkv}, Dv] of the keys' dtype and device, got {tuple(v_cache.shape)}")
-    if int(keep) < 1 or not 0 <= int(recent) <= int(keep):
+    keep, recent = int(keep), int(recent)
+    if keep < 1 or not 0 <= recent <= keep:
         raise ValueError(f"evict: keep must be positive and recent in [0, keep], got keep={keep}, recent={recent}")
     lengths = _int32(kv_lengths, dev, (B,), "kv_lengths")
     ko, vo, wo = (k_cache, v_cache, weights) if out is None else out
     cap_out = ko.shape[1] if ko.dim() == 4 else -1
     for name, t, shape, dtype in (("weights", weights, (B, Hkv, cap), torch.float32), ("out keys", ko, (B, cap_out, Hkv, D), k_cache.dtype),
                                   ("out values", vo, (B, cap_out, Hkv, Dv), k_cache.dtype), ("out weights", wo, (B, Hkv, cap_out), torch.float32)):
-        if tuple(t.shape) != shape or t.dtype != dtype or t.device != dev or not t.is_contiguous():
+        if t.shape != shape or t.dtype is not dtype or t.device != dev or not t.is_contiguous():
             raise ValueError(f"evict: {name} must be a contiguous {dtype} {list(shape)} on {dev}, got {t.dtype} {tuple(t.shape)}")
     if not k_cache.is_contiguous() or not v_cache.is_contiguous():
         raise ValueError("evict: the caches must be contiguous")
     if lengths_out is None:
-        lengths_out = torch.empty((B,), dtype=torch.int32, device=dev)
+        lengths_out = torch.empty_like(lengths)
     elif tuple(lengths_out.shape) != (B,) or lengths_out.dtype != torch.int32 or lengths_out.device != dev or not lengths_out.is_contiguous():
         raise ValueError(f"evict: lengths_out must be a contiguous int32 [{B}] on {dev}")
-    kept = torch.empty((B, Hkv, int(keep)), dtype=torch.int32, device=dev)
-    L = _lib.lib()
-    ws = _workspace(dev, "evict", L.pjx_kv_cache_evict_workspace_bytes(B, Hkv))
-    with torch.cuda.device(dev):
-        rc = L.pjx_kv_cache_evict(_ptr(k_cache), _ptr(v_cache), _ptr(weights), _ptr(lengths), _ptr(ko), _ptr(vo), _ptr(wo), _ptr(lengths_out),
-                                  _ptr(kept), B, Hkv, D, Dv, cap, cap_out, int(keep), int(recent), _DTYPES[k_cache.dtype], _ptr(ws), ws.numel(),
-                                  _stream(dev))
-    _lib.check(rc)
+    kept = torch.empty((B, Hkv, keep), dtype=torch.int32, device=dev)
+    ws = _workspace(dev, "evict", 8 * B * Hkv)  # pjx_kv_cache_evict_workspace_bytes
+    _launch(dev.index, _lib.lib().pjx_kv_cache_evict, _ptr(k_cache), _ptr(v_cache), _ptr(weights), _ptr(lengths), _ptr(ko), _ptr(vo), _ptr(wo),
+            _ptr(lengths_out), _ptr(kept), B, Hkv, D, Dv, cap, cap_out, keep, recent, _DTYPES[k_cache.dtype], _ptr(ws), ws.numel(), _stream(dev))
     return lengths_out, kept
