@@ -64,8 +64,10 @@ __global__ void __cluster_dims__(kAcceptCluster, 1, 1) __launch_bounds__(256) kv
 
 // ------------------------------------------------------------------------------------------------ evict: selection
 
-constexpr int kSelThreads = 512;
-constexpr int kBins = 2048;
+constexpr int kSelThreads = 1024;
+constexpr int kBins = 8192;
+constexpr int kBinsPerThread = kBins / kSelThreads;
+constexpr int kHeldKeys = 32768;  // keys of a CTA that stay in shared memory (128 KB beside 32 KB of bins)
 
 struct EvictParams {
   const float* weights;      // [B, Hkv, capacity]
@@ -81,6 +83,7 @@ struct EvictParams {
   int cap_out, in_place;
   int row_k, row_v;          // bytes of a row of one head
   int slices_k, slices_v, slice_units, row_splits;
+  int held_keys;             // keys of a slice that stay in shared memory
 };
 
 // Order of the weights as unsigned integers: larger is better, NaN is worst, -0 equals 0.
@@ -112,16 +115,20 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* scratch, ui
   return x + before;
 }
 
-// A cluster per (sequence, head), a slice of the keys per CTA.  The threshold -- the weight of rank keep - recent -- is found digit by
-// digit (11, 11 and 10 bits) with a histogram per CTA that the cluster adds up through distributed shared memory; exact, so ties
-// can be cut by index.  A last pass numbers the kept keys in order.
+// A CTA per (sequence, head), or a cluster with a slice of the keys per CTA.  The weights are read once and stay in shared memory as
+// integers of the same order (what lies past 32768 keys a CTA is read again).  The threshold -- the weight of rank keep - recent --
+// is found digit by digit with a histogram per CTA that the cluster adds up through distributed shared memory; exact, so ties can
+// be cut by index.  13 bits of the first digit hold four mantissa bits: with two, weights that span a few octaves meet
+// in so few bins that the additions queue.  A last pass numbers the kept keys in order.
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictParams p) {
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
   const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
-  __shared__ uint32_t hist[kBins];
+  extern __shared__ uint32_t select_smem[];
+  uint32_t* hist = select_smem;           // [kBins]
+  uint32_t* held_keys = hist + kBins;     // the slice's first p.held_keys keys
   __shared__ uint32_t scratch[kSelThreads / 32];
-  __shared__ uint32_t found[2];     // digit and the count still wanted inside it
+  __shared__ uint32_t found[3];     // digit, the count still wanted inside it, and its keys
   __shared__ uint32_t counts[2];    // keys of this slice above the threshold, and equal to it
   const int64_t unit = (int64_t)b * p.Hkv + h;
   const float* w = p.weights + unit * p.capacity;
@@ -138,67 +145,100 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictPa
   if (want == 0) return;
   const int per = ((old + ranks - 1) / ranks + 3) / 4 * 4;
   const int begin = min(old, rank * per), end = min(old, begin + per);
+  {  // eight loads in flight per thread
+    const int stop = min(end, begin + p.held_keys);
+    int j = begin + tid;
+    for (; j + 7 * kSelThreads < stop; j += 8 * kSelThreads) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = w[j + e * kSelThreads];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) held_keys[j + e * kSelThreads - begin] = weight_order(x[e]);
+    }
+    for (; j < stop; j += kSelThreads) held_keys[j - begin] = weight_order(w[j]);
+  }
+  auto sync = [&] {
+    if (ranks == 1)
+      __syncthreads();
+    else
+      cluster.sync();
+  };
+  auto key_at = [&](int j) { return j - begin < p.held_keys ? held_keys[j - begin] : weight_order(w[j]); };
   uint32_t prefix = 0, rest = (uint32_t)want;
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
-    constexpr int kShift[3] = {21, 10, 0}, kBits[3] = {11, 11, 10};
+    constexpr int kShift[3] = {19, 6, 0}, kBits[3] = {13, 13, 6};
     const int shift = kShift[pass], bits = kBits[pass];
     const uint32_t high = pass == 0 ? 0u : ~0u << (shift + bits);
     for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
     __syncthreads();
     for (int j = begin + tid; j < end; j += kSelThreads) {
-      const uint32_t key = weight_order(w[j]);
+      const uint32_t key = key_at(j);
       if ((key & high) == prefix) atomicAdd(&hist[(key >> shift) & ((1u << bits) - 1)], 1u);
     }
-    cluster.sync();
-    // bins from the top: thread i takes the four below kBins - 4 i
-    uint32_t bin[4], sum = 0;
+    sync();
+    // bins from the top: thread i takes the next kBinsPerThread below kBins - kBinsPerThread i
+    uint32_t bin[kBinsPerThread] = {}, sum = 0;
+    for (int r = 0; r < ranks; ++r) {
+      const uint4* theirs = reinterpret_cast<const uint4*>(ranks == 1 ? hist : cluster.map_shared_rank(hist, r)) + (kSelThreads - 1 - tid) * (kBinsPerThread / 4);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      bin[e] = 0;
-      for (int r = 0; r < ranks; ++r) bin[e] += cluster.map_shared_rank(hist, r)[kBins - 1 - (4 * tid + e)];
-      sum += bin[e];
+      for (int v = 0; v < kBinsPerThread / 4; ++v) {
+        const uint4 x = theirs[v];
+        bin[kBinsPerThread - 1 - 4 * v] += x.x;
+        bin[kBinsPerThread - 2 - 4 * v] += x.y;
+        bin[kBinsPerThread - 3 - 4 * v] += x.z;
+        bin[kBinsPerThread - 4 - 4 * v] += x.w;
+      }
     }
+#pragma unroll
+    for (int e = 0; e < kBinsPerThread; ++e) sum += bin[e];
     uint32_t total;
     uint32_t before = block_scan(sum, scratch, total) - sum;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < kBinsPerThread; ++e) {
       if (before < rest && before + bin[e] >= rest) {
-        found[0] = (uint32_t)(kBins - 1 - (4 * tid + e));
+        found[0] = (uint32_t)(kBins - 1 - (kBinsPerThread * tid + e));
         found[1] = rest - before;
+        found[2] = bin[e];
       }
       before += bin[e];
     }
-    cluster.sync();  // (the histograms have been read; `found` is written)
+    sync();  // (the histograms have been read; `found` is written)
     prefix |= found[0] << shift;
     rest = found[1];
+    if (rest == found[2]) {  // the whole bin is kept: everything above its lowest value less one
+      --prefix;
+      rest = 0;
+      break;
+    }
   }
-  // keys above the threshold and equal to it in the slices before this one
-  uint32_t above = 0, equal = 0;
-  for (int j = begin + tid; j < end; j += kSelThreads) {
-    const uint32_t key = weight_order(w[j]);
-    above += key > prefix;
-    equal += key == prefix;
-  }
-  uint32_t t_above, t_equal;
-  block_scan(above, scratch, t_above);
-  block_scan(equal, scratch, t_equal);
-  if (tid == 0) {
-    counts[0] = t_above;
-    counts[1] = t_equal;
-  }
-  cluster.sync();
-  uint32_t run_above = 0, run_equal = 0;
-  for (int r = 0; r < rank; ++r) {
-    run_above += cluster.map_shared_rank(counts, r)[0];
-    run_equal += cluster.map_shared_rank(counts, r)[1];
+  uint32_t run_above = 0, run_equal = 0;  // keys above the threshold, and equal to it, in the slices before this one
+  if (ranks > 1) {
+    uint32_t above = 0, equal = 0;
+    for (int j = begin + tid; j < end; j += kSelThreads) {
+      const uint32_t key = key_at(j);
+      above += key > prefix;
+      equal += key == prefix;
+    }
+    uint32_t t_above, t_equal;
+    block_scan(above, scratch, t_above);
+    block_scan(equal, scratch, t_equal);
+    if (tid == 0) {
+      counts[0] = t_above;
+      counts[1] = t_equal;
+    }
+    cluster.sync();
+    for (int r = 0; r < rank; ++r) {
+      run_above += cluster.map_shared_rank(counts, r)[0];
+      run_equal += cluster.map_shared_rank(counts, r)[1];
+    }
   }
   for (int j0 = begin; j0 < end; j0 += kSelThreads * 4) {
     uint32_t key[4], packed = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int j = j0 + tid * 4 + e;
-      key[e] = j < end ? weight_order(w[j]) : 0u;
+      key[e] = j < end ? key_at(j) : 0u;
       if (j < end) packed += key[e] > prefix ? 0x10000u : key[e] == prefix ? 1u : 0u;
     }
     uint32_t total;
@@ -219,7 +259,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictPa
     run_above += total >> 16;
     run_equal += total & 0xffffu;
   }
-  cluster.sync();  // (no CTA leaves while another may read its shared memory)
+  sync();  // (no CTA leaves while another may read its shared memory)
 }
 
 // ------------------------------------------------------------------------------------------------ evict: movement
@@ -382,11 +422,19 @@ int pjx_kv_cache_evict(const void* k_cache, const void* v_cache, const float* we
   p.row_k = (int)(D * es); p.row_v = (int)(Dv * es);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
 
-  int ranks = 8;
-  while (ranks > 1 && capacity <= ranks / 2 * 2048) ranks /= 2;  // at least 2048 keys a CTA
+  // a CTA per (sequence, head) up to 32768 keys, a cluster beyond
+  int ranks = 1;
+  while (ranks < 8 && capacity > ranks * kHeldKeys) ranks *= 2;
+  p.held_keys = ((capacity + ranks - 1) / ranks + 3) / 4 * 4;
+  if (p.held_keys > kHeldKeys) p.held_keys = kHeldKeys;
+  const size_t select_smem = (size_t)(kBins + p.held_keys) * sizeof(uint32_t);
+  int rc = check_cuda(cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kBins + kHeldKeys) * (int)sizeof(uint32_t)),
+                      "cudaFuncSetAttribute(evict)");
+  if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ranks, Hkv, B);
   cfg.blockDim = dim3(kSelThreads);
+  cfg.dynamicSmemBytes = select_smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -395,7 +443,7 @@ int pjx_kv_cache_evict(const void* k_cache, const void* v_cache, const float* we
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  int rc = check_cuda(cudaLaunchKernelEx(&cfg, evict_select_kernel, p), "evict selection launch");
+  rc = check_cuda(cudaLaunchKernelEx(&cfg, evict_select_kernel, p), "evict selection launch");
   count_launch();
   if (rc) return rc;
 

@@ -2,9 +2,9 @@
 // every token of every sequence: pair (a, b) of a head vector becomes (a cos - b sin, b cos + a sin) of the angle
 // positions[b, t, axis(pair)] * frequency(pair).  The gradient is the rotation by the negative angle, the same kernel.
 //
-// Bound by HBM: the tensor is read once and written once, 16 bytes per access.  A CTA takes a few tokens.  Its threads
-// first compute the tokens' cosines and sines, one angle each, into shared memory, and the H heads of the tokens share
-// them.  The angle is taken in turns in 64 bits (a position of 10^6 times a frequency near 1 would lose five digits in 32)
+// Bound by HBM: the tensor is read once and written once, 16 bytes per access.  A CTA takes a few tokens.  Its threads issue
+// their first loads, compute the tokens' cosines and sines meanwhile, one angle each, into shared memory, and the H heads of
+// the tokens share them.  The angle is taken in turns in 64 bits (a position of 10^6 times a frequency near 1 would lose five digits in 32)
 // and reduced to half a turn before it is rounded: two 64-bit operations per (token, pair), nothing next to the traffic.
 #include <math.h>
 #include <string.h>
@@ -32,6 +32,7 @@ struct RopeAxesParams {
   int64_t pos_bs;      // entries between sequences of positions (0: shared)
   int64_t tokens;      // B * T
   int T, H, D, axes, pairs, pos_type, inverse, tokens_per_cta;
+  uint32_t inv_heads;  // ceil(2^32 / H): the token of a head vector by a multiplication (H > 1; at most 2^16 vectors a CTA)
 };
 
 __device__ __forceinline__ double load_position(const RopeAxesParams& p, int64_t at) {
@@ -52,20 +53,29 @@ __device__ __forceinline__ void rotate(T& a, T& b, float2 cs) {
 template <typename T, bool HALVES, bool VEC>
 __global__ void __launch_bounds__(kThreads) rope_axes_kernel(const RopeAxesParams p, const __grid_constant__ RopeAxesTable table) {
   extern __shared__ float2 cs[];  // [tokens of the CTA][pairs]
+  __shared__ int64_t from[kTableAngles];  // where the tokens lie in x
   const int64_t n0 = (int64_t)blockIdx.x * p.tokens_per_cta;
   const int n_tok = (int)min((int64_t)p.tokens_per_cta, p.tokens - n0);
-  for (int i = threadIdx.x; i < n_tok * p.pairs; i += kThreads) {
-    const int tok = i / p.pairs, pair = i - tok * p.pairs;
-    const int64_t n = n0 + tok, b = n / p.T, t = n - b * p.T;
-    const double turns = load_position(p, b * p.pos_bs + t * p.axes + table.axis[pair]) * table.turns[pair];
-    float s, c;
-    sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
-    cs[i] = make_float2(c, p.inverse ? -s : s);
-  }
-  __syncthreads();
   const T* x = static_cast<const T*>(p.x);
   T* y = static_cast<T*>(p.y);
   const int vectors = n_tok * p.H;  // head vectors of the CTA
+  for (int i = threadIdx.x; i < n_tok; i += kThreads) {
+    const int64_t b = (n0 + i) / p.T;
+    from[i] = b * p.x_bs + (n0 + i - b * p.T) * p.x_ts;
+  }
+  __syncthreads();
+  auto token_of = [&](int v) { return (int)__umulhi((unsigned)v, p.inv_heads) + (p.H == 1 ? v : 0); };
+  auto angles = [&] {
+    for (int i = threadIdx.x; i < n_tok * p.pairs; i += kThreads) {
+      const int tok = i / p.pairs, pair = i - tok * p.pairs;
+      const int64_t n = n0 + tok, b = n / p.T, t = n - b * p.T;
+      const double turns = load_position(p, b * p.pos_bs + t * p.axes + table.axis[pair]) * table.turns[pair];
+      float s, c;
+      sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
+      cs[i] = make_float2(c, p.inverse ? -s : s);
+    }
+    __syncthreads();
+  };
   if constexpr (VEC) {
     constexpr int V = 16 / sizeof(T);
     // units of a head vector: HALVES V pairs each (two accesses) and then the columns that do not rotate
@@ -73,29 +83,32 @@ __global__ void __launch_bounds__(kThreads) rope_axes_kernel(const RopeAxesParam
     const int units = HALVES ? pair_units + (p.D - 2 * p.pairs) / V : p.D / V;
     const int rows = kThreads / units;
     const int u = threadIdx.x % units, row = threadIdx.x / units;
-    if (row >= rows) return;
+    const bool active = row < rows;
     const bool two = HALVES && u < pair_units;
     const int d0 = HALVES ? (two ? u * V : 2 * p.pairs + (u - pair_units) * V) : u * V;
-    constexpr int UN = 4;
-    for (int v0 = row; v0 < vectors; v0 += UN * rows) {
-      uint4 lo[UN], hi[UN];
+    constexpr int UN = HALVES ? 4 : 8;
+    uint4 lo[UN], hi[HALVES ? UN : 1];
+    auto load = [&](int v0) {
 #pragma unroll
       for (int k = 0; k < UN; ++k) {
         const int v = v0 + k * rows;
-        if (v >= vectors) break;
-        const int tok = v / p.H, h = v - tok * p.H;
-        const int64_t n = n0 + tok, b = n / p.T;
-        const T* src = x + b * p.x_bs + (n - b * p.T) * p.x_ts + (int64_t)h * p.D + d0;
+        if (!active || v >= vectors) break;
+        const int tok = token_of(v);
+        const T* src = x + from[tok] + (int64_t)(v - tok * p.H) * p.D + d0;
         lo[k] = *reinterpret_cast<const uint4*>(src);
         if (two) hi[k] = *reinterpret_cast<const uint4*>(src + p.pairs);
       }
+    };
+    load(row);
+    angles();
+    for (int v0 = row; active && v0 < vectors; v0 += UN * rows) {
+      if (v0 != row) load(v0);
 #pragma unroll
       for (int k = 0; k < UN; ++k) {
         const int v = v0 + k * rows;
         if (v >= vectors) break;
-        const int tok = v / p.H;
         T* dst = y + (n0 * p.H + v) * (int64_t)p.D + d0;
-        const float2* c = cs + tok * p.pairs;
+        const float2* c = cs + token_of(v) * p.pairs;
         T* a = reinterpret_cast<T*>(&lo[k]);
         if (two) {
           T* b = reinterpret_cast<T*>(&hi[k]);
@@ -111,12 +124,12 @@ __global__ void __launch_bounds__(kThreads) rope_axes_kernel(const RopeAxesParam
       }
     }
   } else {
+    angles();
     const int items = p.pairs + (p.D - 2 * p.pairs);  // pairs, then single columns
     for (int64_t i = threadIdx.x; i < (int64_t)vectors * items; i += kThreads) {
       const int v = (int)(i / items), it = (int)(i - (int64_t)v * items);
       const int tok = v / p.H, h = v - tok * p.H;
-      const int64_t n = n0 + tok, b = n / p.T;
-      const T* src = x + b * p.x_bs + (n - b * p.T) * p.x_ts + (int64_t)h * p.D;
+      const T* src = x + from[tok] + (int64_t)h * p.D;
       T* dst = y + (n0 * p.H + v) * (int64_t)p.D;
       if (it < p.pairs) {
         const int ia = HALVES ? it : 2 * it, ib = HALVES ? p.pairs + it : 2 * it + 1;
@@ -187,10 +200,12 @@ extern "C" int pjx_rope_axes(const void* x, int64_t x_batch_stride, int64_t x_to
   const int64_t most = pair > 0 ? (kTableAngles / pair < 1 ? 1 : kTableAngles / pair) : 8;
   int64_t tok = p.tokens / (148 * 8);
   tok = tok < 1 ? 1 : tok > most ? most : tok;
+  while (tok > 1 && tok * H > 65536) --tok;
   p.tokens_per_cta = (int)tok;
+  p.inv_heads = H > 1 ? (uint32_t)(((1ull << 32) + H - 1) / H) : 0u;
   const size_t es = dtype_size(dtype);
   const int V = (int)(16 / es);
-  const bool vec = D % V == 0 && D / V <= kThreads && (interleaved || pair % V == 0) && x_batch_stride % V == 0 && x_token_stride % V == 0 &&
+  const bool vec = D % V == 0 && D / V <= kThreads && H <= 65536 && (interleaved || pair % V == 0) && x_batch_stride % V == 0 && x_token_stride % V == 0 &&
                    ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 15) == 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (dtype) {
