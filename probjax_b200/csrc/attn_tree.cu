@@ -70,6 +70,10 @@ __global__ void __launch_bounds__(NT) attn_tree_kernel(const TreeParams p) {
     const int b = sg.b, hk = sg.column / row_tiles, r0 = (sg.column - hk * row_tiles) * BM;
     const int prefix_tiles = (sg.prefix + kTreeTile - 1) / kTreeTile;
     const int32_t* parents = p.parents + b * p.parents_bs;
+    if (tid == 0) {  // the combine's list
+      if (sg.first == 0) p.slots[2 * sg.pair] = (int)sg.slot;
+      if (sg.last) p.slots[2 * sg.pair + 1] = (int)sg.slot;
+    }
     __syncthreads();  // the segment before is done with shared memory
     if (tid < BM) {
 #pragma unroll
@@ -196,71 +200,79 @@ __global__ void __launch_bounds__(NT) attn_tree_kernel(const TreeParams p) {
   }
 }
 
-// Exact combine of a row's segments, a warp per row.  Rows of absent drafts come out empty whatever the segments hold.
+// Exact combine of a row's segments by a warp, `each` rows a warp.  Rows of absent drafts come out empty whatever the segments hold.
 template <typename TO>
-__global__ void __launch_bounds__(256) tree_combine_kernel(const TreeParams p) {
-  const int b = blockIdx.y, lane = threadIdx.x & 31;
-  const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= p.N * p.Hq) return;
-  const int t = row / p.Hq, h = row - t * p.Hq, G = p.Hq / p.Hkv, hk = h / G;
-  const int r = t * G + h - hk * G, column = hk * (p.columns / p.Hkv) + r / p.column_rows;
-  // (the lengths and the tree only: before the wait for the segments)
-  const bool there = tree_present(p.parents + b * p.parents_bs, t);
-  const TreeLine line = tree_line(p);
-  int before = 0;
-  for (int i = lane; i < b; i += 32) before += tree_tiles(p, tree_prefix(p, i));
-  before = __reduce_add_sync(0xffffffffu, before);
-  const int64_t from = (int64_t)column * line.tiles + before, last = from + tree_tiles(p, tree_prefix(p, b)) - 1;
-  auto cta_of = [&](int64_t pos) { return ((pos + 1) * line.ctas - 1) / line.length; };
-  const int64_t first = cta_of(from);
-  const int ns = (int)(cta_of(last) - first) + 1;
-  const int64_t base = (first + (int64_t)column * p.B + b) * p.column_rows + r % p.column_rows;
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  const float* lses = p.lse_part + base;
-  float m = -INFINITY;
-  if (there)
-    for (int s = lane; s < ns; s += 32) m = fmaxf(m, lses[(int64_t)s * p.column_rows]);
+__global__ void __launch_bounds__(256) tree_combine_kernel(const TreeParams p, int each) {
+  const int b = blockIdx.y, lane = threadIdx.x & 31, G = p.Hq / p.Hkv;
+  const int row0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * each;
+  int walked = -1;
+  bool there = false;
+  for (int row = row0; row < min(row0 + each, p.N * p.Hq); ++row) {
+    const int t = row / p.Hq, h = row - t * p.Hq, hk = h / G;
+    if (t != walked) there = tree_present(p.parents + b * p.parents_bs, t);  // (the tree only: before the wait for the segments)
+    if (walked < 0) asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    walked = t;
+    const int r = t * G + h - hk * G, column = hk * (p.columns / p.Hkv) + r / p.column_rows;
+    const int2 range = *reinterpret_cast<const int2*>(p.slots + 2 * ((int64_t)column * p.B + b));
+    // (a split kernel that gave up may have left no slots)
+    const bool listed = range.x >= 0 && range.y >= range.x && range.y < p.ctas + (int64_t)p.columns * p.B;
+    const int ns = listed ? range.y - range.x + 1 : 0;
+    const int64_t base = (int64_t)range.x * p.column_rows + r % p.column_rows;
+    const float* lses = p.lse_part + base;
+    float m = -INFINITY;
+    if (there)
+      for (int s = lane; s < ns; s += 32) m = fmaxf(m, lses[(int64_t)s * p.column_rows]);
 #pragma unroll
-  for (int o = 16; o > 0; o /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float msafe = m == -INFINITY ? 0.f : m;
-  TO* out = static_cast<TO*>(p.o) + (((int64_t)b * p.N + t) * p.Hq + h) * p.Dv;
-  float denom = 0.f;
-  for (int d0 = 0; d0 < p.Dv; d0 += 128) {
-    const int d = d0 + lane * 4;
-    const bool vec = p.Dv % 4 == 0;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    denom = 0.f;
-    for (int s0 = 0; there && s0 < ns; s0 += 32) {
-      const float w_mine = s0 + lane < ns ? exp2f(lses[(int64_t)(s0 + lane) * p.column_rows] - msafe) : 0.f;
-      denom += w_mine;
-      const int many = min(32, ns - s0);
+    for (int o = 16; o > 0; o /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float msafe = m == -INFINITY ? 0.f : m;
+    TO* out = static_cast<TO*>(p.o) + (((int64_t)b * p.N + t) * p.Hq + h) * p.Dv;
+    float denom = 0.f;
+    for (int d0 = 0; d0 < p.Dv; d0 += 128) {
+      const int d = d0 + lane * 4;
+      const bool vec = p.Dv % 4 == 0;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      denom = 0.f;
+      for (int s0 = 0; there && s0 < ns; s0 += 32) {
+        const float w_mine = s0 + lane < ns ? exp2f(lses[(int64_t)(s0 + lane) * p.column_rows] - msafe) : 0.f;
+        denom += w_mine;
+        const int many = min(32, ns - s0);
 #pragma unroll 4
-      for (int s = 0; s < many; ++s) {
-        const float w = __shfl_sync(0xffffffffu, w_mine, s);
-        const float* x = p.o_part + (base + (int64_t)(s0 + s) * p.column_rows) * p.Dv + d;
-        if (vec && d < p.Dv) {
-          const float4 v = *reinterpret_cast<const float4*>(x);
-          acc.x = fmaf(w, v.x, acc.x);
-          acc.y = fmaf(w, v.y, acc.y);
-          acc.z = fmaf(w, v.z, acc.z);
-          acc.w = fmaf(w, v.w, acc.w);
-        } else if (!vec) {
-          if (d < p.Dv) acc.x = fmaf(w, x[0], acc.x);
-          if (d + 1 < p.Dv) acc.y = fmaf(w, x[1], acc.y);
-          if (d + 2 < p.Dv) acc.z = fmaf(w, x[2], acc.z);
-          if (d + 3 < p.Dv) acc.w = fmaf(w, x[3], acc.w);
+        for (int s = 0; s < many; ++s) {
+          const float w = __shfl_sync(0xffffffffu, w_mine, s);
+          const float* x = p.o_part + (base + (int64_t)(s0 + s) * p.column_rows) * p.Dv + d;
+          if (vec && d < p.Dv) {
+            const float4 v = *reinterpret_cast<const float4*>(x);
+            acc.x = fmaf(w, v.x, acc.x);
+            acc.y = fmaf(w, v.y, acc.y);
+            acc.z = fmaf(w, v.z, acc.z);
+            acc.w = fmaf(w, v.w, acc.w);
+          } else if (!vec) {
+            if (d < p.Dv) acc.x = fmaf(w, x[0], acc.x);
+            if (d + 1 < p.Dv) acc.y = fmaf(w, x[1], acc.y);
+            if (d + 2 < p.Dv) acc.z = fmaf(w, x[2], acc.z);
+            if (d + 3 < p.Dv) acc.w = fmaf(w, x[3], acc.w);
+          }
         }
       }
+#pragma unroll
+      for (int o = 16; o > 0; o /= 2) denom += __shfl_xor_sync(0xffffffffu, denom, o);
+      const float inv = denom > 0.f ? 1.f / denom : 0.f;
+      const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+      if (vec && (reinterpret_cast<uintptr_t>(out) & (4 * sizeof(TO) - 1)) == 0) {
+        if (d < p.Dv) {
+          struct alignas(4 * sizeof(TO)) Four { TO v[4]; } four;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) four.v[e] = Elem<TO>::from_f(y[e]);
+          *reinterpret_cast<Four*>(out + d) = four;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (d + e < p.Dv) out[d + e] = Elem<TO>::from_f(y[e]);
+      }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o /= 2) denom += __shfl_xor_sync(0xffffffffu, denom, o);
-    const float inv = denom > 0.f ? 1.f / denom : 0.f;
-    const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (d + e < p.Dv) out[d + e] = Elem<TO>::from_f(y[e]);
+    if (p.lse && lane == 0) p.lse[((int64_t)b * p.Hq + h) * p.N + t] = denom > 0.f ? (msafe + log2f(denom)) * kLn2 : INFINITY;
   }
-  if (p.lse && lane == 0) p.lse[((int64_t)b * p.Hq + h) * p.N + t] = denom > 0.f ? (msafe + log2f(denom)) * kLn2 : INFINITY;
 }
 
 template <typename T>
@@ -277,7 +289,8 @@ int launch_generic(const TreeParams& p, cudaStream_t stream) {
 
 int launch_combine(const TreeParams& p, int dtype, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((p.N * p.Hq + 7) / 8, p.B);
+  const int each = (int64_t)p.N * p.Hq * p.B >= 148 * 64 ? 4 : 1;  // (few rows: all of them at once)
+  cfg.gridDim = dim3((p.N * p.Hq + 8 * each - 1) / (8 * each), p.B);
   cfg.blockDim = dim3(256);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -285,9 +298,9 @@ int launch_combine(const TreeParams& p, int dtype, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = dtype == PJX_F32    ? cudaLaunchKernelEx(&cfg, tree_combine_kernel<float>, p)
-                        : dtype == PJX_BF16 ? cudaLaunchKernelEx(&cfg, tree_combine_kernel<__nv_bfloat16>, p)
-                                            : cudaLaunchKernelEx(&cfg, tree_combine_kernel<__half>, p);
+  const cudaError_t e = dtype == PJX_F32    ? cudaLaunchKernelEx(&cfg, tree_combine_kernel<float>, p, each)
+                        : dtype == PJX_BF16 ? cudaLaunchKernelEx(&cfg, tree_combine_kernel<__nv_bfloat16>, p, each)
+                                            : cudaLaunchKernelEx(&cfg, tree_combine_kernel<__half>, p, each);
   count_launch();
   return check_cuda(e, "tree combine launch");
 }
@@ -303,7 +316,10 @@ void generic_geometry(TreeParams& p) {
 }
 
 size_t partial_rows(const TreeParams& p) { return ((size_t)p.ctas + (size_t)p.columns * p.B) * p.column_rows; }
-size_t partial_bytes(const TreeParams& p) { return align256(partial_rows(p) * p.Dv * sizeof(float)) + align256(partial_rows(p) * sizeof(float)); }
+size_t partial_bytes(const TreeParams& p) {
+  return align256(partial_rows(p) * p.Dv * sizeof(float)) + align256(partial_rows(p) * sizeof(float)) +
+         align256((size_t)p.columns * p.B * 2 * sizeof(int32_t));
+}
 
 }  // namespace
 
@@ -354,8 +370,8 @@ int pjx_attn_decode_tree(const void* q, int64_t q_batch_stride, int64_t q_token_
     return fail(PJX_ERR_BAD_ARG, "tree: null buffer");
   if (N > kTreeMaxNodes) return fail(PJX_ERR_UNSUPPORTED, "tree: at most %d drafts a sequence (got %d)", kTreeMaxNodes, N);
   if (capacity >= PJX_BAND_NO_UPPER) return fail(PJX_ERR_UNSUPPORTED, "tree: cache capacity must be below 2^30 (got %d)", capacity);
-  if (B > 65535 || Hq > 16384)
-    return fail(PJX_ERR_UNSUPPORTED, "tree: at most 65535 sequences and 16384 heads per call (got B=%d, Hq=%d)", B, Hq);
+  if (B > 65535 || Hq > 16384 || (int64_t)B * Hkv * N > (1 << 30))
+    return fail(PJX_ERR_UNSUPPORTED, "tree: at most 65535 sequences, 16384 heads and 2^30 rows per call (got B=%d, N=%d, Hq=%d)", B, N, Hq);
   TreeParams p = {};
   p.q = q; p.k_new = k_new; p.v_new = v_new; p.k = k_cache; p.v = v_cache;
   p.q_bs = q_batch_stride; p.q_ts = q_token_stride;
@@ -381,6 +397,7 @@ int pjx_attn_decode_tree(const void* q, int64_t q_batch_stride, int64_t q_token_
     generic_geometry(p);
   p.o_part = static_cast<float*>(workspace);
   p.lse_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(partial_rows(p) * Dv * sizeof(float)));
+  p.slots = reinterpret_cast<int32_t*>(reinterpret_cast<char*>(p.lse_part) + align256(partial_rows(p) * sizeof(float)));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int rc = tc ? launch_tree_sm100(p, dtype, st)
               : dtype == PJX_F32 ? launch_generic<float>(p, st) : dtype == PJX_BF16 ? launch_generic<__nv_bfloat16>(p, st) : launch_generic<__half>(p, st);

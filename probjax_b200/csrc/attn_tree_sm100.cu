@@ -23,6 +23,8 @@
 //
 // Every barrier wait is bounded: on expiry the role raises the CTA's abort flag, all roles drain, tensor memory is freed and the
 // status word gets PJX_ERR_DEVICE_TIMEOUT.
+#include <type_traits>
+
 #include "sm100_softmax.cuh"
 #include "tree_plan.cuh"
 
@@ -65,7 +67,8 @@ struct Cfg {
   static constexpr int OFF_V = OFF_K + KST * TILE_BYTES;
   static constexpr int OFF_ML = OFF_V + VST * TILE_BYTES;  // (max, sum) of the second group's rows
   static constexpr int OFF_WORK = OFF_ML + 128 * 8;        // the softmax warps' segments
-  static constexpr int OFF_BAR = OFF_WORK + 8 * 64;
+  static constexpr int OFF_LINE = OFF_WORK + 8 * 64;       // this CTA's run
+  static constexpr int OFF_BAR = OFF_LINE + 64;
   static constexpr int N_BAR = 2 + 2 * KST + 2 * VST + 2 + 2 + 2 + 1 + 2;
   static constexpr int SMEM_BYTES = OFF_BAR + N_BAR * 8 + 16 + 1024;  // + alignment slack
   static constexpr int TMEM_COLS = 512;
@@ -88,13 +91,13 @@ attn_tree_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_unaligned) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = uniform(smem_u32(smem));
   auto BAR = [&](int i) { return sbase + C::OFF_BAR + 8u * i; };
-  constexpr int Q_FULL = 0, Q_FREE = 1;  // Q_FREE: 256 arrivals, the output staged over Q has left
+  constexpr int Q_FULL = 0, Q_FREE = 1;  // Q_FREE: the output staged over Q has left
   constexpr int K_FULL = 2, K_EMPTY = K_FULL + C::KST;
   constexpr int V_FULL = K_EMPTY + C::KST, V_EMPTY = V_FULL + C::VST;
   constexpr int S_FULL = V_EMPTY + C::VST;  // [2]
-  constexpr int P_FULL = S_FULL + 2;        // [2] 128 arrivals
+  constexpr int P_FULL = S_FULL + 2;        // [2]
   constexpr int V_LANDED = P_FULL + 2;      // a tile that may hold keys nobody sees is there
-  constexpr int V_CLEAN = V_LANDED + 1;     // 32 arrivals: their values are cleared
+  constexpr int V_CLEAN = V_LANDED + 1;     // their values are cleared
   constexpr int O_DONE = V_CLEAN + 1;
   constexpr int MEET = O_DONE + 1;          // [2] the softmax threads that stage a tile meet here (bounded, unlike a named barrier)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_BAR + C::N_BAR * 8);
@@ -105,21 +108,41 @@ attn_tree_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   // The combine may be resident early; it waits for this grid.
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   if ((int)blockIdx.x >= line.ctas) return;
-  const int64_t start = tree_run(line, blockIdx.x), stop = tree_run(line, blockIdx.x + 1);
-  const int G = p.Hq / p.Hkv, row_tiles = p.columns / p.Hkv;
+  const int64_t start = tree_run(line, blockIdx.x);
+  // (in shared memory, not in registers: it is looked at once a segment)
+  struct Run {
+    int64_t stop, length;
+    int tiles, ctas;
+  };
+  volatile Run* run = reinterpret_cast<volatile Run*>(smem + C::OFF_LINE);
+  if (threadIdx.x == 0) {
+    run->stop = tree_run(line, blockIdx.x + 1);
+    run->length = line.length;
+    run->tiles = line.tiles;
+    run->ctas = line.ctas;
+  }
   // What the roles need of a segment; every warp walks the same segments.
   struct Work {
     int b, hk, t0, first, n, prefix, prefix_tiles, clean0;
-    int64_t slot;
+    int64_t slot, pair;
+    bool last;
   };
   auto next = [&](int64_t& pos, Work& w) {
+    const int64_t stop = run->stop;
     if (pos >= stop) return false;
-    const TreeSegment sg = tree_segment(p, line, blockIdx.x, pos, stop);
+    TreeLine l;
+    l.tiles = run->tiles;
+    l.length = run->length;
+    l.ctas = run->ctas;
+    const TreeSegment sg = tree_segment(p, l, blockIdx.x, pos, stop);
+    const int row_tiles = p.columns / p.Hkv;
     w.b = uniform(sg.b);
     w.prefix = uniform(sg.prefix);
     w.first = uniform(sg.first);
     w.n = uniform(sg.end - sg.first);
     w.slot = sg.slot;
+    w.pair = sg.pair;
+    w.last = sg.last;
     w.hk = uniform(sg.column / row_tiles);
     w.t0 = uniform((sg.column - w.hk * row_tiles) * ROWS * geo.tokens);
     w.prefix_tiles = (w.prefix + BN - 1) / BN;
@@ -130,7 +153,7 @@ attn_tree_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::N_BAR; ++i)
-      mbar_init(BAR(i), i == Q_FREE ? 256u : i >= P_FULL && i < P_FULL + 2 ? 128u : i == V_CLEAN ? 32u : i >= MEET ? (ROWS == 1 ? 256u : 128u) : 1u);
+      mbar_init(BAR(i), i == Q_FREE ? 8u : i >= P_FULL && i < P_FULL + 2 ? 4u : i >= MEET ? (ROWS == 1 ? 8u : 4u) : 1u);  // (an arrival per warp)
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -159,7 +182,7 @@ attn_tree_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     auto load_q = [&] {
       ok = mbar_wait_all(BAR(Q_FREE), (seg & 1) ^ 1, abort_flag);
       if (!ok || !leader) return;
-      mbar_arrive_expect_tx(BAR(Q_FULL), ROWS * C::SUB * (uint32_t)(geo.tokens * G) * 128u);
+      mbar_arrive_expect_tx(BAR(Q_FULL), ROWS * C::SUB * (uint32_t)(geo.tokens * (p.Hq / p.Hkv)) * 128u);
 #pragma unroll
       for (int t = 0; t < ROWS; ++t)
 #pragma unroll
@@ -220,85 +243,99 @@ attn_tree_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     const uint32_t leader = elect_leader();
     constexpr uint32_t idesc_s = make_idesc(128, BN, BF16, false, false);
     constexpr uint32_t idesc_o = make_idesc(128, HD, BF16, false, true);
-    int g = 0, seg = 0, cleaned = 0;  // tiles before this segment, segments, tiles handed to the clearing warp
-    int p_done[2] = {0, 0};           // P tiles of each group so far
+    // (descriptors differ in the address field, in units of 16 bytes)
+    const uint64_t q_desc = make_smem_desc(sbase + C::OFF_Q, 16, 1024), k_desc = make_smem_desc(sbase + C::OFF_K, 16, 1024);
+    const uint64_t v_desc = make_smem_desc(sbase + C::OFF_V, 128 * 128, 1024);
+    int ks = 0, kp = 0, vs = 0, vp = 0;  // the next K and V tiles' stages, and the parities their arrival is waited with
+    int seg = 0, cleaned = 0;            // segments, tiles handed to the clearing warp
+    int p_done[2] = {0, 0};              // P tiles of each group so far
     bool ok = true;
     Work w = {};
-    auto issue_s = [&](int t, int j) {  // scores of the segment's key tile j into buffer t
-      const uint32_t qa = sbase + C::OFF_Q + (ROWS == 2 ? t : 0) * C::TILE_BYTES;
-      const uint32_t ka = sbase + C::OFF_K + ((g + j) % C::KST) * C::TILE_BYTES;
+    auto issue_s = [&](int t) {  // scores of the next K tile into buffer t
+      const uint64_t qa = q_desc + (ROWS == 2 ? t : 0) * (C::TILE_BYTES / 16), ka = k_desc + ks * (C::TILE_BYTES / 16);
 #pragma unroll
       for (int s = 0; s < C::SUB; ++s)
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
-          mma_ss(tmem + t * BN, make_smem_desc(qa + s * 128 * 128 + kk * 32, 16, 1024),
-                 make_smem_desc(ka + s * 128 * 128 + kk * 32, 16, 1024), idesc_s, (s | kk) != 0, leader);
+          mma_ss(tmem + t * BN, qa + (s * 128 * 128 + kk * 32) / 16, ka + (s * 128 * 128 + kk * 32) / 16, idesc_s, (s | kk) != 0, leader);
       mma_commit(BAR(S_FULL + t), leader);
     };
-    auto issue_pv = [&](int t, int j, bool fresh) {
-      const uint32_t va = sbase + C::OFF_V + ((g + j) % C::VST) * C::TILE_BYTES;
+    auto issue_pv = [&](int t, bool fresh) {
+      const uint64_t va = v_desc + vs * (C::TILE_BYTES / 16);
 #pragma unroll
       for (int kk = 0; kk < BN / 16; ++kk)
-        mma_ts(tmem + 2 * BN + t * HD, tmem + t * BN + kk * 8, make_smem_desc(va + kk * 2048, 128 * 128, 1024), idesc_o,
-               !fresh || kk != 0, leader);
+        mma_ts(tmem + 2 * BN + t * HD, tmem + t * BN + kk * 8, va + kk * 2048 / 16, idesc_o, !fresh || kk != 0, leader);
     };
-    auto wait_k = [&](int j) {
-      const bool there = mbar_wait_all(BAR(K_FULL + (g + j) % C::KST), ((g + j) / C::KST) & 1, abort_flag);
+    auto wait_k = [&] {
+      const bool there = mbar_wait_all(BAR(K_FULL + ks), kp, abort_flag);
       tc_fence_after();
       return there;
     };
-    auto free_k = [&](int j) { mma_commit(BAR(K_EMPTY + (g + j) % C::KST), leader); };
+    auto free_k = [&] {
+      mma_commit(BAR(K_EMPTY + ks), leader);
+      if (++ks == C::KST) {
+        ks = 0;
+        kp ^= 1;
+      }
+    };
     auto wait_v = [&](int j) {
-      bool there = mbar_wait_all(BAR(V_FULL + (g + j) % C::VST), ((g + j) / C::VST) & 1, abort_flag);
+      bool there = mbar_wait_all(BAR(V_FULL + vs), vp, abort_flag);
       if (there && j >= w.clean0) {
         if (leader) mbar_arrive(BAR(V_LANDED));
         there = mbar_wait_all(BAR(V_CLEAN), cleaned++ & 1, abort_flag);
       }
       return there;
     };
+    auto free_v = [&] {
+      mma_commit(BAR(V_EMPTY + vs), leader);
+      if (++vs == C::VST) {
+        vs = 0;
+        vp ^= 1;
+      }
+    };
     auto wait_p = [&](int t) {
-      const bool there = mbar_wait_all(BAR(P_FULL + t), p_done[t]++ & 1, abort_flag);
+      const bool there = mbar_wait_all(BAR(P_FULL + t), (t ? p_done[1]++ : p_done[0]++) & 1, abort_flag);
       tc_fence_after();
       return there;
     };
-    for (int64_t pos = start; ok && next(pos, w); ++seg, g += w.n) {
+    for (int64_t pos = start; ok && next(pos, w); ++seg) {
       const int n = w.n;
       ok = mbar_wait_all(BAR(Q_FULL), seg & 1, abort_flag);
       if constexpr (ROWS == 1) {
         for (int j = 0; ok && j < min(2, n); ++j) {
-          if (!(ok = wait_k(j))) break;
-          issue_s(j, j);
-          free_k(j);
+          if (!(ok = wait_k())) break;
+          issue_s(j);
+          free_k();
         }
         for (int j = 0; ok && j < n; ++j) {
           const int t = j & 1;
           if (!(ok = wait_v(j) && wait_p(t))) break;
-          issue_pv(t, j, j < 2);
-          mma_commit(BAR(V_EMPTY + (g + j) % C::VST), leader);
+          issue_pv(t, j < 2);
+          free_v();
           if (j + 2 < n) {
-            if (!(ok = wait_k(j + 2))) break;
-            issue_s(t, j + 2);
-            free_k(j + 2);
+            if (!(ok = wait_k())) break;
+            issue_s(t);
+            free_k();
           }
         }
       } else {
-        if (ok && (ok = wait_k(0))) {
-          issue_s(0, 0);
-          issue_s(1, 0);
-          free_k(0);
+        if (ok && (ok = wait_k())) {
+          issue_s(0);
+          issue_s(1);
+          free_k();
         }
         for (int j = 0; ok && j < n; ++j) {
           const bool more = j + 1 < n;
-          if (!(ok = wait_v(j) && (!more || wait_k(j + 1)))) break;
+          if (!(ok = wait_v(j) && (!more || wait_k()))) break;
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             if (!(ok = ok && wait_p(t))) break;
-            issue_pv(t, j, j == 0);
-            if (more) issue_s(t, j + 1);
+            issue_pv(t, j == 0);
+            if (more) issue_s(t);
           }
           if (!ok) break;
-          mma_commit(BAR(V_EMPTY + (g + j) % C::VST), leader);
-          if (more) free_k(j + 1);
+          free_v();
+          if (more) free_k();
         }
       }
       if (ok) mma_commit(BAR(O_DONE), leader);
@@ -329,7 +366,8 @@ attn_tree_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
               asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(row + s * 128 * 128 + u * 16), "r"(0) : "memory");
         }
         if (wrote) fence_proxy_async();
-        mbar_arrive(BAR(V_CLEAN));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(BAR(V_CLEAN));
       }
     }
   } else {
@@ -344,8 +382,8 @@ attn_tree_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     constexpr int STEP = ROWS == 1 ? 2 : 1;
     // The segment lives in shared memory: the registers hold the scores of a row and little else.
     struct Held {
-      int b, t0, first, prefix, prefix_tiles;
-      int64_t slot, pos;
+      int b, t0, first, prefix, prefix_tiles, last;
+      int64_t slot, pos, pair;
     };
     static_assert(sizeof(Held) <= 64, "a warp's slot");
     volatile Held* held = reinterpret_cast<volatile Held*>(smem + C::OFF_WORK + (warp - 2) * 64);
@@ -353,7 +391,8 @@ attn_tree_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     bool ok = true;
     auto meet = [&] {
       const uint32_t bar = BAR(MEET + (ROWS == 1 ? 0 : t));
-      mbar_arrive(bar);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
       const bool there = mbar_wait(bar, met++ & 1, abort_flag);
       ok = __all_sync(0xffffffffu, there) && ok;
     };
@@ -369,6 +408,8 @@ attn_tree_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         held->prefix = w.prefix;
         held->prefix_tiles = w.prefix_tiles;
         held->slot = w.slot;
+        held->pair = w.pair;
+        held->last = w.last;
         held->pos = pos;
       }
       __syncwarp();
@@ -379,17 +420,17 @@ attn_tree_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     int n, clean0;
     for (; ok && next_held(n, clean0); ++seg) {
       float m_ref = -INFINITY, l = 0.f;
-      bool any = false;  // this group has accumulated a tile of the segment
-      for (int j = ROWS == 1 ? t : 0; j < n; j += STEP, ++it) {
+      // One score tile; the few tiles that hold keys not everybody sees have a copy of the code of their own.
+      auto score_tile = [&](int j, auto masked) {
         ok = mbar_wait(BAR(S_FULL + t), it & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+        if (!ok) return;
         tc_fence_after();
         float s[BN];
 #pragma unroll
         for (int c = 0; c < BN / 32; ++c) tmem_ld32f(s_addr + c * 32, &s[c * 32]);
         tmem_wait_ld();
-        if (j >= clean0) {  // keep bits of the tile's 128 keys
+        if constexpr (decltype(masked)::value) {  // keep bits of the tile's 128 keys
           const int tile = held->first + j;
           uint32_t bits[4];
           if (tile < held->prefix_tiles) {
@@ -403,6 +444,7 @@ attn_tree_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             const int node0 = (tile - held->prefix_tiles) * BN;
             const int32_t* parents = p.parents + held->b * p.parents_bs;
             uint32_t b0 = 0, b1 = 0, b2 = 0, b3 = 0;
+            const int G = p.Hq / p.Hkv;
             const int node = held->t0 + (ROWS == 2 ? t * geo.tokens : 0) + r_in / G;
             int i = r_in < geo.tokens * G && node < p.N ? node : -1;
             while (i >= 0) {
@@ -447,7 +489,7 @@ attn_tree_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         exp_pack_store<BN, BF16>(s, make_float2(c1, c1), make_float2(neg_m, neg_m), sum0, sum1, s_addr);
         const float lsum = (sum0.x + sum0.y) + (sum1.x + sum1.y);
         // the group's previous P.V completed before these scores became visible
-        if (rescale && any) {
+        if (rescale && j >= STEP) {
 #pragma unroll
           for (int c = 0; c < HD / 32; ++c) {
             float o[32];
@@ -459,18 +501,26 @@ attn_tree_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           }
         }
         l += lsum;
-        any = true;
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(BAR(P_FULL + t));
-      }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(BAR(P_FULL + t));
+      };
+      int j = ROWS == 1 ? t : 0;
+      for (; ok && j < min(n, clean0); j += STEP, ++it) score_tile(j, std::false_type{});
+      for (; ok && j < n; j += STEP, ++it) score_tile(j, std::true_type{});
+      const bool any = ROWS == 2 || n > t;  // this group has accumulated a tile of the segment
       ok = ok && mbar_wait(BAR(O_DONE), seg & 1, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
+      if (warp == 2 && lane == 0) {  // the combine's list: first and last slot of the (sequence, column)
+        if (held->first == 0) p.slots[2 * held->pair] = (int)held->slot;
+        if (held->last) p.slots[2 * held->pair + 1] = (int)held->slot;
+      }
       // All products of the segment are done and Q is dead.  The rows leave through Q's shared memory, half a row (HD / 2 floats) at a
       // time, 16-byte units swizzled by row, so that whole lines are written; the rings go on loading.
       constexpr int HALF = HD / 2, UNITS = HALF / 4;
-      const int tile_rows = geo.tokens * G;
+      const int G = p.Hq / p.Hkv, tile_rows = geo.tokens * G;
       const int token0 = held->t0 + (ROWS == 2 ? t * geo.tokens : 0);
       const int n_rows = min(geo.tokens, p.N - token0) * G;  // rows of the tile that exist (may be none)
       const int64_t part = held->slot * p.column_rows + (ROWS == 2 ? t * tile_rows : 0);
@@ -543,7 +593,8 @@ attn_tree_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       }
       fence_proxy_async();  // the queries of the next segment are written here by TMA
       tc_fence_before();
-      mbar_arrive(BAR(Q_FREE));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(BAR(Q_FREE));
     }
   }
 

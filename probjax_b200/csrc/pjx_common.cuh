@@ -311,6 +311,7 @@ struct TreeParams {
   float* lse;         // [B, Hq, N] or null
   float* o_part;      // [slots, column_rows, Dv] fp32, normalised by the segment's own sum
   float* lse_part;    // [slots, column_rows] base 2, -inf where the segment holds no key of the row
+  int32_t* slots;     // [columns, B, 2] first and last slot of a (column, sequence)
   int B, N, Hq, Hkv, D, Dv, capacity;
   // A column is a tile of `column_rows` packed rows (t, g) of one KV head; see tree_plan.cuh.
   int column_rows, columns, ctas;

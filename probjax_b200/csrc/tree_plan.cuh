@@ -46,7 +46,9 @@ struct TreeSegment {
   int b, prefix;   // sequence, its cached keys
   int column;
   int first, end;  // tiles of the sequence
+  bool last;       // its last tile is among them
   int64_t slot;
+  int64_t pair;    // number of the (column, sequence)
 };
 // The segment at `pos` of CTA `cta`, whose run ends at `stop`.
 __device__ __forceinline__ TreeSegment tree_segment(const TreeParams& p, const TreeLine& l, int cta, int64_t pos, int64_t stop) {
@@ -75,8 +77,10 @@ __device__ __forceinline__ TreeSegment tree_segment(const TreeParams& p, const T
     }
     at -= __shfl_sync(0xffffffffu, incl, 31);
   }
+  s.last = s.end <= s.first + (stop - pos);
   s.end = (int)min((int64_t)s.end, s.first + (stop - pos));
-  s.slot = (int64_t)cta + (int64_t)s.column * p.B + s.b;
+  s.pair = (int64_t)s.column * p.B + s.b;
+  s.slot = cta + s.pair;
   return s;
 }
 __device__ __forceinline__ int64_t tree_run(const TreeLine& l, int cta) { return l.length * cta / l.ctas; }
