@@ -187,18 +187,19 @@ class _RopeAxesFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, positions, args, inverse):
-        ctx.save_for_backward(positions)
-        ctx.save_for_forward(positions)
-        ctx.args, ctx.inverse = args, inverse
+        # (an input that takes no gradient: kept as it is, which costs less per call than the saved-tensor machinery)
+        ctx.positions, ctx.args, ctx.inverse = positions, args, inverse
         return _rope_axes_call(x, positions, *args, inverse)
 
     @staticmethod
     def backward(ctx, dy):
-        return _RopeAxesFunction.apply(dy, ctx.saved_tensors[0], ctx.args, not ctx.inverse), None, None, None
+        if torch.is_grad_enabled():  # a gradient of the gradient is wanted
+            return _RopeAxesFunction.apply(dy, ctx.positions, ctx.args, not ctx.inverse), None, None, None
+        return _rope_axes_call(dy, ctx.positions, *ctx.args, not ctx.inverse), None, None, None
 
     @staticmethod
     def jvp(ctx, tx, *_):
-        return _rope_axes_call(tx, ctx.saved_tensors[0], *ctx.args, ctx.inverse)
+        return _rope_axes_call(tx, ctx.positions, *ctx.args, ctx.inverse)
 
 
 def rope_axes(x: torch.Tensor, positions, sections, *, base: float = 10_000.0, shared: bool = False, interleaved: bool = True,
@@ -234,7 +235,8 @@ def rope_axes(x: torch.Tensor, positions, sections, *, base: float = 10_000.0, s
     if _wants_grad(x):
         if out is not None:
             raise ValueError("rope_axes: out cannot be given where a gradient is wanted")
-        return _RopeAxesFunction.apply(x4, pos, (sections, base, shared, interleaved), False).reshape(x.shape)
+        y = _RopeAxesFunction.apply(x4, pos, (sections, base, shared, interleaved), False)
+        return y if x.dim() == 4 else y.reshape(x.shape)
     if out is not None:
         if tuple(out.shape) != tuple(x.shape) or out.dtype != x.dtype or out.device != x.device or not out.is_contiguous():
             raise ValueError("rope_axes: out must be a dense tensor like x")

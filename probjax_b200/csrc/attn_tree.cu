@@ -13,7 +13,7 @@ namespace pjx {
 namespace {
 
 constexpr int NT = 256;
-constexpr int BM = 64, BN = 64;
+constexpr int BN = 64;
 constexpr int PP = BN + 4;
 constexpr int kWords = kTreeMaxNodes / 32;
 
@@ -48,8 +48,10 @@ __device__ __forceinline__ void load_keys(const TreeParams& p, float* dst, int w
   }
 }
 
-template <typename T, int NCOL>  // NCOL: groups of 64 output columns
+// NCOL: groups of 64 output columns.  RT: rows per thread; 16 RT rows a tile (with few rows the 64-row tile would work on padding).
+template <typename T, int NCOL, int RT>
 __global__ void __launch_bounds__(NT) attn_tree_kernel(const TreeParams p) {
+  constexpr int BM = 16 * RT;
   extern __shared__ float smem[];
   __shared__ uint32_t sees[BM][kWords];
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
@@ -74,6 +76,8 @@ __global__ void __launch_bounds__(NT) attn_tree_kernel(const TreeParams p) {
       if (sg.first == 0) p.slots[2 * sg.pair] = (int)sg.slot;
       if (sg.last) p.slots[2 * sg.pair + 1] = (int)sg.slot;
     }
+    if (sg.first == 0 && sg.column == 0)
+      for (int i = tid; i < p.N; i += NT) p.present[(int64_t)b * p.N + i] = tree_present(parents, i);
     __syncthreads();  // the segment before is done with shared memory
     if (tid < BM) {
 #pragma unroll
@@ -86,10 +90,10 @@ __global__ void __launch_bounds__(NT) attn_tree_kernel(const TreeParams p) {
       const int r = i / Dp, d = i - r * Dp, row = r0 + r, t = row / G;
       Qs[i] = row < rows && d < D ? Elem<T>::to_f(static_cast<const T*>(p.q)[b * p.q_bs + t * p.q_ts + (int64_t)(hk * G + row - t * G) * D + d]) : 0.f;
     }
-    float m[4], l[4];
-    float4 acc[4][NCOL];
+    float m[RT], l[RT];
+    float4 acc[RT][NCOL];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < RT; ++i) {
       m[i] = -INFINITY;
       l[i] = 0.f;
 #pragma unroll
@@ -103,22 +107,22 @@ __global__ void __launch_bounds__(NT) attn_tree_kernel(const TreeParams p) {
       load_keys<T>(p, Ks, D, p.k, p.k_new, p.kn_bs, p.kn_ts, b, hk, sg.prefix, key0, node0, parents);
       load_keys<T>(p, Vs, Dv, p.v, p.v_new, p.vn_bs, p.vn_ts, b, hk, sg.prefix, key0, node0, parents);
       __syncthreads();
-      float s[4][4] = {};
+      float s[RT][4] = {};
 #pragma unroll 4
       for (int d = 0; d < D; d += 4) {
-        float4 qv[4], kv[4];
+        float4 qv[RT], kv[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) qv[i] = ld4(Qs + (ty * 4 + i) * Dp + d);
+        for (int i = 0; i < RT; ++i) qv[i] = ld4(Qs + (ty * RT + i) * Dp + d);
 #pragma unroll
         for (int c = 0; c < 4; ++c) kv[c] = ld4(Ks + (tx + 16 * c) * Dp + d);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < RT; ++i)
 #pragma unroll
           for (int c = 0; c < 4; ++c) s[i][c] = dot4(qv[i], kv[c], s[i][c]);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = ty * 4 + i;
+      for (int i = 0; i < RT; ++i) {
+        const int r = ty * RT + i;
         float tmax = -INFINITY;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -157,9 +161,9 @@ __global__ void __launch_bounds__(NT) attn_tree_kernel(const TreeParams p) {
       }
       __syncthreads();
       for (int kk = 0; kk < BN; kk += 4) {
-        float4 pv[4];
+        float4 pv[RT];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pv[i] = ld4(Ps + (ty * 4 + i) * PP + kk);
+        for (int i = 0; i < RT; ++i) pv[i] = ld4(Ps + (ty * RT + i) * PP + kk);
 #pragma unroll
         for (int c = 0; c < NCOL; ++c) {
           const int d = tx * 4 + 64 * c;
@@ -168,7 +172,7 @@ __global__ void __launch_bounds__(NT) attn_tree_kernel(const TreeParams p) {
           for (int e = 0; e < 4; ++e) {
             const float4 x = ld4(Vs + (kk + e) * Dvp + d);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < RT; ++i) {
               const float w = e == 0 ? pv[i].x : e == 1 ? pv[i].y : e == 2 ? pv[i].z : pv[i].w;
               acc[i][c].x = fmaf(w, x.x, acc[i][c].x);
               acc[i][c].y = fmaf(w, x.y, acc[i][c].y);
@@ -181,8 +185,8 @@ __global__ void __launch_bounds__(NT) attn_tree_kernel(const TreeParams p) {
     }
     const int64_t part = sg.slot * p.column_rows;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = ty * 4 + i;
+    for (int i = 0; i < RT; ++i) {
+      const int r = ty * RT + i;
       if (r0 + r >= rows) continue;
       const bool there = l[i] > 0.f;
       const float inv = there ? 1.f / l[i] : 0.f;
@@ -200,91 +204,127 @@ __global__ void __launch_bounds__(NT) attn_tree_kernel(const TreeParams p) {
   }
 }
 
-// Exact combine of a row's segments by a warp, `each` rows a warp.  Rows of absent drafts come out empty whatever the segments hold.
 template <typename TO>
-__global__ void __launch_bounds__(256) tree_combine_kernel(const TreeParams p, int each) {
-  const int b = blockIdx.y, lane = threadIdx.x & 31, G = p.Hq / p.Hkv;
-  const int row0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * each;
-  int walked = -1;
-  bool there = false;
-  for (int row = row0; row < min(row0 + each, p.N * p.Hq); ++row) {
-    const int t = row / p.Hq, h = row - t * p.Hq, hk = h / G;
-    if (t != walked) there = tree_present(p.parents + b * p.parents_bs, t);  // (the tree only: before the wait for the segments)
-    if (walked < 0) asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    walked = t;
-    const int r = t * G + h - hk * G, column = hk * (p.columns / p.Hkv) + r / p.column_rows;
-    const int2 range = *reinterpret_cast<const int2*>(p.slots + 2 * ((int64_t)column * p.B + b));
-    // (a split kernel that gave up may have left no slots)
-    const bool listed = range.x >= 0 && range.y >= range.x && range.y < p.ctas + (int64_t)p.columns * p.B;
-    const int ns = listed ? range.y - range.x + 1 : 0;
-    const int64_t base = (int64_t)range.x * p.column_rows + r % p.column_rows;
-    const float* lses = p.lse_part + base;
-    float m = -INFINITY;
-    if (there)
-      for (int s = lane; s < ns; s += 32) m = fmaxf(m, lses[(int64_t)s * p.column_rows]);
+__device__ __forceinline__ void store_row4(TO* out, int d, int width, float4 x) {
+  const float y[4] = {x.x, x.y, x.z, x.w};
+  if (width % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (4 * sizeof(TO) - 1)) == 0) {
+    if (d < width) {
+      struct alignas(4 * sizeof(TO)) Four { TO v[4]; } four;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) four.v[e] = Elem<TO>::from_f(y[e]);
+      *reinterpret_cast<Four*>(out + d) = four;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (d + e < width) out[d + e] = Elem<TO>::from_f(y[e]);
+  }
+}
+__device__ __forceinline__ float4 load_part4(const float* x, int d, int width) {
+  if (width % 4 == 0) return d < width ? *reinterpret_cast<const float4*>(x + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+  return make_float4(d < width ? x[d] : 0.f, d + 1 < width ? x[d + 1] : 0.f, d + 2 < width ? x[d + 2] : 0.f, d + 3 < width ? x[d + 3] : 0.f);
+}
+__device__ __forceinline__ void add4(float4& acc, float w, float4 x) {
+  acc.x = fmaf(w, x.x, acc.x);
+  acc.y = fmaf(w, x.y, acc.y);
+  acc.z = fmaf(w, x.z, acc.z);
+  acc.w = fmaf(w, x.w, acc.w);
+}
+
+// Exact combine of the rows' segments, EACH rows a warp.  The chain of a row is slot range -> log-sum-exps and partial rows -> result; the
+// rows of a warp take it side by side, with the first two partial rows loaded before their weights are known (B16 N64 32/8
+// heads: 28 us one row after the other).  Rows of absent drafts come out empty whatever the segments hold.
+template <typename TO, int EACH>
+__global__ void __launch_bounds__(256) tree_combine_kernel(const TreeParams p) {
+  const int b = blockIdx.y, lane = threadIdx.x & 31, G = p.Hq / p.Hkv, total = p.N * p.Hq;
+  const int row0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * EACH;
+  if (row0 >= total) return;
+  // lane e: row row0 + e
+  const int my_t = min(row0 + lane, total - 1) / p.Hq, my_h = min(row0 + lane, total - 1) - my_t * p.Hq, my_hk = my_h / G;
+  const int my_r = my_t * G + my_h - my_hk * G, my_column = my_hk * (p.columns / p.Hkv) + my_r / p.column_rows;
+  const bool mine = lane < EACH && row0 + lane < total;
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  int my_ns = 0;
+  int64_t my_base = 0;
+  if (mine) {
+    const bool there = p.present[(int64_t)b * p.N + my_t] != 0;
+    const int2 range = *reinterpret_cast<const int2*>(p.slots + 2 * ((int64_t)my_column * p.B + b));
+    // (a kernel that gave up may have left no slots)
+    if (there && range.x >= 0 && range.y >= range.x && range.y < p.ctas + (int64_t)p.columns * p.B) my_ns = range.y - range.x + 1;
+    my_base = (int64_t)range.x * p.column_rows + my_r % p.column_rows;
+  }
+  int ns[EACH];
+  int64_t base[EACH];
+  float l[EACH];  // lane s: log-sum-exp of segment s
+  float4 x[EACH][2];
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    ns[e] = __shfl_sync(0xffffffffu, my_ns, e);
+    base[e] = __shfl_sync(0xffffffffu, my_base, e);
+    l[e] = lane < ns[e] ? p.lse_part[base[e] + (int64_t)lane * p.column_rows] : -INFINITY;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      x[e][s] = s < ns[e] ? load_part4(p.o_part + (base[e] + (int64_t)s * p.column_rows) * p.Dv, lane * 4, p.Dv) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    if (row0 + e >= total) break;
+    const float* lses = p.lse_part + base[e];
+    float m = l[e];
+    for (int s = 32 + lane; s < ns[e]; s += 32) m = fmaxf(m, lses[(int64_t)s * p.column_rows]);
 #pragma unroll
     for (int o = 16; o > 0; o /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     const float msafe = m == -INFINITY ? 0.f : m;
+    const float w0 = exp2f(l[e] - msafe);
+    float denom = w0;
+    for (int s = 32 + lane; s < ns[e]; s += 32) denom += exp2f(lses[(int64_t)s * p.column_rows] - msafe);
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) denom += __shfl_xor_sync(0xffffffffu, denom, o);
+    const float inv = denom > 0.f ? 1.f / denom : 0.f;
+    const int t = (row0 + e) / p.Hq, h = row0 + e - t * p.Hq;
     TO* out = static_cast<TO*>(p.o) + (((int64_t)b * p.N + t) * p.Hq + h) * p.Dv;
-    float denom = 0.f;
-    for (int d0 = 0; d0 < p.Dv; d0 += 128) {
-      const int d = d0 + lane * 4;
-      const bool vec = p.Dv % 4 == 0;
+    for (int d = lane * 4; d - lane * 4 < p.Dv; d += 128) {
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      denom = 0.f;
-      for (int s0 = 0; there && s0 < ns; s0 += 32) {
-        const float w_mine = s0 + lane < ns ? exp2f(lses[(int64_t)(s0 + lane) * p.column_rows] - msafe) : 0.f;
-        denom += w_mine;
-        const int many = min(32, ns - s0);
+      for (int s0 = 0; s0 < ns[e]; s0 += 32) {
+        const float w_mine = s0 == 0 ? w0 : s0 + lane < ns[e] ? exp2f(lses[(int64_t)(s0 + lane) * p.column_rows] - msafe) : 0.f;
+        const int many = min(32, ns[e] - s0);
+        int s = 0;
+        if (s0 == 0 && d < 128) {
+          add4(acc, __shfl_sync(0xffffffffu, w_mine, 0), x[e][0]);
+          add4(acc, __shfl_sync(0xffffffffu, w_mine, 1), x[e][1]);  // (zero with a weight of zero where there is one segment)
+          s = 2;
+        }
 #pragma unroll 4
-        for (int s = 0; s < many; ++s) {
-          const float w = __shfl_sync(0xffffffffu, w_mine, s);
-          const float* x = p.o_part + (base + (int64_t)(s0 + s) * p.column_rows) * p.Dv + d;
-          if (vec && d < p.Dv) {
-            const float4 v = *reinterpret_cast<const float4*>(x);
-            acc.x = fmaf(w, v.x, acc.x);
-            acc.y = fmaf(w, v.y, acc.y);
-            acc.z = fmaf(w, v.z, acc.z);
-            acc.w = fmaf(w, v.w, acc.w);
-          } else if (!vec) {
-            if (d < p.Dv) acc.x = fmaf(w, x[0], acc.x);
-            if (d + 1 < p.Dv) acc.y = fmaf(w, x[1], acc.y);
-            if (d + 2 < p.Dv) acc.z = fmaf(w, x[2], acc.z);
-            if (d + 3 < p.Dv) acc.w = fmaf(w, x[3], acc.w);
-          }
-        }
+        for (; s < many; ++s)
+          add4(acc, __shfl_sync(0xffffffffu, w_mine, s), load_part4(p.o_part + (base[e] + (int64_t)(s0 + s) * p.column_rows) * p.Dv, d, p.Dv));
       }
-#pragma unroll
-      for (int o = 16; o > 0; o /= 2) denom += __shfl_xor_sync(0xffffffffu, denom, o);
-      const float inv = denom > 0.f ? 1.f / denom : 0.f;
-      const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
-      if (vec && (reinterpret_cast<uintptr_t>(out) & (4 * sizeof(TO) - 1)) == 0) {
-        if (d < p.Dv) {
-          struct alignas(4 * sizeof(TO)) Four { TO v[4]; } four;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) four.v[e] = Elem<TO>::from_f(y[e]);
-          *reinterpret_cast<Four*>(out + d) = four;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (d + e < p.Dv) out[d + e] = Elem<TO>::from_f(y[e]);
-      }
+      store_row4(out, d, p.Dv, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
     }
     if (p.lse && lane == 0) p.lse[((int64_t)b * p.Hq + h) * p.N + t] = denom > 0.f ? (msafe + log2f(denom)) * kLn2 : INFINITY;
   }
 }
 
-template <typename T>
-int launch_generic(const TreeParams& p, cudaStream_t stream) {
+constexpr int generic_rows(int rows) { return rows <= 16 ? 16 : 64; }
+
+template <typename T, int RT>
+int launch_generic_t(const TreeParams& p, cudaStream_t stream) {
+  constexpr int BM = 16 * RT;
   const int ncol = (p.Dv + 63) / 64;
-  auto kern = ncol == 1 ? attn_tree_kernel<T, 1> : ncol == 2 ? attn_tree_kernel<T, 2> : ncol == 3 ? attn_tree_kernel<T, 3> : attn_tree_kernel<T, 4>;
-  const int smem = (2 * BM * pitch4(p.D) + BN * pitch4(p.Dv) + BM * PP) * (int)sizeof(float);
+  auto kern = ncol == 1   ? attn_tree_kernel<T, 1, RT>
+              : ncol == 2 ? attn_tree_kernel<T, 2, RT>
+              : ncol == 3 ? attn_tree_kernel<T, 3, RT>
+                          : attn_tree_kernel<T, 4, RT>;
+  const int smem = ((BM + BN) * pitch4(p.D) + BN * pitch4(p.Dv) + BM * PP) * (int)sizeof(float);
   int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute(tree)");
   if (rc) return rc;
   kern<<<p.ctas, NT, smem, stream>>>(p);
   count_launch();
   return check_cuda(cudaGetLastError(), "tree attention launch");
+}
+
+template <typename T>
+int launch_generic(const TreeParams& p, cudaStream_t stream) {
+  return generic_rows(p.N * (p.Hq / p.Hkv)) == 16 ? launch_generic_t<T, 1>(p, stream) : launch_generic_t<T, 4>(p, stream);
 }
 
 int launch_combine(const TreeParams& p, int dtype, cudaStream_t stream) {
@@ -298,27 +338,28 @@ int launch_combine(const TreeParams& p, int dtype, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = dtype == PJX_F32    ? cudaLaunchKernelEx(&cfg, tree_combine_kernel<float>, p, each)
-                        : dtype == PJX_BF16 ? cudaLaunchKernelEx(&cfg, tree_combine_kernel<__nv_bfloat16>, p, each)
-                                            : cudaLaunchKernelEx(&cfg, tree_combine_kernel<__half>, p, each);
+  auto kern = dtype == PJX_F32    ? (each == 1 ? tree_combine_kernel<float, 1> : tree_combine_kernel<float, 4>)
+              : dtype == PJX_BF16 ? (each == 1 ? tree_combine_kernel<__nv_bfloat16, 1> : tree_combine_kernel<__nv_bfloat16, 4>)
+                                  : (each == 1 ? tree_combine_kernel<__half, 1> : tree_combine_kernel<__half, 4>);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
   count_launch();
   return check_cuda(e, "tree combine launch");
 }
 
 inline size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
-// Columns of 64 rows, two CTAs per SM.
+// Columns of 16 or 64 rows, two CTAs per SM.
 void generic_geometry(TreeParams& p) {
-  const int rows = p.N * (p.Hq / p.Hkv);
-  p.column_rows = rows < BM ? rows : BM;
-  p.columns = p.Hkv * ((rows + BM - 1) / BM);
+  const int rows = p.N * (p.Hq / p.Hkv), tile = generic_rows(rows);
+  p.column_rows = rows < tile ? rows : tile;
+  p.columns = p.Hkv * ((rows + tile - 1) / tile);
   p.ctas = 2 * 148;
 }
 
 size_t partial_rows(const TreeParams& p) { return ((size_t)p.ctas + (size_t)p.columns * p.B) * p.column_rows; }
 size_t partial_bytes(const TreeParams& p) {
   return align256(partial_rows(p) * p.Dv * sizeof(float)) + align256(partial_rows(p) * sizeof(float)) +
-         align256((size_t)p.columns * p.B * 2 * sizeof(int32_t));
+         align256((size_t)p.columns * p.B * 2 * sizeof(int32_t)) + align256((size_t)p.B * p.N);
 }
 
 }  // namespace
@@ -398,6 +439,7 @@ int pjx_attn_decode_tree(const void* q, int64_t q_batch_stride, int64_t q_token_
   p.o_part = static_cast<float*>(workspace);
   p.lse_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(partial_rows(p) * Dv * sizeof(float)));
   p.slots = reinterpret_cast<int32_t*>(reinterpret_cast<char*>(p.lse_part) + align256(partial_rows(p) * sizeof(float)));
+  p.present = reinterpret_cast<uint8_t*>(p.slots) + align256((size_t)p.columns * B * 2 * sizeof(int32_t));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int rc = tc ? launch_tree_sm100(p, dtype, st)
               : dtype == PJX_F32 ? launch_generic<float>(p, st) : dtype == PJX_BF16 ? launch_generic<__nv_bfloat16>(p, st) : launch_generic<__half>(p, st);

@@ -348,6 +348,8 @@ attn_tree_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     Work w = {};
     for (int64_t pos = start; ok && next(pos, w); g += w.n) {
       const int32_t* parents = p.parents + w.b * p.parents_bs;
+      if (w.first == 0 && w.pair < p.B)  // (once for every sequence, for the combine)
+        for (int i = lane; i < p.N; i += 32) p.present[(int64_t)w.b * p.N + i] = tree_present(parents, i);
       for (int j = w.clean0; ok && j < w.n; ++j, ++cleaned) {
         const int tile = w.first + j, st = (g + j) % C::VST;
         ok = mbar_wait_all(BAR(V_LANDED), cleaned & 1, abort_flag);
@@ -646,8 +648,8 @@ int launch_t(const TreeParams& p, int dtype, cudaStream_t stream) {
       return rc;
   }
   auto kern = attn_tree_sm100_kernel<HD, BF16, ROWS>;
-  if ((rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES), "cudaFuncSetAttribute(tree)")))
-    return rc;
+  static std::atomic<uint64_t> allowed{0};
+  if ((rc = allow_smem(reinterpret_cast<const void*>(kern), C::SMEM_BYTES, allowed))) return rc;
   kern<<<p.ctas, NTHREADS, C::SMEM_BYTES, stream>>>(tq, tk, tv, tkn, tvn, p, geo);
   count_launch();
   return check_cuda(cudaGetLastError(), "tree attention launch");

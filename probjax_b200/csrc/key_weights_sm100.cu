@@ -404,8 +404,8 @@ int launch_t(const KeyWeightsParams& p, int dtype, cudaStream_t stream) {
   if ((rc = make_tmap_16bit(&tq, p.q, dtype, 5, dims, strides, box))) return rc;
   const bool resident = geo.chunks <= C::QST;
   auto kern = resident ? key_weights_sm100_kernel<HD, BF16, true> : key_weights_sm100_kernel<HD, BF16, false>;
-  if ((rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES), "cudaFuncSetAttribute(key weights)")))
-    return rc;
+  static std::atomic<uint64_t> allowed[2] = {};
+  if ((rc = allow_smem(reinterpret_cast<const void*>(kern), C::SMEM_BYTES, allowed[resident]))) return rc;
   kern<<<resident ? p.Hkv * (148 / p.Hkv) : 148, NTHREADS, C::SMEM_BYTES, stream>>>(tk, tq, p, geo);
   count_launch();
   return check_cuda(cudaGetLastError(), "key weights launch");

@@ -428,8 +428,8 @@ int pjx_kv_cache_evict(const void* k_cache, const void* v_cache, const float* we
   p.held_keys = ((capacity + ranks - 1) / ranks + 3) / 4 * 4;
   if (p.held_keys > kHeldKeys) p.held_keys = kHeldKeys;
   const size_t select_smem = (size_t)(kBins + p.held_keys) * sizeof(uint32_t);
-  int rc = check_cuda(cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kBins + kHeldKeys) * (int)sizeof(uint32_t)),
-                      "cudaFuncSetAttribute(evict)");
+  static std::atomic<uint64_t> allowed{0};
+  int rc = allow_smem(reinterpret_cast<const void*>(evict_select_kernel), (kBins + kHeldKeys) * (int)sizeof(uint32_t), allowed);
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ranks, Hkv, B);

@@ -56,6 +56,16 @@ int bind_context() {
   return rc;
 }
 
+int allow_smem(const void* kern, int bytes, std::atomic<uint64_t>& done) {
+  int dev = -1, rc = check_cuda(cudaGetDevice(&dev), "query the current device");
+  if (rc) return rc;
+  const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return PJX_OK;
+  rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "cudaFuncSetAttribute");
+  if (!rc) done.fetch_or(bit, std::memory_order_relaxed);
+  return rc;
+}
+
 // Validates a caller's pjx_score_mod and converts it to the kernels' form (null: no modifiers).
 int convert_score_mod(const pjx_score_mod* m, ScoreMod* out) {
   *out = ScoreMod();

@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/pjx_attention.h"
 #include "score_mod.cuh"
 
@@ -312,6 +314,7 @@ struct TreeParams {
   float* o_part;      // [slots, column_rows, Dv] fp32, normalised by the segment's own sum
   float* lse_part;    // [slots, column_rows] base 2, -inf where the segment holds no key of the row
   int32_t* slots;     // [columns, B, 2] first and last slot of a (column, sequence)
+  uint8_t* present;   // [B, N] the draft hangs on the context
   int B, N, Hq, Hkv, D, Dv, capacity;
   // A column is a tile of `column_rows` packed rows (t, g) of one KV head; see tree_plan.cuh.
   int column_rows, columns, ctas;
@@ -346,6 +349,8 @@ void count_launch(int n = 1);
 // Makes the current device's context current on this thread: cuTensorMapEncodeTiled is a driver call and fails on a
 // thread that has made no runtime call yet (the first call of an autograd worker thread).
 int bind_context();
+// Lets `kern` use `bytes` of dynamic shared memory on the current device; `done` (one per kernel) remembers the devices.
+int allow_smem(const void* kern, int bytes, std::atomic<uint64_t>& done);
 
 // ---------------------------------------------------------------------------
 // Launchers implemented in the kernel translation units. Each returns a
