@@ -49,7 +49,9 @@ def _status_word(device) -> torch.Tensor:
     key = device.index or 0
     word = _status_words.get(key)
     if word is None:
-        word = _status_words[key] = torch.zeros(1, dtype=torch.int32, device=device)
+        word = torch.zeros(1, dtype=torch.int32, device=device)
+        if not torch.cuda.is_current_stream_capturing():  # (a graph's memory goes with the graph: its calls get a word of their own)
+            _status_words[key] = word
     return word
 
 

@@ -205,7 +205,8 @@ class _RopeAxesFunction(torch.autograd.Function):
 def rope_axes(x: torch.Tensor, positions, sections, *, base: float = 10_000.0, shared: bool = False, interleaved: bool = True,
               out: torch.Tensor | None = None) -> torch.Tensor:
     """Rotary embedding with several axes and positions of every sequence's own (``pjx_rope_axes``): ``x [..., T, H, D]``,
-    ``positions [T, axes]`` or ``[..., T, axes]`` (float32, int32 or int64, leading dimensions as ``x``), ``sections`` the
+    ``positions [T, axes]`` or ``[..., T, axes]`` (float32, int32 or int64; other integers become int64, other floats float32; leading
+    dimensions as ``x``), ``sections`` the
     elements of a head vector that each axis rotates (even; they follow one another, the rest is copied).  Pair ``i`` of an axis turns
     by ``position * base**(-2 i / section)``; with ``shared`` the frequencies run through all axes,
     ``base**(-2 p / sum(sections))`` for pair ``p``.  ``interleaved``: pairs are neighbours, otherwise the two halves of the rotated

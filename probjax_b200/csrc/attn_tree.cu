@@ -413,6 +413,8 @@ int pjx_attn_decode_tree(const void* q, int64_t q_batch_stride, int64_t q_token_
   if (capacity >= PJX_BAND_NO_UPPER) return fail(PJX_ERR_UNSUPPORTED, "tree: cache capacity must be below 2^30 (got %d)", capacity);
   if (B > 65535 || Hq > 16384 || (int64_t)B * Hkv * N > (1 << 30))
     return fail(PJX_ERR_UNSUPPORTED, "tree: at most 65535 sequences, 16384 heads and 2^30 rows per call (got B=%d, N=%d, Hq=%d)", B, N, Hq);
+  if ((int64_t)B * ((capacity + kTreeTile - 1) / kTreeTile + 2) > 0x7fffffffLL)
+    return fail(PJX_ERR_UNSUPPORTED, "tree: at most 2^31 key tiles of %d per call (B=%d, capacity=%d)", kTreeTile, B, capacity);
   TreeParams p = {};
   p.q = q; p.k_new = k_new; p.v_new = v_new; p.k = k_cache; p.v = v_cache;
   p.q_bs = q_batch_stride; p.q_ts = q_token_stride;

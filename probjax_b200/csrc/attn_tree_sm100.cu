@@ -675,7 +675,7 @@ bool tree_sm100_supported(const TreeParams& p, int dtype, const char** why) {
   else if ((reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) |
             reinterpret_cast<uintptr_t>(p.k_new) | reinterpret_cast<uintptr_t>(p.v_new)) & 15)
     w = "addresses must be 16-byte aligned";
-  else if (p.block_table && (int64_t)p.num_pages * p.page_size >= 0x7fffffff) w = "a pool of fewer than 2^31 rows";
+  else if (p.block_table && (p.num_pages == 0 || (int64_t)p.num_pages * p.page_size >= 0x7fffffff)) w = "a pool of 1 to 2^31 - 2 rows";
   if (why) *why = w;
   return w == nullptr;
 }

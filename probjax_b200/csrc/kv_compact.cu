@@ -329,6 +329,7 @@ __global__ void __launch_bounds__(256) evict_move_kernel(const EvictParams p) {
   }
 }
 
+// Whether [a, a + na) and [b, b + nb) share a byte.
 bool overlap(const void* a, size_t na, const void* b, size_t nb) {
   const char *x = static_cast<const char*>(a), *y = static_cast<const char*>(b);
   return x < y + nb && y < x + na;
@@ -366,6 +367,15 @@ int pjx_kv_cache_accept(void* k_cache, void* v_cache, const void* k_new, int64_t
   if ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(k_new) |
        reinterpret_cast<uintptr_t>(v_new)) & 15)
     return fail(PJX_ERR_UNSUPPORTED, "accept: buffers must be 16-byte aligned");
+  if (P > 0 && N > 0 && capacity > 0) {  // (the drafts are read while the cache is written)
+    const size_t rows = block_table ? (size_t)num_pages * page_size : (size_t)B * capacity;
+    const size_t k_span = ((size_t)(B - 1) * k_new_batch_stride + (size_t)(N - 1) * k_new_token_stride + (size_t)Hkv * D) * es;
+    const size_t v_span = ((size_t)(B - 1) * v_new_batch_stride + (size_t)(N - 1) * v_new_token_stride + (size_t)Hkv * Dv) * es;
+    const size_t k_bytes = rows * Hkv * D * es, v_bytes = rows * Hkv * Dv * es;
+    if (overlap(k_new, k_span, k_cache, k_bytes) || overlap(k_new, k_span, v_cache, v_bytes) || overlap(v_new, v_span, k_cache, k_bytes) ||
+        overlap(v_new, v_span, v_cache, v_bytes))
+      return fail(PJX_ERR_BAD_ARG, "accept: the drafts lie inside the cache that is written");
+  }
   AcceptParams p = {};
   p.k_cache = k_cache; p.v_cache = v_cache;
   p.k_new = static_cast<const char*>(k_new); p.v_new = static_cast<const char*>(v_new);

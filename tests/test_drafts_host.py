@@ -30,7 +30,7 @@ def tree(L, **kw):
     (dict(table=P, page=24, max_pages=2, num_pages=2), BAD, "multiple of 16"), (dict(table=P, page=0, max_pages=2, num_pages=2), BAD, "multiple of 16"),
     (dict(table=P, page=64, max_pages=1 << 25, num_pages=2), BAD, "2^30"), (dict(table=P, page=64, max_pages=1, num_pages=-1), BAD, "2^30"),
     (dict(q=None), BAD, "null"), (dict(parents=None), BAD, "null"), (dict(lengths=None), BAD, "null"), (dict(v=None), BAD, "null"),
-    (dict(N=257), UNSUPPORTED, "256"), (dict(cap=1 << 30), UNSUPPORTED, "2^30"), (dict(B=65536), UNSUPPORTED, "65535"),
+    (dict(N=257), UNSUPPORTED, "256"), (dict(cap=1 << 30), UNSUPPORTED, "2^30"), (dict(B=65536), UNSUPPORTED, "65535"), (dict(B=60000, cap=1 << 29), UNSUPPORTED, "2^31"),
     (dict(Hq=32768, Hkv=32768), UNSUPPORTED, "16384"),
     (dict(wsb=0), WORKSPACE, "workspace"), (dict(ws=P + 4, wsb=1 << 40), WORKSPACE, "16-byte"),
     (dict(B=0), 0, None), (dict(N=0), 0, None),
@@ -52,7 +52,7 @@ def test_tree_workspace_sizes(L):
 
 
 def accept(L, **kw):
-    a = dict(k=P, v=P, kn=P, kb=0, kt=0, vn=P, vb=0, vt=0, lengths=P, path=P, counts=P, table=None, B=1, N=4, Pw=2, Hkv=2, D=64, Dv=64, cap=128, page=0,
+    a = dict(k=0x100000, v=0x200000, kn=P, kb=0, kt=0, vn=P, vb=0, vt=0, lengths=P, path=P, counts=P, table=None, B=1, N=4, Pw=2, Hkv=2, D=64, Dv=64, cap=128, page=0,
              max_pages=0, num_pages=0, dtype=1, out=P, overflow=None, stream=None)
     a.update(kw)
     return L.pjx_kv_cache_accept(*a.values())
@@ -62,7 +62,7 @@ def accept(L, **kw):
     (dict(dtype=9), BAD), (dict(N=-1), BAD), (dict(kt=-8), BAD), (dict(table=P, page=0), BAD), (dict(table=P, page=64, max_pages=1 << 24), BAD),
     (dict(lengths=None), BAD), (dict(counts=None), BAD), (dict(out=None), BAD), (dict(path=None), BAD), (dict(v=None), BAD),
     (dict(B=65536), UNSUPPORTED), (dict(D=1, Hkv=1), UNSUPPORTED), (dict(kt=4), UNSUPPORTED), (dict(vb=3), UNSUPPORTED), (dict(kn=P + 8), UNSUPPORTED),
-    (dict(B=0), 0)])
+    (dict(B=0), 0), (dict(kn=0x40000, k=0x40000 - 64), BAD), (dict(vn=0x40000, k=0x40000 + 64, v=0x90000), BAD)])
 def test_accept_refusals(L, kw, rc):
     assert accept(L, **kw) == rc
 

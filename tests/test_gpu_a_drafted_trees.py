@@ -144,6 +144,20 @@ def test_pages_outside_the_pool_read_as_zeros():
         assert torch.equal(got[0], want[0])
 
 
+def test_an_empty_pool():
+    """No page at all: nothing cached, or keys that all read as zeros."""
+    case = list(make(1, 4, 4, 2, 64, 64, [0], torch.bfloat16, seed=15, page=64))
+    want = run(case)
+    case[3], case[4] = case[3][:0], case[4][:0]
+    got = run(case)
+    check(case, *got)
+    assert float((got[0] - want[0]).abs().max()) <= 2.0 ** -7 * 4  # (the other kernel: a rounding of P and one of the result, |v| < 4)
+    case[6] = torch.tensor([10], dtype=torch.int32)
+    zeros = list(case)
+    zeros[3], zeros[4], zeros[7] = torch.zeros(1, 64, 2, 64, dtype=torch.bfloat16), torch.zeros(1, 64, 2, 64, dtype=torch.bfloat16), torch.zeros(1, 1, dtype=torch.int32)
+    check(zeros, *run(case))
+
+
 def test_slices_of_a_fused_projection_and_unaligned_inputs():
     import probjax_b200 as pj
 
