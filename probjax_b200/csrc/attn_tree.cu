@@ -407,7 +407,7 @@ int pjx_attn_decode_tree(const void* q, int64_t q_batch_stride, int64_t q_token_
     capacity = max_pages * page_size;
   }
   if (B == 0 || N == 0) return PJX_OK;
-  if (!q || !k_new || !v_new || !o || !parents || !kv_lengths || (capacity > 0 && (!k_cache || !v_cache)))
+  if (!q || !k_new || !v_new || !o || !parents || !kv_lengths || (capacity > 0 && !(block_table && num_pages == 0) && (!k_cache || !v_cache)))
     return fail(PJX_ERR_BAD_ARG, "tree: null buffer");
   if (N > kTreeMaxNodes) return fail(PJX_ERR_UNSUPPORTED, "tree: at most %d drafts a sequence (got %d)", kTreeMaxNodes, N);
   if (capacity >= PJX_BAND_NO_UPPER) return fail(PJX_ERR_UNSUPPORTED, "tree: cache capacity must be below 2^30 (got %d)", capacity);

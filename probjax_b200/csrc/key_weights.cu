@@ -14,6 +14,20 @@ constexpr int NT = 256;
 constexpr int BT = 64;  // keys and rows per tile
 
 __host__ __device__ inline int pitch4(int d) { return (d + 3) / 4 * 4 + 4; }
+__device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float dot4(float4 a, float4 b, float s) {
+  return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, s))));
+}
+// One row of `width` elements, zeros where there is none and up to a multiple of four; u: one of 8 threads.
+template <typename T>
+__device__ __forceinline__ void load_row(float* dst, const T* row, int width, bool there, int u) {
+  if (sizeof(T) == 4 && width % 4 == 0 && (reinterpret_cast<uintptr_t>(row) & 15) == 0) {
+    for (int d = u * 4; d < width; d += 32)
+      *reinterpret_cast<float4*>(dst + d) = there ? __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(row) + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+  } else {
+    for (int d = u; d < (width + 3) / 4 * 4; d += 8) dst[d] = there && d < width ? Elem<T>::to_f(row[d]) : 0.f;
+  }
+}
 
 template <typename T>
 __global__ void __launch_bounds__(NT) key_weights_kernel(const KeyWeightsParams p) {
@@ -34,17 +48,14 @@ __global__ void __launch_bounds__(NT) key_weights_kernel(const KeyWeightsParams 
   const int t_first = (int)max((int64_t)0, (int64_t)k0 - p.band_hi);
   const int t_last = (int)min((int64_t)p.Lq, (int64_t)k0 + BT - p.band_lo);
   if (k0 < len && t_first < t_last) {
-    for (int i = tid; i < BT * D; i += NT) {
-      const int r = i / D, d = i - r * D;
-      Ks[r * Dp + d] = k0 + r < len ? Elem<T>::to_f(k[(((int64_t)b * p.Lkv + k0 + r) * p.Hkv + hk) * D + d]) : 0.f;
-    }
+    for (int r = tid >> 3; r < BT; r += NT / 8)
+      load_row<T>(Ks + r * Dp, k + (((int64_t)b * p.Lkv + k0 + r) * p.Hkv + hk) * D, D, k0 + r < len, tid & 7);
     const float c1 = p.sm_scale * kLog2e;
     for (int r0 = t_first * G; r0 < t_last * G; r0 += BT) {
       __syncthreads();
-      for (int i = tid; i < BT * D; i += NT) {
-        const int r = i / D, d = i - r * D, row = r0 + r;
-        const int t = row / G, g = row - t * G;
-        Qs[r * Dp + d] = row < rows ? Elem<T>::to_f(q[(((int64_t)b * p.Lq + t) * p.Hq + hk * G + g) * D + d]) : 0.f;
+      for (int r = tid >> 3; r < BT; r += NT / 8) {
+        const int row = r0 + r, t = row / G, g = row - t * G;
+        load_row<T>(Qs + r * Dp, q + (((int64_t)b * p.Lq + t) * p.Hq + hk * G + g) * D, D, row < rows, tid & 7);
       }
       if (tid < BT) {
         const int row = r0 + tid, t = row / G, g = row - t * G;
@@ -52,17 +63,18 @@ __global__ void __launch_bounds__(NT) key_weights_kernel(const KeyWeightsParams 
       }
       __syncthreads();
       float s[4][4] = {};
-      for (int d = 0; d < D; ++d) {
-        float a[4], c[4];
+#pragma unroll 4
+      for (int d = 0; d < D; d += 4) {
+        float4 a[4], c[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          a[i] = Qs[(ty * 4 + i) * Dp + d];
-          c[i] = Ks[(tx + 16 * i) * Dp + d];
+          a[i] = ld4(Qs + (ty * 4 + i) * Dp + d);
+          c[i] = ld4(Ks + (tx + 16 * i) * Dp + d);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[i][e] = fmaf(a[i], c[e], s[i][e]);
+          for (int e = 0; e < 4; ++e) s[i][e] = dot4(a[i], c[e], s[i][e]);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {

@@ -358,7 +358,9 @@ int pjx_kv_cache_accept(void* k_cache, void* v_cache, const void* k_new, int64_t
   }
   if (B == 0) return PJX_OK;
   if (!lengths || !counts || !lengths_out) return fail(PJX_ERR_BAD_ARG, "accept: null buffer");
-  if (P > 0 && N > 0 && capacity > 0 && (!k_cache || !v_cache || !k_new || !v_new || !path)) return fail(PJX_ERR_BAD_ARG, "accept: null buffer");
+  const bool rows_there = capacity > 0 && !(block_table && num_pages == 0);  // (an empty pool has no address)
+  if (P > 0 && N > 0 && rows_there && (!k_cache || !v_cache || !k_new || !v_new || !path)) return fail(PJX_ERR_BAD_ARG, "accept: null buffer");
+  if (P > 0 && !path) return fail(PJX_ERR_BAD_ARG, "accept: null buffer");
   if (B > 65535) return fail(PJX_ERR_UNSUPPORTED, "accept: batch above 65535");
   const size_t es = dtype_size(dtype);
   if ((Hkv * (size_t)D * es) % 16 || (Hkv * (size_t)Dv * es) % 16 || (k_new_batch_stride * es) % 16 || (k_new_token_stride * es) % 16 ||
@@ -367,7 +369,7 @@ int pjx_kv_cache_accept(void* k_cache, void* v_cache, const void* k_new, int64_t
   if ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(k_new) |
        reinterpret_cast<uintptr_t>(v_new)) & 15)
     return fail(PJX_ERR_UNSUPPORTED, "accept: buffers must be 16-byte aligned");
-  if (P > 0 && N > 0 && capacity > 0) {  // (the drafts are read while the cache is written)
+  if (P > 0 && N > 0 && rows_there) {  // (the drafts are read while the cache is written)
     const size_t rows = block_table ? (size_t)num_pages * page_size : (size_t)B * capacity;
     const size_t k_span = ((size_t)(B - 1) * k_new_batch_stride + (size_t)(N - 1) * k_new_token_stride + (size_t)Hkv * D) * es;
     const size_t v_span = ((size_t)(B - 1) * v_new_batch_stride + (size_t)(N - 1) * v_new_token_stride + (size_t)Hkv * Dv) * es;
