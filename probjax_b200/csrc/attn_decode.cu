@@ -472,7 +472,9 @@ __global__ void combine_splits_kernel(const DecodeParams p) {
 }
 
 // The combine of a decode with key weights: CTAs x < rows combine a row's splits, the others turn a chunk of scores into the
-// attention its keys received.  Both need the splits' log-sum-exps only, so they run side by side.
+// attention its keys received.  Both need the splits' log-sum-exps only, so they run side by side.  The scores go through memory
+// once (16 bytes a key at four rows, beside 512 of K and V); a second pass over K would cost 256.  16 ragged sequences of 1k-32k keys,
+// 32/8 heads of 128: 197 us with the weights, 5.8 TB/s of what the call cannot do without.
 constexpr int kWeightChunk = 1024;  // keys per CTA: eight per thread
 template <typename TO>
 __global__ void __launch_bounds__(128) combine_weights_kernel(const DecodeParams p) {

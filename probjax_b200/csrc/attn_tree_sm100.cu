@@ -23,6 +23,13 @@
 //
 // Every barrier wait is bounded: on expiry the role raises the CTA's abort flag, all roles drain, tensor memory is freed and the
 // status word gets PJX_ERR_DEVICE_TIMEOUT.
+//
+// Measured (bf16, 16 sequences of 16384 keys, 8 KV heads of 128, 1.07 GB of K and V; kernel alone, us): 4 rows per KV head 190
+// (5.65 TB/s), 64 rows 193, 128 rows 199, 256 rows 262 (1050 TFLOP/s; the chain softmax -> P.V -> next scores of the two row tiles
+// bounds it, as in the forward kernel).  Pages of 64 cost 1 %, of 16 7 %.  Head width 64: 164 (3.3 TB/s): a key tile takes half the
+// time to load but the same chain.  Equal runs of the work per CTA against 592 splits of equal length (ragged 1k-32k keys, 256
+// rows, with the combine): 371 against 426; masked tiles in a copy of the code of their own and one barrier arrival per warp
+// instead of one per thread: kernel 322 -> 280.
 #include <type_traits>
 
 #include "sm100_softmax.cuh"
