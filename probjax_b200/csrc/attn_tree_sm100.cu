@@ -24,12 +24,15 @@
 // Every barrier wait is bounded: on expiry the role raises the CTA's abort flag, all roles drain, tensor memory is freed and the
 // status word gets PJX_ERR_DEVICE_TIMEOUT.
 //
-// Measured (bf16, 16 sequences of 16384 keys, 8 KV heads of 128, 1.07 GB of K and V; kernel alone, us): 4 rows per KV head 190
-// (5.65 TB/s), 64 rows 193, 128 rows 199, 256 rows 262 (1050 TFLOP/s; the chain softmax -> P.V -> next scores of the two row tiles
-// bounds it, as in the forward kernel).  Pages of 64 cost 1 %, of 16 7 %.  Head width 64: 164 (3.3 TB/s): a key tile takes half the
-// time to load but the same chain.  Equal runs of the work per CTA against 592 splits of equal length (ragged 1k-32k keys, 256
-// rows, with the combine): 371 against 426; masked tiles in a copy of the code of their own and one barrier arrival per warp
-// instead of one per thread: kernel 322 -> 280.
+// Measured over the whole call with CUDA events (bf16, 16 sequences of 16384 keys, 8 KV heads of 128, 1.07 GB of K and V, us): 4 rows
+// per KV head 192 (5.6 TB/s), 32 rows 197, 64 rows 201 (5.3), 128 rows 241 (4.5), 256 rows 345 (3.1).  In a profiler's trace the kernel
+// without the combine takes 190, 191, 193, 199 and 262; the rest is the combine, and at 256 rows, where calls follow one another
+// without a pause, clocks under the power cap (1.46 GHz seen).  At 256 rows the chain softmax -> P.V -> next scores of the two row tiles
+// bounds the kernel.  Pages: at 4 rows 128 and 64 cost nothing, 16 costs 19 % (a tile is eight loads); at 64 rows 3, 8 and 32 %.  Head
+// width 64, half the bytes: 177 (3.0 TB/s), 166, 291 at 4, 64, 256 rows: a key tile takes half the time to load but the same chain.
+// Equal runs of the work on 148 CTAs against 592 splits (16 ragged sequences of 1k-32k keys in pages of 128, 256 rows, whole call): 371
+// against 426; masked tiles in a copy of the code of their own and one barrier arrival per warp instead of one per thread: 322 -> 280
+// in the trace.
 #include <type_traits>
 
 #include "sm100_softmax.cuh"

@@ -5,15 +5,16 @@
 // 128 keys a step, the even and the odd steps with groups of threads and two score buffers (128 columns each) of their own, so that the
 // MMAs run ahead of the exponentials; rows (t, g) in chunks of up to 128.  The log-sum-exp of a row is subtracted by the MMAs too: one
 // more step of 16 columns multiplies -lse2 / c, split into three 16-bit numbers (24 bits and more), with a constant; read per column and
-// thread out of shared memory it cost as much of that memory's bandwidth as all MMA operands.
+// thread out of shared memory, the loads took a third of the peak rate of shared-memory wavefronts.
 //
 //   warp 0       producer: key tiles (KST stages) and chunks of Q (QST stages) by TMA, the chunks' log-sum-exp columns
 //   warp 1       MMA issuer
 //   warps 2-17   four groups of 128 threads, two per parity: a key has a thread for the first 64 rows of a chunk and one for the
 //                others (with one thread per key, 2.5 warps per scheduler, the kernel waits for latencies)
 //
-// 8 prompts of 32k keys, 8 KV heads of 128 (537 MB of keys), us: 4 rows per KV head 105, 64 rows 107, 128 rows 114 (4.7 TB/s), 256 rows
-// 183, where the exponentials alone take 131.  Steps at 256 rows: a thread per key 259, two threads 224, log-sum-exps inside the
+// 8 prompts of 32k keys, 8 KV heads of 128 (537 MB of keys), whole calls by CUDA events, us: 4 rows per KV head 105 (5.1 TB/s), 64 rows 101,
+// 128 rows 110-127 between runs, 256 rows 211 (180 for a prompt's window under its causal mask, 202 among other calls), where the
+// exponentials alone take 131 at 1.73 GHz.  Steps at 256 rows (the kernel in a trace, causal): a thread per key 259, two threads 224, log-sum-exps inside the
 // MMAs 198, sums of the second half added a step later and short loops around the MMAs 183.  A part of the exponentials as a
 // polynomial on the FMA pipe (a quarter, a third, a half) is no faster: 187, 185, 209.
 //
