@@ -187,12 +187,16 @@ class _RopeAxesFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, positions, args, inverse):
-        # (an input that takes no gradient: kept as it is, which costs less per call than the saved-tensor machinery)
-        ctx.positions, ctx.args, ctx.inverse = positions, args, inverse
+        # (an input that takes no gradient: kept with its version, which costs less per call than the saved-tensor machinery; a tensor
+        # of inference mode has no version and is copied)
+        ctx.positions = positions.clone() if positions.is_inference() else positions
+        ctx.version, ctx.args, ctx.inverse = ctx.positions._version if not ctx.positions.is_inference() else None, args, inverse
         return _rope_axes_call(x, positions, *args, inverse)
 
     @staticmethod
     def backward(ctx, dy):
+        if ctx.version is not None and ctx.positions._version != ctx.version:
+            raise RuntimeError("rope_axes: positions were changed in place after the call whose gradient is wanted; pass a copy")
         if torch.is_grad_enabled():  # a gradient of the gradient is wanted
             return _RopeAxesFunction.apply(dy, ctx.positions, ctx.args, not ctx.inverse), None, None, None
         return _rope_axes_call(dy, ctx.positions, *ctx.args, not ctx.inverse), None, None, None
@@ -210,8 +214,9 @@ def rope_axes(x: torch.Tensor, positions, sections, *, base: float = 10_000.0, s
     elements of a head vector that each axis rotates (even; they follow one another, the rest is copied).  Pair ``i`` of an axis turns
     by ``position * base**(-2 i / section)``; with ``shared`` the frequencies run through all axes,
     ``base**(-2 p / sum(sections))`` for pair ``p``.  ``interleaved``: pairs are neighbours, otherwise the two halves of the rotated
-    part.  A slice of a fused projection is read in place.  Differentiable with respect to ``x``; ``out`` (dense, may be a dense ``x``)
-    takes the result where no gradient is wanted.  One axis is :func:`rope_interleaved` with positions per sequence."""
+    part.  A slice of a fused projection is read in place.  Differentiable with respect to ``x`` (``positions`` must not change in place until the
+    gradient has been taken: the backward pass refuses then); ``out`` (dense, may be a dense ``x``) takes the result where no gradient is
+    wanted.  One axis is :func:`rope_interleaved` with positions per sequence."""
     _require_gpu()
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dim() < 3 or x.dtype not in _DTYPES:
         raise ValueError("rope_axes takes a CUDA tensor [..., T, H, D] of dtype float32, bfloat16 or float16")

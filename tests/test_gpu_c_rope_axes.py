@@ -126,3 +126,19 @@ def test_drafts_are_rotated_to_their_own_positions():
     y = pj.rope_axes(x.to(DEV), pos.to(DEV), (64,))
     want, tol = rope_reference(x, pos, (64,))
     assert bool(((y.cpu().double() - want).abs() <= tol).all())
+
+
+def test_gradient_refuses_positions_that_changed():
+    """The gradient turns by the angles of the forward pass: positions that moved on meanwhile are refused, a copy is not."""
+    import probjax_b200 as pj
+
+    x = torch.randn(2, 5, 3, 16, device="cuda", requires_grad=True)
+    pos = torch.arange(5, device="cuda", dtype=torch.int32)[:, None].contiguous()
+    w = torch.randn(2, 5, 3, 16, device="cuda")
+    want = torch.autograd.grad((pj.rope_axes(x, pos, (16,)) * w).sum(), x)[0]
+    y = pj.rope_axes(x, pos.clone(), (16,))
+    z = pj.rope_axes(x, pos, (16,))
+    pos += 1
+    assert torch.equal(torch.autograd.grad((y * w).sum(), x)[0], want)
+    with pytest.raises(RuntimeError, match="changed in place"):
+        (z * w).sum().backward()
