@@ -115,7 +115,8 @@ class DecodeCache:
     def attend_tree(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, parents, *, sm_scale: float | None = None,
                     return_lse: bool = False):
         """Attention of a tree of drafted tokens ``query [B, N, Hq, D]`` over the filled prefix and their ancestors among the
-        drafts (:func:`decode_tree`); ``key`` / ``value`` ``[B, N, Hkv, D]`` are the drafts' own and do not enter the cache."""
+        drafts (:func:`decode_tree`); ``key`` / ``value`` ``[B, N, Hkv, D]`` are the drafts' own and do not enter the cache.  Nothing is
+        added to ``key_weights``: for the accepted drafts that is a call of :func:`key_weights` with ``return_lse``'s result."""
         return decode_tree(query, key, value, self.cached_key, self.cached_value, parents, kv_lengths=self.cache_index, sm_scale=sm_scale,
                            return_lse=return_lse)
 
@@ -233,11 +234,11 @@ def rope_axes(x: torch.Tensor, positions, sections, *, base: float = 10_000.0, s
     if pos.shape == (T, len(sections)):
         pos = pos[None].contiguous()
     elif pos.shape == lead + (T, len(sections)):
-        pos = (pos if pos.dim() == 3 else pos.reshape(-1, T, len(sections))).contiguous()
+        pos = (pos if pos.dim() == 3 else pos.reshape(math.prod(lead), T, len(sections))).contiguous()
     else:
         raise ValueError(f"positions must be [T={T}, axes={len(sections)}] or [..., T, axes] with the leading dimensions {list(lead)}, "
                          f"got {tuple(pos.shape)}")
-    x4 = x[None] if x.dim() == 3 else x if x.dim() == 4 else x.reshape((-1,) + tuple(x.shape[-3:]))
+    x4 = x[None] if x.dim() == 3 else x if x.dim() == 4 else x.reshape((math.prod(lead),) + tuple(x.shape[-3:]))
     if _wants_grad(x):
         if out is not None:
             raise ValueError("rope_axes: out cannot be given where a gradient is wanted")

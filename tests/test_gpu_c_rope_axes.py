@@ -142,3 +142,14 @@ def test_gradient_refuses_positions_that_changed():
     assert torch.equal(torch.autograd.grad((y * w).sum(), x)[0], want)
     with pytest.raises(RuntimeError, match="changed in place"):
         (z * w).sum().backward()
+
+
+@pytest.mark.parametrize("shape", [(2, 3, 0, 4, 8), (0, 3, 5, 4, 8), (2, 0, 4, 8), (0, 4, 8)])
+def test_empty_tensors(shape):
+    import probjax_b200 as pj
+
+    x = torch.zeros(shape, device=DEV, requires_grad=True)
+    for pos in (torch.zeros(shape[-3], 1, device=DEV), torch.zeros(shape[:-2] + (1,), device=DEV)):
+        y = pj.rope_axes(x, pos, (8,))
+        assert y.shape == x.shape
+        assert torch.autograd.grad(y.sum(), x)[0].shape == x.shape
