@@ -12,10 +12,10 @@
 //   warps 2-17   four groups of 128 threads, two per parity: a key has a thread for the first 64 rows of a chunk and one for the
 //                others (with one thread per key, 2.5 warps per scheduler, the kernel waits for latencies)
 //
-// 8 prompts of 32k keys, 8 KV heads of 128 (537 MB of keys), whole calls by CUDA events, us: 4 rows per KV head 105 (5.1 TB/s), 64 rows 101,
-// 128 rows 110-127 between runs, 256 rows 211 (180 for a prompt's window under its causal mask, 202 among other calls), where the
-// exponentials alone take 131 at 1.73 GHz.  Steps at 256 rows (the kernel in a trace, causal): a thread per key 259, two threads 224, log-sum-exps inside the
-// MMAs 198, sums of the second half added a step later and short loops around the MMAs 183.  A part of the exponentials as a
+// 8 prompts of 32k keys, 8 KV heads of 128 (537 MB of keys), whole calls by CUDA events, us: 4 rows per KV head 105 (5.1 TB/s),
+// 64 rows 101, 128 rows 110-127 between runs, 256 rows 211 (180 for a prompt's window under its causal mask, 204 among other calls),
+// where the exponentials alone take 131 at 1.73 GHz.  Steps at 256 rows (the kernel in a trace, causal): a thread per key 259, two
+// threads 224, log-sum-exps inside the MMAs 198, sums of the second half added a step later and short loops around the MMAs 183.  A part of the exponentials as a
 // polynomial on the FMA pipe (a quarter, a third, a half) is no faster: 187, 185, 209.
 //
 // RESIDENT: all rows fit into the stages, stay there while the CTA walks the keys of one (sequence, head), and the key steps are dealt

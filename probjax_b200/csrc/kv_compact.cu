@@ -5,9 +5,9 @@
 //  * evict: every (sequence, KV head) keeps the `recent` last keys and, of the others, those with the most accumulated
 //    attention (the lowest index first where weights tie); the kept rows move to the front in their order.
 //
-// Measured on a cache of 16 ragged sequences of 4k-32k keys, 8 heads of 128, bf16, cut to 8192 keys: the call 212 us; in a trace selection 36 (259 with the
-// weights read again in every pass, 11-bit digits and a cluster of eight CTAs a head), movement 177 = 5.8 TB/s of rows read and
-// written.  One sequence of 4001 keys cut to 1024: 11 and 6 us on the device, the call 20.
+// Measured on a cache of 16 ragged sequences of 4k-32k keys, 8 heads of 128, bf16, cut to 8192 keys: the call 213 us; in
+// a trace selection 36 (259 with the weights read again in every pass, 11-bit digits and clusters), movement 177 = 5.8 TB/s of rows
+// read and written.  One sequence of 4001 keys cut to 1024: 11 and 6 us on the device, the call 20.
 //
 // No counterpart in the reference, whose cache only grows (probjax/nn/layers/attention.py:631-643).
 #include <cooperative_groups.h>
