@@ -18,6 +18,10 @@
 // threads 224, log-sum-exps inside the MMAs 198, sums of the second half added a step later and short loops around the MMAs 183.  A part of the exponentials as a
 // polynomial on the FMA pipe (a quarter, a third, a half) is no faster: 187, 185, 209.
 //
+// Rows apart: a row without keys (lse = +inf) may hold anything in its query, and NaN plus -inf is NaN.  Where a chunk has such a row, the
+// producer leaves what to add to each of its rows in 32 bits (-inf: the row adds nothing, whatever its score) instead of in the MMA's
+// columns, the issuer hands it to the score buffer, and the compute warps take it from there.  A chunk without them pays for a flag.
+//
 // RESIDENT: all rows fit into the stages, stay there while the CTA walks the keys of one (sequence, head), and the key steps are dealt
 // in contiguous runs; otherwise the rows stream past every key step out of L2 and the steps are dealt in turn, which balances a
 // causal mask.  Every wait is bounded as in the other tcgen05 kernels.
@@ -46,6 +50,13 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* m, 
       : "memory");
 }
 
+__device__ __forceinline__ void st_shared1(uint32_t addr, float x) { asm volatile("st.shared.f32 [%0], %1;\n" ::"r"(addr), "f"(x) : "memory"); }
+__device__ __forceinline__ float ld_shared1(uint32_t addr) {
+  float x;
+  asm volatile("ld.shared.f32 %0, [%1];\n" : "=f"(x) : "r"(addr) : "memory");
+  return x;
+}
+
 template <int HD>
 struct Cfg {
   static constexpr int SUB = HD / 64;
@@ -56,11 +67,14 @@ struct Cfg {
   static constexpr int OFF_Q = OFF_K + KST * TILE_BYTES;       // [QST]
   static constexpr int OFF_EXT = OFF_Q + QST * TILE_BYTES;     // 128 rows of 4 x 16 columns: the QST stages' log-sum-exps, then the constant
   static constexpr int OFF_SUM = OFF_EXT + BT * 128;           // [4 steps][2 parities][BT] sums of the second halves
-  static constexpr int OFF_BAR = OFF_SUM + 8 * BT * 4;
+  static constexpr int OFF_APART = OFF_SUM + 8 * BT * 4;       // [QST stages, then 4 score buffers][BT] what is added to rows apart (below)
+  static constexpr int OFF_FLAG = OFF_APART + (QST + 4) * BT * 4;  // [QST + 4] whether a stage, a score buffer holds such rows
+  static constexpr int OFF_BAR = OFF_FLAG + 32;
   static constexpr int N_BAR = 2 * KST + 2 * QST + 8 + 32;
   static constexpr int SMEM_BYTES = OFF_BAR + N_BAR * 8 + 16 + 1024;
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
   static_assert(QST <= 3, "the constant takes the last of the four column groups");
+  static_assert((QST + 4) * 4 <= 32, "flags");
 };
 // -lse2 / c = 4096 a + 64 b + c': in fp16 that reaches to 2.6 * 10^8 and down to 6 * 10^-8.
 constexpr float kExt0 = 4096.f, kExt1 = 64.f;
@@ -125,6 +139,7 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
                 SUM = S_FREE + 4;  // [4 steps][2 parities][4 warps] the second half's sums are there
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_BAR + C::N_BAR * 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const uint32_t apart = sbase + C::OFF_APART, apart_flag = sbase + C::OFF_FLAG;
   const int warp = uniform(static_cast<int>(threadIdx.x >> 5)), lane = threadIdx.x & 31;
   const int G = p.Hq / p.Hkv;
   const int per_head = key_line(p);
@@ -159,7 +174,8 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::N_BAR; ++i)
-      mbar_init(BAR(i), i >= Q_FULL && i < Q_EMPTY ? 2u : i >= S_FREE && i < SUM ? 8u : 1u);
+      mbar_init(BAR(i), (i >= Q_FULL && i < Q_EMPTY) || (i >= S_FULL && i < S_FREE) ? 2u : i >= S_FREE && i < SUM ? 8u : 1u);
+    for (int i = 0; i < C::QST + 4; ++i) st_shared1(apart_flag + 4 * i, 0.f);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -192,16 +208,27 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
       ok = ok && mbar_wait_all(BAR(Q_EMPTY + st), ((fill / C::QST) & 1) ^ 1, abort_flag);
       if (!ok) return;
       ++fill;
-      for (int i = lane; i < BT; i += 32) {
-        const int t = c * geo.tokens + i / G, h = s.hk * G + i % G;
-        float l = INFINITY;  // rows without keys add nothing
-        if (i < geo.tokens * G && t < p.Lq) l = p.lse[((int64_t)s.b * p.Hq + h) * p.Lq + t] * kLog2e;
-        const float x = -l / (p.sm_scale * kLog2e);
+      float l[BT / 32];
+      bool any = false;
+#pragma unroll
+      for (int k = 0; k < BT / 32; ++k) {
+        const int i = lane + 32 * k, t = c * geo.tokens + i / G, h = s.hk * G + i % G;
+        const bool row = i < geo.tokens * G && t < p.Lq;  // (columns past the rows are masked)
+        l[k] = row ? p.lse[((int64_t)s.b * p.Hq + h) * p.Lq + t] * kLog2e : 0.f;
+        any |= l[k] == INFINITY;
+      }
+      any = __any_sync(0xffffffffu, any);
+#pragma unroll
+      for (int k = 0; k < BT / 32; ++k) {
+        const int i = lane + 32 * k;
+        const float x = any ? 0.f : -l[k] / (p.sm_scale * kLog2e);
         const float hi = Elem<T>::round(x / kExt0), rest = fmaf(-kExt0, hi, x);
         const float mid = Elem<T>::round(rest / kExt1), lo = fmaf(-kExt1, mid, rest);
         const bool finite = fabsf(hi) < INFINITY;
         write_ext(i, st, pack16<BF16>(hi, finite ? mid : 0.f), pack16<BF16>(finite ? lo : 0.f, 0.f));
+        if (any) st_shared1(apart + (st * BT + i) * 4, -l[k]);
       }
+      if (lane == 0) st_shared1(apart_flag + 4 * st, any ? 1.f : 0.f);
       fence_proxy_async();
       __syncwarp();
       if (leader) {
@@ -243,6 +270,7 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
     bool ok = true;
     int used = 0, ks = 0, kp = 0, step = 0;  // Q stages used; K stage and parity; steps
     uint32_t n_s = 0x0000;                   // score tiles of either parity, mod 4: bits 0-1 and 2-3
+    uint32_t odd = 0;                        // stages and (bits 4-7) score buffers with rows apart
     for (int64_t pos = start; ok && pos < stop;) {
       const KeyStep s = run_at(pos);
       int c0, c1;
@@ -254,11 +282,22 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
         const bool last = !RESIDENT || j == s.n - 1;
         for (int c = c0; c < c1; ++c) {
           const int f = used + c - c0, st = f % C::QST;
-          if (j == 0 && !(ok = mbar_wait_all(BAR(Q_FULL + st), (f / C::QST) & 1, abort_flag))) break;
+          if (j == 0) {
+            if (!(ok = mbar_wait_all(BAR(Q_FULL + st), (f / C::QST) & 1, abort_flag))) break;
+            odd = (odd & ~(1u << st)) | (uniform(ld_shared1(apart_flag + 4 * st)) != 0.f ? 1u << st : 0u);
+          }
           const uint32_t n = (n_s >> (2 * t)) & 3u, buf = t * 2 + (n & 1);
           if (!(ok = mbar_wait_all(BAR(S_FREE + buf), (n >> 1) ^ 1, abort_flag))) break;
           n_s = (n_s & ~(3u << (2 * t))) | (((n + 1) & 3u) << (2 * t));
           tc_fence_after();
+          if (((odd >> st) | (odd >> (4 + buf))) & 1u) {  // (the buffer's readers are done with it, as with its scores)
+            const bool now = (odd >> st) & 1u;
+            if (now)
+              for (int i = lane; i < BT; i += 32) st_shared1(apart + ((C::QST + buf) * BT + i) * 4, ld_shared1(apart + (st * BT + i) * 4));
+            if (lane == 0) st_shared1(apart_flag + 4 * (C::QST + buf), now ? 1.f : 0.f);
+            odd = (odd & ~(16u << buf)) | (now ? 16u << buf : 0u);
+            __syncwarp();
+          }
           const uint64_t qa = q_desc + st * (C::TILE_BYTES / 16);
 #pragma unroll
           for (int u = 0; u < C::SUB; ++u)
@@ -268,6 +307,7 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
           // (last: one more rounding at the size of the result)
           mma_ss(tmem + buf * BT, ext_desc + 3 * 2, ext_desc + st * 2, idesc, true, leader);
           mma_commit(BAR(S_FULL + buf), leader);
+          if (leader) mbar_arrive(BAR(S_FULL + buf));  // (for what was written above: the commit speaks for the MMAs)
           if (last) mma_commit(BAR(Q_EMPTY + st), leader);
         }
         if (ok) mma_commit(BAR(K_EMPTY + ks), leader);
@@ -338,11 +378,20 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
           for (int c32 = 2 * half; c32 < end; ++c32) {
             float x[32];
             tmem_ld32f(s_addr + c32 * 32, x);
+            const bool has_apart = ld_shared1(apart_flag + 4 * (C::QST + buf)) != 0.f;
             tmem_wait_ld();
+            if (has_apart) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float2 a = __fmul2_rn(make_float2(x[2 * i], x[2 * i + 1]), cc);
-              x[2 * i] = a.x; x[2 * i + 1] = a.y;
+              for (int i = 0; i < 32; ++i) {
+                const float add = ld_shared1(apart + ((C::QST + buf) * BT + c32 * 32 + i) * 4);
+                x[i] = add == -INFINITY ? -INFINITY : fmaf(x[i], c1, add);
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float2 a = __fmul2_rn(make_float2(x[2 * i], x[2 * i + 1]), cc);
+                x[2 * i] = a.x; x[2 * i + 1] = a.y;
+              }
             }
             if (!all || c32 * 32 + 32 > cols) {  // (columns past the rows hold anything)
 #pragma unroll

@@ -1,0 +1,78 @@
+"""Corners of the decode loop's calls (drafted trees, key weights, eviction)."""
+
+import math
+
+import pytest
+import torch
+
+from _operators_ref import key_weights_reference
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def normal(seed, *shape, dtype=torch.float32):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+def natural_lse(q, k, hi=None, scale=None):
+    """Log-sum-exp in 64 bits of every query over all keys, or over those up to its own plus ``hi``, rounded to 32."""
+    G = q.shape[2] // k.shape[2]
+    s = torch.einsum("bqhd,bkhd->bhqk", q.double(), k.double().repeat_interleave(G, 2)) * (1 / math.sqrt(q.shape[3]) if scale is None else scale)
+    if hi is not None:
+        s = s.masked_fill(torch.arange(k.shape[1])[None] > torch.arange(q.shape[1])[:, None] + hi, -math.inf)
+    return torch.logsumexp(s, -1).float()
+
+
+@pytest.mark.parametrize("impl", [None, "b200:generic"])
+@pytest.mark.parametrize("Lq,Hq,Hkv,D,Lkv,causal,dtype", [
+    (9, 8, 2, 128, 400, False, torch.bfloat16),
+    (100, 4, 2, 64, 260, False, torch.float16),   # 200 rows a KV head: several chunks that stay
+    (300, 8, 1, 64, 300, True, torch.bfloat16),   # 2400 rows: chunks that stream past the keys
+    (70, 4, 4, 128, 70, True, torch.float16),
+])
+def test_rows_without_keys_add_nothing_whatever_they_hold(Lq, Hq, Hkv, D, Lkv, causal, dtype, impl):
+    """Rows with lse = +inf hold NaN or infinite queries, and keys that only such rows see hold NaN: nothing of it reaches a weight."""
+    import probjax_b200 as pj
+
+    B = 2
+    q, k = normal(1, B, Lq, Hq, D, dtype=dtype), normal(2, B, Lkv, Hkv, D, dtype=dtype)
+    lse = natural_lse(q, k, 0 if causal else None)
+    dead = torch.rand(B, Hq, Lq, generator=torch.Generator().manual_seed(3)) < 0.25
+    dead[:, :, 0] = True      # a whole token,
+    dead[:, :, -3:] = True    # the last ones,
+    dead[1] = True            # and a whole sequence
+    lse[dead] = math.inf
+    at = dead.transpose(1, 2)
+    clean = torch.where(at[..., None], torch.zeros_like(q), q)
+    bad = torch.where(torch.arange(Lq)[None, :, None] % 3 == 0, math.inf, math.nan).expand(B, Lq, Hq)
+    q = torch.where(at[..., None], bad[..., None].to(dtype), q)
+    k[1, 5], k[1, 6, :, 0] = math.nan, math.inf
+    if causal:
+        k[0, Lq - 3:] = math.nan
+    old = normal(4, B, Hkv, Lkv).abs()
+    w = pj.key_weights(q.to(DEV), k.to(DEV), lse.to(DEV), weights=old.to(DEV), mask=pj.CausalMask() if causal else pj.NoMask(), implementation=impl).cpu()
+    pj.check_status(DEV)
+    want, tol = key_weights_reference(clean, k, lse, None, None, 0 if causal else None)
+    assert bool(((w.double() - old - want).abs() <= tol + 2.0 ** -23 * (old + want)).all())
+    assert torch.equal(w[1], old[1])
+    if causal:
+        assert torch.equal(w[0, :, Lq - 3:], old[0, :, Lq - 3:])
+
+
+def test_absent_drafts_do_not_reach_the_key_weights():
+    """``decode_tree`` gives absent drafts lse = +inf and lets their queries hold anything: its lse goes into ``key_weights`` as it is."""
+    import probjax_b200 as pj
+
+    B, N, Hq, Hkv, D, cap = 2, 6, 8, 2, 128, 384
+    q, kn, vn = (normal(10 + i, B, N, h, D, dtype=torch.bfloat16) for i, h in enumerate((Hq, Hkv, Hkv)))
+    k, v = normal(13, B, cap, Hkv, D, dtype=torch.bfloat16), normal(14, B, cap, Hkv, D, dtype=torch.bfloat16)
+    parents, lengths = torch.tensor([[-1, 0, -9, 1, 2, 0], [-9, -1, 0, 1, 3, -9]], dtype=torch.int32), torch.tensor([300, 77], dtype=torch.int32)
+    live = torch.tensor([[1, 1, 0, 1, 0, 1], [0, 1, 0, 1, 1, 0]], dtype=torch.bool)
+    q[~live] = math.nan
+    _, lse = pj.decode_tree(*(x.to(DEV) for x in (q, kn, vn, k, v, parents)), kv_lengths=lengths.to(DEV), return_lse=True)
+    w = pj.key_weights(q.to(DEV), k.to(DEV), lse, mask=pj.KVLenMask(lengths.to(DEV))).cpu()
+    pj.check_status(DEV)
+    clean = torch.where(live[..., None, None], q, torch.zeros_like(q))
+    want, tol = key_weights_reference(clean, k, lse.cpu(), lengths)
+    assert bool(((w.double() - want).abs() <= tol + 2.0 ** -23 * want).all())
