@@ -18,9 +18,10 @@
 // threads 224, log-sum-exps inside the MMAs 198, sums of the second half added a step later and short loops around the MMAs 183.  A part of the exponentials as a
 // polynomial on the FMA pipe (a quarter, a third, a half) is no faster: 187, 185, 209.
 //
-// Rows apart: a row without keys (lse = +inf) may hold anything in its query, and NaN plus -inf is NaN.  Where a chunk has such a row, the
-// producer leaves what to add to each of its rows in 32 bits (-inf: the row adds nothing, whatever its score) instead of in the MMA's
-// columns, the issuer hands it to the score buffer, and the compute warps take it from there.  A chunk without them pays for a flag.
+// Rows apart: a row without keys (lse = +inf) may hold anything in its query, and NaN plus -inf is NaN; a log-sum-exp whose three parts pass
+// the type (fp16: |lse / scale| from 2.6 * 10^8 on) would come out as infinite.  Where a chunk has such a row, the producer leaves what to
+// add to each of its rows in 32 bits (-inf: the row adds nothing, whatever its score) instead of in the MMA's columns, the issuer hands it
+// to the score buffer, and the compute warps take it from there.  A chunk without them pays for a flag.
 //
 // RESIDENT: all rows fit into the stages, stay there while the CTA walks the keys of one (sequence, head), and the key steps are dealt
 // in contiguous runs; otherwise the rows stream past every key step out of L2 and the steps are dealt in turn, which balances a
@@ -76,7 +77,7 @@ struct Cfg {
   static_assert(QST <= 3, "the constant takes the last of the four column groups");
   static_assert((QST + 4) * 4 <= 32, "flags");
 };
-// -lse2 / c = 4096 a + 64 b + c': in fp16 that reaches to 2.6 * 10^8 and down to 6 * 10^-8.
+// -lse2 / c = 4096 a + 64 b + c': in fp16 that reaches to 2.6 * 10^8 (rows beyond are added apart) and down to 6 * 10^-8.
 constexpr float kExt0 = 4096.f, kExt1 = 64.f;
 
 struct KeyGeometry {
@@ -208,25 +209,30 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
       ok = ok && mbar_wait_all(BAR(Q_EMPTY + st), ((fill / C::QST) & 1) ^ 1, abort_flag);
       if (!ok) return;
       ++fill;
-      float l[BT / 32];
+      float l[BT / 32], x[BT / 32];
       bool any = false;
 #pragma unroll
       for (int k = 0; k < BT / 32; ++k) {
         const int i = lane + 32 * k, t = c * geo.tokens + i / G, h = s.hk * G + i % G;
         const bool row = i < geo.tokens * G && t < p.Lq;  // (columns past the rows are masked)
         l[k] = row ? p.lse[((int64_t)s.b * p.Hq + h) * p.Lq + t] * kLog2e : 0.f;
-        any |= l[k] == INFINITY;
+      }
+#pragma unroll
+      for (int k = 0; k < BT / 32; ++k) {
+        x[k] = -l[k] / (p.sm_scale * kLog2e);
+        any |= !(fabsf(Elem<T>::round(x[k] / kExt0)) < INFINITY);
       }
       any = __any_sync(0xffffffffu, any);
 #pragma unroll
       for (int k = 0; k < BT / 32; ++k) {
         const int i = lane + 32 * k;
-        const float x = any ? 0.f : -l[k] / (p.sm_scale * kLog2e);
-        const float hi = Elem<T>::round(x / kExt0), rest = fmaf(-kExt0, hi, x);
+        if (any) {
+          st_shared1(apart + (st * BT + i) * 4, -l[k]);
+          x[k] = 0.f;
+        }
+        const float hi = Elem<T>::round(x[k] / kExt0), rest = fmaf(-kExt0, hi, x[k]);
         const float mid = Elem<T>::round(rest / kExt1), lo = fmaf(-kExt1, mid, rest);
-        const bool finite = fabsf(hi) < INFINITY;
-        write_ext(i, st, pack16<BF16>(hi, finite ? mid : 0.f), pack16<BF16>(finite ? lo : 0.f, 0.f));
-        if (any) st_shared1(apart + (st * BT + i) * 4, -l[k]);
+        write_ext(i, st, pack16<BF16>(hi, mid), pack16<BF16>(lo, 0.f));
       }
       if (lane == 0) st_shared1(apart_flag + 4 * st, any ? 1.f : 0.f);
       fence_proxy_async();

@@ -76,3 +76,29 @@ def test_absent_drafts_do_not_reach_the_key_weights():
     clean = torch.where(live[..., None, None], q, torch.zeros_like(q))
     want, tol = key_weights_reference(clean, k, lse.cpu(), lengths)
     assert bool(((w.double() - want).abs() <= tol + 2.0 ** -23 * want).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("Lq", [2, 700])  # (chunks that stay, chunks that stream)
+def test_scores_and_log_sum_exps_of_many_millions(Lq, dtype):
+    """q.k up to 2^29 with a scale of 2^-13, so that lse / scale passes what three 16-bit numbers carry in fp16.  All sums are exact in 32
+    bits (2^29 plus multiples of 2^6), so the exponent scale q.k - lse is off by the roundings at |s| = 65536: the constant's, the lse's, the
+    product's, each 2^-24 relative, and three 16-bit parts' 2^-24: below 2^-22 (|s| + |lse|)."""
+    import probjax_b200 as pj
+
+    B, Hq, Hkv, D, Lkv = 1, 4, 2, 64, 200
+    q, k = torch.zeros(B, Lq, Hq, D), torch.zeros(B, Lkv, Hkv, D)
+    q[..., 0], q[..., 1] = 2.0 ** 15, 64.0
+    k[..., 0] = 2.0 ** 14
+    k[..., 1] = torch.randint(0, 256, (B, Lkv, Hkv), generator=torch.Generator().manual_seed(5)).float()
+    q[:, 0, 1] *= -1  # a row that is not among them
+    q[:, 0, 0] = 0.0
+    q, k, scale = q.to(dtype), k.to(dtype), 2.0 ** -13
+    lse = natural_lse(q, k, scale=scale)
+    assert float(lse.max()) / scale > 2.0 ** 28
+    old = normal(6, B, Hkv, Lkv).abs()
+    w = pj.key_weights(q.to(DEV), k.to(DEV), lse.to(DEV), weights=old.to(DEV), sm_scale=scale).cpu().double()
+    pj.check_status(DEV)
+    want, _ = key_weights_reference(q, k, lse, scale=scale)
+    rel = math.expm1(2.0 ** -22 * 2 * (2.0 ** 16 + 8)) + Hq // Hkv * Lq * 2.0 ** -23 + 2.0 ** -20
+    assert bool(((w - old - want).abs() <= rel * want + 2.0 ** -23 * (old + want)).all())
