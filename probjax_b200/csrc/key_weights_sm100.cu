@@ -23,8 +23,8 @@
 // add to each of its rows in 32 bits (-inf: the row adds nothing, whatever its score) instead of in the MMA's columns, the issuer hands it
 // to the score buffer, and the compute warps take it from there.  A chunk without them pays for a flag.
 //
-// RESIDENT: all rows fit into the stages, stay there while the CTA walks the keys of one (sequence, head), and the key steps are dealt
-// in contiguous runs; otherwise the rows stream past every key step out of L2 and the steps are dealt in turn, which balances a
+// RESIDENT: all rows fit into the stages, stay there while the CTA walks the keys of one (sequence, head), and the key steps of all heads
+// are dealt in contiguous runs, one per CTA (a run may go on into the next sequence or head, whose rows it then loads); otherwise the rows stream past every key step out of L2 and the steps are dealt in turn, which balances a
 // causal mask.  Every wait is bounded as in the other tcgen05 kernels.
 #include <type_traits>
 
@@ -146,9 +146,8 @@ key_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_
   const int per_head = key_line(p);
   const int64_t total = (int64_t)per_head * p.Hkv;
   // this CTA's steps: pos = start, start + stride, .. below stop
-  const int head = blockIdx.x % p.Hkv, part = blockIdx.x / p.Hkv, parts = gridDim.x / p.Hkv;
-  const int64_t start = RESIDENT ? (int64_t)head * per_head + (int64_t)per_head * part / parts : blockIdx.x;
-  const int64_t stop = RESIDENT ? (int64_t)head * per_head + (int64_t)per_head * (part + 1) / parts : total;
+  const int64_t start = RESIDENT ? total * blockIdx.x / gridDim.x : blockIdx.x;
+  const int64_t stop = RESIDENT ? total * (blockIdx.x + 1) / gridDim.x : total;
   // The run of steps at `pos` (one step where the rows stream).
   auto run_at = [&](int64_t pos) {
     KeyStep s = key_step(p, per_head, pos);
@@ -462,7 +461,7 @@ int launch_t(const KeyWeightsParams& p, int dtype, cudaStream_t stream) {
   auto kern = resident ? key_weights_sm100_kernel<HD, BF16, true> : key_weights_sm100_kernel<HD, BF16, false>;
   static std::atomic<uint64_t> allowed[2] = {};
   if ((rc = allow_smem(reinterpret_cast<const void*>(kern), C::SMEM_BYTES, allowed[resident]))) return rc;
-  kern<<<resident ? p.Hkv * (148 / p.Hkv) : 148, NTHREADS, C::SMEM_BYTES, stream>>>(tk, tq, p, geo);
+  kern<<<148, NTHREADS, C::SMEM_BYTES, stream>>>(tk, tq, p, geo);
   count_launch();
   return check_cuda(cudaGetLastError(), "key weights launch");
 }

@@ -102,3 +102,33 @@ def test_scores_and_log_sum_exps_of_many_millions(Lq, dtype):
     want, _ = key_weights_reference(q, k, lse, scale=scale)
     rel = math.expm1(2.0 ** -22 * 2 * (2.0 ** 16 + 8)) + Hq // Hkv * Lq * 2.0 ** -23 + 2.0 ** -20
     assert bool(((w - old - want).abs() <= rel * want + 2.0 ** -23 * (old + want)).all())
+
+
+@pytest.mark.parametrize("Hkv,G,Lq,D", [(75, 2, 3, 64), (148, 1, 1, 64), (149, 1, 5, 128), (200, 2, 70, 64), (300, 1, 130, 64)])
+def test_key_weights_of_many_heads(Hkv, G, Lq, D):
+    """More KV heads than half of the SMs, as many, and more: rows that stay in shared memory (one to three chunks)."""
+    import probjax_b200 as pj
+
+    B, Lkv, Hq = 2, 200, Hkv * G
+    q, k = normal(20, B, Lq, Hq, D, dtype=torch.bfloat16), normal(21, B, Lkv, Hkv, D, dtype=torch.bfloat16)
+    n = torch.tensor([200, 131], dtype=torch.int32)
+    k[1, 131:] = math.nan
+    lse = torch.stack([natural_lse(q[b:b + 1], k[b:b + 1, :int(n[b])])[0] for b in range(B)])
+    old = normal(22, B, Hkv, Lkv).abs()
+    w = pj.key_weights(q.to(DEV), k.to(DEV), lse.to(DEV), weights=old.to(DEV), mask=pj.KVLenMask(n.to(DEV))).cpu()
+    pj.check_status(DEV)
+    want, tol = key_weights_reference(q, k, lse, n)
+    assert bool(((w.double() - old - want).abs() <= tol + 2.0 ** -23 * (old + want)).all())
+    assert torch.equal(w[1, :, 131:], old[1, :, 131:])
+
+
+def test_decode_weights_of_many_heads_and_rows():
+    """Rows above what the streaming kernel takes: the forward kernels, then the key weights, over 150 KV heads."""
+    import probjax_b200 as pj
+
+    B, Lq, Hkv, D, cap = 1, 20, 150, 64, 90
+    q, k, v = (normal(23 + i, B, n, Hkv, D, dtype=torch.float16).to(DEV) for i, n in enumerate((Lq, cap, cap)))
+    _, lse, w = pj.decode_weights(q, k, v, return_lse=True)
+    pj.check_status(DEV)
+    want, tol = key_weights_reference(q.cpu(), k.cpu(), lse.cpu())
+    assert bool(((w.cpu().double() - want).abs() <= tol + 2.0 ** -23 * want).all())
