@@ -14,6 +14,7 @@ or a GPU is missing.
 from __future__ import annotations
 
 import math
+import threading
 from typing import Optional
 
 import numpy as np
@@ -67,10 +68,13 @@ def check_status(device=None) -> None:
 
 def _scratch_bytes(device, tag: str, nbytes: int) -> torch.Tensor:
     """A cached, growing device byte buffer (decode partials, projections, staging), one per
-    (device, CUDA stream, purpose): calls issued on different streams never share scratch, and a
+    (host thread, device, CUDA stream, purpose): calls issued on different streams never share scratch, and a
     buffer that is outgrown is only dropped by the stream that owns it, whose earlier kernels
-    are ordered before anything that reuses the memory."""
-    key = (device.index or 0, _stream(device), tag)
+    are ordered before anything that reuses the memory.  Threads do not share it either: a call
+    of several launches hands over through its scratch, and on one stream the launches of another
+    thread's call may fall between them (the library call runs without the interpreter's lock).
+    A thread's buffers outlive it, for graphs that it captured, and go to the next thread of its number."""
+    key = (threading.get_ident(), device.index or 0, _stream(device), tag)
     buf = _scratch.get(key)
     if buf is None or buf.numel() < nbytes:
         buf = torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)

@@ -1,6 +1,7 @@
 """Corners of the decode loop's calls (drafted trees, key weights, eviction)."""
 
 import math
+import threading
 
 import pytest
 import torch
@@ -132,3 +133,48 @@ def test_decode_weights_of_many_heads_and_rows():
     pj.check_status(DEV)
     want, tol = key_weights_reference(q.cpu(), k.cpu(), lse.cpu())
     assert bool(((w.cpu().double() - want).abs() <= tol + 2.0 ** -23 * want).all())
+
+
+def test_two_host_threads_on_one_stream():
+    """Two threads evict, decode and verify on the default stream at once, with sizes of their own: each gets what it gets alone (a call of two
+    launches hands over through memory that no other thread's call writes)."""
+    import probjax_b200 as pj
+
+    def job(seed, B, cap, keep, Hkv, N):
+        D, Hq = 64, 4 * Hkv
+        t = lambda i, *s: normal(seed + i, *s, dtype=torch.bfloat16).to(DEV)
+        k, v, w = t(0, B, cap, Hkv, D), t(1, B, cap, Hkv, D), normal(seed + 2, B, Hkv, cap).abs().to(DEV)
+        n = torch.tensor([cap - 13 * b for b in range(B)], dtype=torch.int32, device=DEV)
+        q, kn, vn = t(3, B, N, Hq, D), t(4, B, N, Hkv, D), t(5, B, N, Hkv, D)
+        parents = torch.arange(N, dtype=torch.int32, device=DEV) - 1
+        out = tuple(torch.empty(s, dtype=x, device=DEV) for s, x in (((B, keep, Hkv, D), k.dtype), ((B, keep, Hkv, D), k.dtype), ((B, Hkv, keep), w.dtype)))
+
+        def once():
+            lengths, kept = pj.evict(k, v, w, n, keep, recent=3, out=out)
+            o = pj.decode_tree(q, kn, vn, k, v, parents, kv_lengths=n)
+            s = pj.decode_weights(q[:, :1], k, v, kv_lengths=n)
+            d = pj.decode_forward(q[:, :1], k, v, kv_lengths=n, sm_scale=0.125)
+            return [x.clone() for x in (lengths, kept, *out, o, *s, d)]
+        return once
+
+    jobs = [job(100, 2, 1500, 700, 2, 5), job(200, 3, 900, 64, 4, 9)]
+    alone = [f() for f in jobs]
+    torch.cuda.synchronize()
+    wrong, start = [], threading.Barrier(2)
+
+    def loop(f, want):
+        try:
+            start.wait(timeout=60)
+            got = [f() for _ in range(150)]
+            torch.cuda.synchronize()
+            wrong.extend(i for g in got for i, (a, b) in enumerate(zip(g, want)) if not torch.equal(a, b))
+        except Exception as e:
+            wrong.append(e)
+
+    threads = [threading.Thread(target=loop, args=a) for a in zip(jobs, alone)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong[:5]
+    pj.check_status(DEV)
