@@ -19,6 +19,7 @@ from typing import Optional
 
 import numpy as np
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import _lib
 from .masks import (AttentionBias, AttentionMask, LoweredBias, LoweredMask, NoMask, lower_bias, lower_bias_structured,
@@ -450,6 +451,16 @@ def _wants_grad(*tensors) -> bool:
         if fwd_ad.unpack_dual(t).tangent is not None:
             return True
     return False
+
+
+def _refuse_grad(what: str, *tensors) -> None:
+    """Refuses inputs that ask for a gradient or carry a tangent where the call has neither."""
+    if torch.is_grad_enabled():
+        asked = any([t.requires_grad for t in tensors if t is not None])
+    else:
+        asked = False
+    if asked or (_forward_ad._current_level >= 0 and _wants_grad(*tensors)):
+        raise NotImplementedError(f"{what} has no gradient: detach its inputs, or call it under torch.no_grad()")
 
 
 def decode_forward(q, k_cache, v_cache, *, kv_lengths=None, sm_scale, split_len=0, return_lse=False,

@@ -109,7 +109,7 @@ class DecodeCache:
         if window is not None and window < n:
             q, part = q[:, n - window:], part[:, :, n - window:]
             mask = KVLenMask(self.cache_index) & CausalFromBottomRightMask(window, int(prefix_length))
-        key_weights(q, self.cached_key, part, weights=self.key_weights, mask=mask, sm_scale=sm_scale, out=self.key_weights)
+        key_weights(q, self.cached_key.detach(), part, weights=self.key_weights, mask=mask, sm_scale=sm_scale, out=self.key_weights)
         return (out, lse) if return_lse else out
 
     def attend_tree(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, parents, *, sm_scale: float | None = None,

@@ -16,7 +16,7 @@ import math
 import torch
 
 from . import _lib
-from .attention import _DTYPES, _IMPL, _launch, _ptr, _require_gpu, _status_word, _stream, _workspace
+from .attention import _DTYPES, _IMPL, _launch, _ptr, _refuse_grad, _require_gpu, _status_word, _stream, _workspace
 
 
 def _token_rows(t: torch.Tensor):
@@ -94,7 +94,8 @@ def decode_tree(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_cac
     ``[num_pages, page_size, Hkv, D]`` with a page size that is a multiple of 16.  At most 256 drafts a sequence.
 
     A chain of drafts is ``parents = arange(N) - 1``.  Positions for a rotary embedding are ``kv_lengths + depth``
-    (:func:`probjax_b200.rope_axes`).  Returns ``o [B, N, Hq, Dv]`` and, with ``return_lse``, ``lse [B, Hq, N]``."""
+    (:func:`probjax_b200.rope_axes`).  Returns ``o [B, N, Hq, Dv]`` and, with ``return_lse``, ``lse [B, Hq, N]``; no gradient (inputs
+    that ask for one are refused)."""
     _require_gpu()
     if implementation not in _IMPL:
         raise ValueError(f"implementation must be None or one of {sorted(k for k in _IMPL if k)}")
@@ -107,6 +108,7 @@ def decode_tree(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_cac
         raise ValueError(f"decode_tree: q must be [B={B}, N={N}, Hq, D={D}], got {tuple(q.shape)}")
     if Hq < 1 or Hkv < 1 or Hq % Hkv != 0:
         raise ValueError(f"query heads ({Hq}) must be a multiple of key/value heads ({Hkv})")
+    _refuse_grad("decode_tree", q, k_new, v_new, k_cache, v_cache)
     lengths = _int32(kv_lengths, dev, (B,), "kv_lengths")
     if not isinstance(parents, torch.Tensor):
         parents = torch.as_tensor(parents)

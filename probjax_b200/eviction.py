@@ -15,7 +15,8 @@ import math
 import torch
 
 from . import _lib
-from .attention import (_DTYPES, _IMPL, _as_tensor, _band_args, _check_call, _launch, _ptr, _require_gpu, _status_word, _stream, _workspace)
+from .attention import (_DTYPES, _IMPL, _as_tensor, _band_args, _check_call, _launch, _ptr, _refuse_grad, _require_gpu, _status_word,
+                        _stream, _workspace)
 from .drafts import _int32
 from .masks import AttentionMask, split_mask
 
@@ -49,13 +50,15 @@ def decode_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     """Split-KV decode (as :func:`decode_forward`) that also returns ``weights`` plus what every key received of this step's
     attention, summed over the query tokens and the heads of its group (``pjx_attn_decode_weights``): ``q [B, Lq, Hq, D]`` over
     ``k_cache``, ``v_cache`` ``[B, capacity, Hkv, D]``, ``weights`` float32 ``[B, Hkv, capacity]`` (``None``: zeros).
-    ``out`` takes the sum and may be ``weights`` itself.  Returns ``(o, out)`` or ``(o, lse, out)``."""
+    ``out`` takes the sum and may be ``weights`` itself.  Returns ``(o, out)`` or ``(o, lse, out)``; no gradient (inputs that ask for one
+    are refused)."""
     _require_gpu()
     for t in (q, k_cache, v_cache):
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise ValueError("decode_weights takes CUDA tensors")
     B, Lq, cap, Hq, Hkv, D, Dv = _check_call(q, k_cache, v_cache, what="decode_weights")
     dev = q.device
+    _refuse_grad("decode_weights", q, k_cache, v_cache, weights)
     lengths = None if kv_lengths is None else _int32(kv_lengths, dev, (B,), "kv_lengths")
     weights, out = _weights_args("decode_weights", weights, out, (B, Hkv, cap), dev)
     q, k_cache, v_cache = q.contiguous(), k_cache.contiguous(), v_cache.contiguous()
@@ -79,7 +82,8 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, weights:
     """What every key received of an attention call that has been made (``pjx_attn_key_weights``): ``weights`` (float32
     ``[B, Hkv, Lkv]``, ``None``: zeros) plus the sum over the queries that see it of ``exp(sm_scale q.k - lse)``, with the call's own
     ``mask``, ``sm_scale`` (default ``1/sqrt(D)``) and natural-log ``lse [B, Hq, Lq]``.  ``mask`` may hold key lengths and bands
-    (causal, windows, bottom-right causal).  ``out`` takes the sum and may be ``weights`` itself."""
+    (causal, windows, bottom-right causal).  ``out`` takes the sum and may be ``weights`` itself.  No gradient (inputs that ask for one
+    are refused)."""
     _require_gpu()
     if implementation not in _IMPL:
         raise ValueError(f"implementation must be None or one of {sorted(x for x in _IMPL if x)}")
@@ -88,6 +92,7 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, weights:
             raise ValueError("key_weights takes CUDA tensors")
     B, Lq, Lkv, Hq, Hkv, D, _ = _check_call(q, k, k, lse=lse, what="key_weights")
     dev = q.device
+    _refuse_grad("key_weights", q, k, lse, weights)
     if lse.device != dev or lse.dtype != torch.float32:
         raise ValueError(f"key_weights: lse must be float32 on {dev}")
     lm, residual = split_mask(mask, B, Lq, Lkv)

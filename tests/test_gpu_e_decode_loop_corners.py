@@ -178,3 +178,45 @@ def test_two_host_threads_on_one_stream():
         t.join()
     assert not wrong, wrong[:5]
     pj.check_status(DEV)
+
+
+def test_calls_without_a_gradient_refuse_inputs_that_ask_for_one():
+    import probjax_b200 as pj
+
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device=DEV)
+    q, kn, k = z(1, 3, 4, 64), z(1, 3, 2, 64), z(1, 8, 2, 64)
+    par, lse = torch.tensor([-1, 0, 1], dtype=torch.int32), torch.zeros(1, 4, 3, device=DEV)
+    calls = {
+        "tree": (lambda a, b, c, d, e: pj.decode_tree(a, b, c, d, e, par, kv_lengths=[4]), (q, kn, kn, k, k)),
+        "decode": (lambda a, b, c: pj.decode_weights(a[:, :1], b, c), (q, k, k)),
+        "weights": (lambda a, b, c: pj.key_weights(a, b, c), (q, k, lse)),
+        "attend_tree": (lambda a, b, c: pj.DecodeCache(1, 8, 2, 64).attend_tree(a, b, c, par), (q, kn, kn)),
+    }
+    for name, (f, args) in calls.items():
+        f(*args)
+        for i in range(len(args)):
+            wanting = [x.clone().requires_grad_(j == i) for j, x in enumerate(args)]
+            with pytest.raises(NotImplementedError, match="gradient"):
+                f(*wanting)
+            with torch.no_grad():
+                f(*wanting)
+
+
+def test_a_tracked_cache_still_differentiates():
+    """``attend`` with tracked weights: gradients of the queries and of a cache that asks for them, weights as without."""
+    import probjax_b200 as pj
+
+    t = lambda i, *s: normal(60 + i, *s, dtype=torch.bfloat16).to(DEV)
+    q, k, v, dy = t(0, 1, 5, 4, 64), t(1, 1, 40, 2, 64), t(2, 1, 40, 2, 64), t(3, 1, 5, 4, 64)
+    weights = []
+    for wants in (False, True):
+        cache = pj.DecodeCache(1, 64, 2, 64, track_weights=True)
+        cache.update(k, v)
+        x = q.clone().requires_grad_(wants)
+        cache.cached_key.requires_grad_(wants)
+        o = cache.attend(x, prefix_length=40)
+        if wants:
+            dx, dk = torch.autograd.grad(o, (x, cache.cached_key), dy)
+            assert bool(dx.any()) and bool(dk[:, :40].any()) and not bool(dk[:, 40:].any())
+        weights.append(cache.key_weights)
+    assert torch.equal(*weights)
