@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(NT) attn_tree_kernel(const TreeParams p) {
     for (int i = 0; i < RT; ++i) {
       const int r = ty * RT + i;
       if (r0 + r >= rows) continue;
-      const bool there = l[i] > 0.f;
+      const bool there = l[i] != 0.f;  // (a sum that is not a number stays one, in the output and in the log-sum-exp)
       const float inv = there ? 1.f / l[i] : 0.f;
 #pragma unroll
       for (int c = 0; c < NCOL; ++c) {
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeParams p) {
     for (int s = 32 + lane; s < ns[e]; s += 32) denom += exp2f(lses[(int64_t)s * p.column_rows] - msafe);
 #pragma unroll
     for (int o = 16; o > 0; o /= 2) denom += __shfl_xor_sync(0xffffffffu, denom, o);
-    const float inv = denom > 0.f ? 1.f / denom : 0.f;
+    const float inv = denom != 0.f ? 1.f / denom : 0.f;
     const int t = (row0 + e) / p.Hq, h = row0 + e - t * p.Hq;
     TO* out = static_cast<TO*>(p.o) + (((int64_t)b * p.N + t) * p.Hq + h) * p.Dv;
     for (int d = lane * 4; d - lane * 4 < p.Dv; d += 128) {
@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeParams p) {
       }
       store_row4(out, d, p.Dv, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
     }
-    if (p.lse && lane == 0) p.lse[((int64_t)b * p.Hq + h) * p.N + t] = denom > 0.f ? (msafe + log2f(denom)) * kLn2 : INFINITY;
+    if (p.lse && lane == 0) p.lse[((int64_t)b * p.Hq + h) * p.N + t] = denom != 0.f ? (msafe + log2f(denom)) * kLn2 : INFINITY;
   }
 }
 

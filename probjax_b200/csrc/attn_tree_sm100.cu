@@ -571,8 +571,8 @@ attn_tree_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
               wb = m1 == -INFINITY ? 0.f : exp2f(m1 - m);
               lsum = l * wa + l1 * wb;
             }
-            inv = lsum > 0.f ? 1.f / lsum : 0.f;
-            if (r_in < n_rows) p.lse_part[part + r_in] = lsum > 0.f ? m + log2f(lsum) : -INFINITY;
+            inv = lsum != 0.f ? 1.f / lsum : 0.f;  // (NaN stays NaN)
+            if (r_in < n_rows) p.lse_part[part + r_in] = lsum != 0.f ? m + log2f(lsum) : -INFINITY;
           }
 #pragma unroll
           for (int c = 0; c < HALF / 32; ++c) {

@@ -6,7 +6,7 @@ import threading
 import pytest
 import torch
 
-from _operators_ref import key_weights_reference
+from _operators_ref import key_weights_reference, tree_reference
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -220,3 +220,29 @@ def test_a_tracked_cache_still_differentiates():
             assert bool(dx.any()) and bool(dk[:, :40].any()) and not bool(dk[:, 40:].any())
         weights.append(cache.key_weights)
     assert torch.equal(*weights)
+
+
+@pytest.mark.parametrize("impl,dtype", [(None, torch.bfloat16), ("b200:generic", torch.bfloat16), (None, torch.float32)])
+@pytest.mark.parametrize("N", [5, 70])  # (one row tile, two)
+def test_a_key_that_is_not_a_number_shows_in_the_rows_that_see_it(N, impl, dtype):
+    """NaN in a cached key, in a draft's key and in a query: the rows that see it are NaN in output and lse, the others are as without it."""
+    import probjax_b200 as pj
+
+    B, Hq, Hkv, D, cap = 2, 4, 2, 64, 1400
+    q, kn, vn = (normal(30 + i, B, N, h, D, dtype=dtype) for i, h in enumerate((Hq, Hkv, Hkv)))
+    k, v = normal(33, B, cap, Hkv, D, dtype=dtype), normal(34, B, cap, Hkv, D, dtype=dtype)
+    parents, lengths = torch.tensor([[-1, 0, 0, 1, 2] + [3] * (N - 5)] * B, dtype=torch.int32), torch.tensor([1300, 900], dtype=torch.int32)
+    want, want_l, tol, tol_l = tree_reference(q, kn, vn, k, v, parents, lengths)
+    k[0, 700, 1] = math.nan    # sequence 0, KV head 1: every row of its heads
+    kn[1, 2, 0] = math.nan     # sequence 1, KV head 0: drafts 2 and 4
+    q[0, 3, 0] = math.nan      # sequence 0, query head 0, draft 3
+    o, lse = pj.decode_tree(*(x.to(DEV) for x in (q, kn, vn, k, v, parents)), kv_lengths=lengths.to(DEV), return_lse=True, implementation=impl)
+    pj.check_status(DEV)
+    nan = torch.zeros(B, N, Hq, dtype=torch.bool)
+    nan[0, :, 2:] = True
+    nan[1, [2, 4], :2] = True
+    nan[0, 3, 0] = True
+    o, lse = o.cpu().double(), lse.cpu().double()
+    assert bool(torch.isnan(o[nan]).all()) and bool(torch.isnan(lse.transpose(1, 2)[nan]).all())
+    assert bool(((o - want).abs() <= tol)[~nan].all())
+    assert bool(((lse - want_l).abs() <= tol_l).transpose(1, 2)[~nan].all())
