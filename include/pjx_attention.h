@@ -438,7 +438,8 @@ size_t pjx_attn_decode_tree_workspace_bytes(int B, int N, int Hq, int Hkv, int D
  * lengths[b] + i for i < counts[b] (clamped to [0, P]), and lengths_out[b] = min(lengths[b] + counts[b], capacity);
  * lengths_out may be lengths.  Caches and block_table as in pjx_attn_decode_tree (any page_size).  A path entry outside [0, N), a row
  * past the capacity or a page outside the pool leaves its row as it was; `overflow` (int32 device word or NULL) is set to 1
- * where a sequence ran past the capacity.  A token's keys, its values and the drafts' strides are whole 16-byte units.
+ * where a sequence ran past the capacity.  A token's keys, its values and the drafts' strides are whole 16-byte units.  The caches do not
+ * share memory, unless v_cache is k_cache and v_new is k_new.
  */
 int pjx_kv_cache_accept(void* k_cache, void* v_cache, const void* k_new, int64_t k_new_batch_stride,
                         int64_t k_new_token_stride, const void* v_new, int64_t v_new_batch_stride,
@@ -481,6 +482,8 @@ int pjx_attn_key_weights(const void* q, const void* k, const float* lse, const f
  *   k_out ...    either k_cache, v_cache, weights themselves (in place, capacity_out = capacity) or other buffers.  Rows behind the
  *                kept ones are not written; the weights of the rows that fell free are cleared (in place: up to lengths[b],
  *                otherwise up to capacity_out), so that new keys start at zero.
+ *                Results share no memory with each other or, but in place, with a source; only values that are the keys (v_cache =
+ *                k_cache, D = Dv) may have v_out = k_out.
  *   workspace    pjx_kv_cache_evict_workspace_bytes(B, Hkv) bytes, 8-byte aligned.
  */
 int pjx_kv_cache_evict(const void* k_cache, const void* v_cache, const float* weights, const int32_t* lengths, void* k_out,

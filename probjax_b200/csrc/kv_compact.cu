@@ -373,6 +373,8 @@ int pjx_kv_cache_accept(void* k_cache, void* v_cache, const void* k_new, int64_t
   if ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(k_new) |
        reinterpret_cast<uintptr_t>(v_new)) & 15)
     return fail(PJX_ERR_UNSUPPORTED, "accept: buffers must be 16-byte aligned");
+  // a cache whose values are its keys, and drafts to match: their rows are written once
+  const bool one = k_cache == v_cache && k_new == v_new && D == Dv && k_new_batch_stride == v_new_batch_stride && k_new_token_stride == v_new_token_stride;
   if (P > 0 && N > 0 && rows_there) {  // (the drafts are read while the cache is written)
     const size_t rows = block_table ? (size_t)num_pages * page_size : (size_t)B * capacity;
     const size_t k_span = ((size_t)(B - 1) * k_new_batch_stride + (size_t)(N - 1) * k_new_token_stride + (size_t)Hkv * D) * es;
@@ -381,6 +383,8 @@ int pjx_kv_cache_accept(void* k_cache, void* v_cache, const void* k_new, int64_t
     if (overlap(k_new, k_span, k_cache, k_bytes) || overlap(k_new, k_span, v_cache, v_bytes) || overlap(v_new, v_span, k_cache, k_bytes) ||
         overlap(v_new, v_span, v_cache, v_bytes))
       return fail(PJX_ERR_BAD_ARG, "accept: the drafts lie inside the cache that is written");
+    if (!one && overlap(k_cache, k_bytes, v_cache, v_bytes))
+      return fail(PJX_ERR_BAD_ARG, "accept: the caches of keys and values share memory");
   }
   AcceptParams p = {};
   p.k_cache = k_cache; p.v_cache = v_cache;
@@ -390,7 +394,7 @@ int pjx_kv_cache_accept(void* k_cache, void* v_cache, const void* k_new, int64_t
   p.lengths = lengths; p.path = path; p.counts = counts; p.block_table = block_table;
   p.lengths_out = lengths_out; p.overflow = overflow;
   p.capacity = capacity; p.N = N; p.P = P; p.page_size = page_size; p.max_pages = max_pages; p.num_pages = num_pages;
-  p.k_units = (int)(Hkv * (size_t)D * es / 16); p.v_units = (int)(Hkv * (size_t)Dv * es / 16);
+  p.k_units = (int)(Hkv * (size_t)D * es / 16); p.v_units = one ? 0 : (int)(Hkv * (size_t)Dv * es / 16);
   kv_accept_kernel<<<dim3(kAcceptCluster, B), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
   count_launch();
   return check_cuda(cudaGetLastError(), "kv cache accept launch");
@@ -420,10 +424,16 @@ int pjx_kv_cache_evict(const void* k_cache, const void* v_cache, const float* we
   const bool in_place = k_out == k_cache;
   if ((v_out == v_cache) != in_place || (weights_out == weights) != in_place || (in_place && capacity_out != capacity))
     return fail(PJX_ERR_BAD_ARG, "evict: keys, values and weights move in place together, or all into other buffers");
-  if (!in_place && (overlap(k_cache, rows * capacity * D * es, k_out, rows * capacity_out * D * es) ||
-                    overlap(v_cache, rows * capacity * Dv * es, v_out, rows * capacity_out * Dv * es) ||
-                    overlap(weights, rows * capacity * 4, weights_out, rows * capacity_out * 4)))
-    return fail(PJX_ERR_BAD_ARG, "evict: source and result overlap in part");
+  const bool one = k_cache == v_cache && k_out == v_out && D == Dv;  // the values are the keys: their rows move once
+  const void *from[3] = {k_cache, v_cache, weights}, *to[3] = {k_out, v_out, weights_out};
+  const size_t row_bytes[3] = {D * es, Dv * es, 4};
+  for (int i = 0; i < 3; ++i)
+    for (int j = 0; j < 3; ++j) {
+      if (!in_place && overlap(from[i], rows * capacity * row_bytes[i], to[j], rows * capacity_out * row_bytes[j]))
+        return fail(PJX_ERR_BAD_ARG, "evict: source and result overlap in part");
+      if (i < j && !(one && j == 1) && overlap(to[i], rows * capacity_out * row_bytes[i], to[j], rows * capacity_out * row_bytes[j]))
+        return fail(PJX_ERR_BAD_ARG, "evict: keys, values and weights share memory that is written");
+    }
   const size_t need = pjx_kv_cache_evict_workspace_bytes(B, Hkv);
   if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 7))
     return fail(PJX_ERR_WORKSPACE, "evict workspace: need %zu bytes, 8-byte aligned, got %zu", need, workspace ? workspace_bytes : (size_t)0);
@@ -469,7 +479,7 @@ int pjx_kv_cache_evict(const void* k_cache, const void* v_cache, const float* we
   const int unit = vec ? 16 : (int)es;
   p.slice_units = 128 / unit;  // 128 bytes of a row
   p.slices_k = (p.row_k / unit + p.slice_units - 1) / p.slice_units;
-  p.slices_v = (p.row_v / unit + p.slice_units - 1) / p.slice_units;
+  p.slices_v = one ? 0 : (p.row_v / unit + p.slice_units - 1) / p.slice_units;
   p.row_splits = 1;
   if (!in_place)  // rows move independently: enough CTAs for eight per SM, at least two chunks each
     while (p.row_splits < 8 && (int64_t)B * Hkv * (p.slices_k + p.slices_v) * p.row_splits < 148 * 8 &&

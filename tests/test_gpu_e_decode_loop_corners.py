@@ -6,7 +6,7 @@ import threading
 import pytest
 import torch
 
-from _operators_ref import key_weights_reference, tree_reference
+from _operators_ref import evict_reference, key_weights_reference, tree_reference
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -246,3 +246,32 @@ def test_a_key_that_is_not_a_number_shows_in_the_rows_that_see_it(N, impl, dtype
     assert bool(torch.isnan(o[nan]).all()) and bool(torch.isnan(lse.transpose(1, 2)[nan]).all())
     assert bool(((o - want).abs() <= tol)[~nan].all())
     assert bool(((lse - want_l).abs() <= tol_l).transpose(1, 2)[~nan].all())
+
+
+def test_keys_and_values_that_are_one_tensor():
+    """A cache whose values are its keys: the rows move once, in place and into a shared result; accepted rows are written once."""
+    import probjax_b200 as pj
+
+    B, cap, Hkv, D, keep, lengths = 2, 700, 2, 64, 200, [700, 431]
+    k, w = normal(40, B, cap, Hkv, D, dtype=torch.bfloat16), normal(41, B, Hkv, cap).abs()
+    kept = evict_reference(k, k, w, lengths, keep, 9)
+    want = torch.stack([torch.stack([k[b, kept[b][h], h] for h in range(Hkv)], 1) for b in range(B)])
+    kd, wd, n = k.to(DEV), w.to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    ko, wo = torch.zeros(B, keep, Hkv, D, dtype=torch.bfloat16, device=DEV), torch.zeros(B, Hkv, keep, device=DEV)
+    _, idx = pj.evict(kd, kd, wd, n, keep, recent=9, out=(ko, ko, wo))
+    assert torch.equal(idx.cpu(), torch.tensor(kept, dtype=torch.int32)) and torch.equal(ko.cpu(), want)
+    pj.evict(kd, kd, wd, n, keep, recent=9)
+    assert torch.equal(kd[:, :keep].cpu(), want) and torch.equal(wd[:, :, :keep], wo)
+    kn = normal(42, B, 5, Hkv, D, dtype=torch.bfloat16).to(DEV)
+    before = kd.clone()
+    pj.accept_drafts(kn, kn, kd, kd, [[0, 3], [1, 2]], [2, 1], kv_lengths=[200, 200])
+    before[0, 200], before[0, 201], before[1, 200] = kn[0, 0], kn[0, 3], kn[1, 1]
+    assert torch.equal(kd, before)
+    with pytest.raises(ValueError, match="share"):
+        pj.accept_drafts(kn, kn.clone(), kd, kd, [[0, 3], [1, 2]], [2, 1], kv_lengths=[200, 200])
+    both = torch.zeros(B * cap * Hkv * D + 64, dtype=torch.bfloat16, device=DEV)
+    a, c = both[:-64].view(k.shape), both[64:].view(k.shape)
+    with pytest.raises(ValueError, match="share"):
+        pj.evict(a, c, wd, n, keep)
+    with pytest.raises(ValueError, match="share"):
+        pj.evict(kd, kd.clone(), wd, n, keep, out=(ko, ko, wo))
