@@ -43,6 +43,8 @@ def _int32(x, device, shape, what):
     t = torch.as_tensor(x)
     if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
         raise ValueError(f"{what} must hold integers, got {t.dtype}")
+    if t.dtype not in (torch.int32, torch.int16, torch.int8, torch.uint8):  # (wrapped to 32 bits, a number far out of range might be in range)
+        t = t.to(torch.int64).clamp(-2 ** 31, 2 ** 31 - 1)
     t = t.to(device=device, dtype=torch.int32).contiguous()
     if tuple(t.shape) != tuple(shape):
         raise ValueError(f"{what} must be {list(shape)}, got {tuple(t.shape)}")

@@ -82,3 +82,18 @@ def test_accept_refuses_caches_that_share_memory(L, kw):
 
     assert accept(L, **kw) == BAD
     assert "share" in _lib.last_error()
+
+
+def test_integers_beyond_32_bits_stay_out_of_range():
+    """Parents, lengths, paths and pages of 64-bit tensors: what does not fit is cut to the nearest 32-bit number, which is as far out of range,
+    and does not come back as a small one."""
+    from probjax_b200.drafts import _int32
+
+    big = torch.tensor([2 ** 32, 2 ** 32 - 1, -2 ** 40, 2 ** 63 - 1, -2 ** 63, 7, -1, 2 ** 31 - 1])
+    want = [2 ** 31 - 1, 2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, -2 ** 31, 7, -1, 2 ** 31 - 1]
+    assert _int32(big, torch.device("cpu"), (8,), "parents").tolist() == want
+    assert _int32(big.tolist(), torch.device("cpu"), (8,), "parents").tolist() == want
+    for dtype in (torch.uint8, torch.int8, torch.int16):
+        assert _int32(torch.tensor([3, 100], dtype=dtype), torch.device("cpu"), (2,), "path").tolist() == [3, 100]
+    assert _int32(torch.tensor([5, 2 ** 32 - 1], dtype=torch.uint32), torch.device("cpu"), (2,), "path").tolist() == [5, 2 ** 31 - 1]
+    assert _int32(torch.zeros((0, 3), dtype=torch.int64), torch.device("cpu"), (0, 3), "path").shape == (0, 3)
