@@ -646,6 +646,9 @@ size_t pjx_attn_fwd_host_staging_bytes(int bias_batch, int bias_heads, int has_l
 /* Synchronises `stream`, reads the device status word and returns it (0 = ok). */
 int pjx_read_status(const int32_t* status, void* stream);
 
+/* A status word of the library's own on the current device, zero at first, for callers that keep none; may be asked for in a capture. */
+int pjx_status_word(int32_t** word);
+
 /* Number of this library's kernels launched by the calling process so far. */
 int64_t pjx_launch_count(void);
 

@@ -107,6 +107,7 @@ SIGNATURES = {
                                _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _vp, _sz, _vp]),
     "pjx_attn_fwd_host_staging_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i]),
     "pjx_read_status": (_i, [_vp, _vp]),
+    "pjx_status_word": (_i, [C.POINTER(_vp)]),
     "pjx_launch_count": (_i64, []),
 }
 

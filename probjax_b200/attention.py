@@ -13,6 +13,7 @@ or a GPU is missing.
 
 from __future__ import annotations
 
+import ctypes
 import math
 import threading
 from typing import Optional
@@ -47,13 +48,21 @@ def _stream(device) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
+class _DeviceWord:
+    """An int32 at a device address, for ``torch.as_tensor``."""
+
+    def __init__(self, address):
+        self.__cuda_array_interface__ = {"shape": (1,), "typestr": "<i4", "data": (address, False), "version": 3, "strides": None}
+
+
 def _status_word(device) -> torch.Tensor:
     key = device.index or 0
     word = _status_words.get(key)
     if word is None:
-        word = torch.zeros(1, dtype=torch.int32, device=device)
-        if not torch.cuda.is_current_stream_capturing():  # (a graph's memory goes with the graph: its calls get a word of their own)
-            _status_words[key] = word
+        # The library's own, not allocated here: in a capture that memory would be the graph's, cleared by every replay.
+        address = ctypes.c_void_p()
+        _launch(key, _lib.lib().pjx_status_word, ctypes.byref(address))
+        word = _status_words[key] = torch.as_tensor(_DeviceWord(address.value), device=torch.device("cuda", key))
     return word
 
 

@@ -911,4 +911,18 @@ int pjx_read_status(const int32_t* status, void* stream) {
   return PJX_OK;
 }
 
+static __device__ int32_t g_status_word;
+
+int pjx_status_word(int32_t** word) {
+  if (!word) return fail(PJX_ERR_BAD_ARG, "status word: null pointer");
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // (the module may have to be loaded first, which allocates)
+  int rc = check_cuda(cudaThreadExchangeStreamCaptureMode(&mode), "capture mode");
+  if (rc) return rc;
+  void* p = nullptr;
+  rc = check_cuda(cudaGetSymbolAddress(&p, g_status_word), "address of the status word");
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  *word = static_cast<int32_t*>(p);
+  return rc;
+}
+
 }  // extern "C"

@@ -275,3 +275,33 @@ def test_keys_and_values_that_are_one_tensor():
         pj.evict(a, c, wd, n, keep)
     with pytest.raises(ValueError, match="share"):
         pj.evict(kd, kd.clone(), wd, n, keep, out=(ko, ko, wo))
+
+
+def test_a_status_word_first_needed_in_a_capture(monkeypatch):
+    """The word that a captured call reports to is the one that ``check_status`` reads, also where the capture is the process's first call."""
+    import probjax_b200 as pj
+    from probjax_b200 import _lib
+    from probjax_b200 import attention as A
+
+    t = lambda i, *s: normal(50 + i, *s, dtype=torch.bfloat16).to(DEV)
+    args = (t(0, 1, 3, 4, 64), t(1, 1, 3, 2, 64), t(2, 1, 3, 2, 64), t(3, 1, 256, 2, 64), t(4, 1, 256, 2, 64), torch.tensor([-1, 0, 0], dtype=torch.int32, device=DEV))
+    n = torch.tensor([200], dtype=torch.int32, device=DEV)
+    want = pj.decode_tree(*args, kv_lengths=n)
+    monkeypatch.setattr(A, "_status_words", {})
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = pj.decode_tree(*args, kv_lengths=n)
+    (word,) = A._status_words.values()
+    pj.check_status(DEV)
+    graph.replay()
+    pj.check_status(DEV)
+    assert torch.equal(o, want)
+    word.fill_(_lib.PJX_ERR_DEVICE_TIMEOUT)  # what a kernel whose wait ran out writes
+    with pytest.raises(_lib.KernelTimeout):
+        pj.check_status(DEV)
+    pj.check_status(DEV)
+    del graph, o
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    assert int(word) == 0
