@@ -314,8 +314,10 @@ int launch_generic_t(const TreeParams& p, cudaStream_t stream) {
               : ncol == 2 ? attn_tree_kernel<T, 2, RT>
               : ncol == 3 ? attn_tree_kernel<T, 3, RT>
                           : attn_tree_kernel<T, 4, RT>;
-  const int smem = ((BM + BN) * pitch4(p.D) + BN * pitch4(p.Dv) + BM * PP) * (int)sizeof(float);
-  int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute(tree)");
+  auto smem_bytes = [](int D, int Dv) { return ((BM + BN) * pitch4(D) + BN * pitch4(Dv) + BM * PP) * (int)sizeof(float); };
+  const int smem = smem_bytes(p.D, p.Dv);
+  static std::atomic<uint64_t> allowed[4] = {};  // (for the widest call: another thread's must not lower it before this launch)
+  int rc = allow_smem(reinterpret_cast<const void*>(kern), smem_bytes(256, 64 * ncol), allowed[ncol - 1]);
   if (rc) return rc;
   kern<<<p.ctas, NT, smem, stream>>>(p);
   count_launch();

@@ -105,9 +105,10 @@ __global__ void __launch_bounds__(NT) key_weights_kernel(const KeyWeightsParams 
 
 template <typename T>
 int launch_t(const KeyWeightsParams& p, cudaStream_t stream) {
-  const int smem = (2 * BT * pitch4(p.D) + BT + 16 * BT) * (int)sizeof(float);
-  int rc = check_cuda(cudaFuncSetAttribute(key_weights_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
-                      "cudaFuncSetAttribute(key weights)");
+  auto smem_bytes = [](int D) { return (2 * BT * pitch4(D) + BT + 16 * BT) * (int)sizeof(float); };
+  const int smem = smem_bytes(p.D);
+  static std::atomic<uint64_t> allowed{0};  // (for the widest call: another thread's must not lower it before this launch)
+  int rc = allow_smem(reinterpret_cast<const void*>(key_weights_kernel<T>), smem_bytes(256), allowed);
   if (rc) return rc;
   key_weights_kernel<T><<<dim3((p.Lkv + BT - 1) / BT, p.Hkv, p.B), NT, smem, stream>>>(p);
   count_launch();

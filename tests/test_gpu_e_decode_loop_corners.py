@@ -305,3 +305,37 @@ def test_a_status_word_first_needed_in_a_capture(monkeypatch):
     torch.cuda.synchronize()
     torch.cuda.empty_cache()
     assert int(word) == 0
+
+
+def test_two_host_threads_with_different_head_widths():
+    """One kernel serves many head widths with shared memory of the call's size: a call of another thread does not take it away."""
+    import probjax_b200 as pj
+
+    def job(seed, D):
+        t = lambda i, *s: normal(seed + i, *s, dtype=torch.float32).to(DEV)
+        q, kn, k = t(0, 1, 20, 4, D), t(1, 1, 20, 2, D), t(2, 1, 130, 2, D)
+        lse, par = natural_lse(q.cpu(), k.cpu()).to(DEV), torch.arange(20, dtype=torch.int32, device=DEV) - 1
+
+        def once():
+            return pj.decode_tree(q, kn, kn, k, k, par, kv_lengths=[130]), pj.key_weights(q, k, lse)
+        return once
+
+    jobs = [job(300, 196), job(310, 256)]  # (both in the instantiation of 256 columns)
+    alone = [f() for f in jobs]
+    wrong, start = [], threading.Barrier(2)
+
+    def loop(f, want):
+        try:
+            start.wait(timeout=60)
+            for _ in range(100):
+                if not all(torch.equal(a, b) for a, b in zip(f(), want)):
+                    wrong.append("differs")
+        except Exception as e:
+            wrong.append(e)
+
+    threads = [threading.Thread(target=loop, args=a) for a in zip(jobs, alone)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong[:3]
