@@ -3,7 +3,7 @@
 // (padding of a ragged batch) gives o = 0 and lse = +inf.
 //
 // This file holds the exact fp32 kernel on CUDA cores (fp32 inputs, head widths and alignments that the tensor-core kernel of
-// attn_tree_sm100.cu does not take), the exact combine of the splits, and the entry point.
+// attn_tree_sm100.cu does not take; P stays in 32 bits, the one rounding is the result's), the exact combine of the splits, and the entry point.
 //
 // The work is cut into equal runs of (row tile, key tile) pairs, one per CTA (tree_plan.cuh); every segment of a run leaves O,
 // normalised by its own sum, and a base-2 log-sum-exp in fp32.
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(NT) attn_tree_kernel(const TreeParams p) {
         for (int c = 0; c < 4; ++c) {
           const float pv = exp2f(s[i][c] - m_safe);
           rsum += pv;
-          Ps[r * PP + tx + 16 * c] = Elem<T>::round(pv);  // as the other attention kernels round P before the product with V
+          Ps[r * PP + tx + 16 * c] = pv;
         }
 #pragma unroll
         for (int off = 8; off >= 1; off >>= 1) rsum += __shfl_xor_sync(0xffffffffu, rsum, off);

@@ -6,7 +6,7 @@ import threading
 import pytest
 import torch
 
-from _operators_ref import evict_reference, key_weights_reference, tree_reference
+from _operators_ref import HALF_STEP, attention_row, evict_reference, key_weights_reference, tree_reference
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -339,3 +339,22 @@ def test_two_host_threads_with_different_head_widths():
     for t in threads:
         t.join()
     assert not wrong, wrong[:3]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_the_exact_tree_kernel_rounds_only_its_result(dtype):
+    """16-bit inputs of a head width that the tensor cores do not take: sums in 32 bits, one rounding at the end."""
+    import probjax_b200 as pj
+
+    B, N, Hq, Hkv, D, cap = 2, 7, 4, 2, 96, 500
+    q, kn, vn = (normal(60 + i, B, N, h, D, dtype=dtype) for i, h in enumerate((Hq, Hkv, Hkv)))
+    k, v = normal(63, B, cap, Hkv, D, dtype=dtype), normal(64, B, cap, Hkv, D, dtype=dtype)
+    parents, n = [-1, 0, 0, 1, 3, -1, 5], [500, 33]
+    o = pj.decode_tree(*(x.to(DEV) for x in (q, kn, vn, k, v)), parents, kv_lengths=n).cpu().double()
+    chains = {0: [0], 2: [0, 2], 4: [0, 1, 3, 4], 6: [5, 6]}
+    for b in range(B):
+        for h in range(Hq):
+            for i, c in chains.items():
+                keys, vals = torch.cat([k[b, :n[b], h // 2], kn[b, c, h // 2]]), torch.cat([v[b, :n[b], h // 2], vn[b, c, h // 2]])
+                r, _, _, tol, _ = attention_row(q[b, i, h], keys, vals, 1 / math.sqrt(D))
+                assert bool(((o[b, i, h] - r).abs() <= tol + HALF_STEP[dtype] * (r.abs() + tol)).all())
