@@ -115,8 +115,12 @@ class DecodeCache:
     def attend_tree(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, parents, *, sm_scale: float | None = None,
                     return_lse: bool = False):
         """Attention of a tree of drafted tokens ``query [B, N, Hq, D]`` over the filled prefix and their ancestors among the
-        drafts (:func:`decode_tree`); ``key`` / ``value`` ``[B, N, Hkv, D]`` are the drafts' own and do not enter the cache.  Nothing is
-        added to ``key_weights``: for the accepted drafts that is a call of :func:`key_weights` with ``return_lse``'s result."""
+        drafts (:func:`decode_tree`); ``key`` / ``value`` ``[B, N, Hkv, D]`` are the drafts' own and do not enter the cache.
+
+        Nothing is added to ``key_weights``.  For the accepted drafts that is, after :meth:`accept` and before an eviction, one call of :func:`key_weights` for
+        every depth ``i`` of the path (a draft sees the keys up to its own, which is another end for every sequence and depth, and a call
+        has one end a sequence): the queries and ``lse`` rows of drafts ``path[:, i]``, ``lse = +inf`` where ``i >= counts``, the cache's
+        keys, ``mask=KVLenMask(lengths + i + 1)`` with the lengths before the acceptance, ``weights`` and ``out`` the cache's."""
         return decode_tree(query, key, value, self.cached_key, self.cached_value, parents, kv_lengths=self.cache_index, sm_scale=sm_scale,
                            return_lse=return_lse)
 

@@ -358,3 +358,47 @@ def test_the_exact_tree_kernel_rounds_only_its_result(dtype):
                 keys, vals = torch.cat([k[b, :n[b], h // 2], kn[b, c, h // 2]]), torch.cat([v[b, :n[b], h // 2], vn[b, c, h // 2]])
                 r, _, _, tol, _ = attention_row(q[b, i, h], keys, vals, 1 / math.sqrt(D))
                 assert bool(((o[b, i, h] - r).abs() <= tol + HALF_STEP[dtype] * (r.abs() + tol)).all())
+
+
+def loop_inputs(seed, B, N, Hq, Hkv, D):
+    return [normal(seed + i, B, N, h, D, dtype=torch.bfloat16).to(DEV) for i, h in enumerate((Hq, Hkv, Hkv))]
+
+
+def test_accepted_drafts_of_a_ragged_batch_get_their_weights():
+    """The recipe of ``DecodeCache.attend_tree``: one call a depth, with that depth's query of every sequence, the lengths up to it and
+    lse = +inf where nothing was accepted so deep, adds for a ragged batch what the accepted drafts paid to every key."""
+    import probjax_b200 as pj
+
+    B, N, Hq, Hkv, D, cap = 3, 7, 8, 2, 64, 256
+    cache = pj.DecodeCache(B, cap, Hkv, D, track_weights=True)
+    k0, v0 = (normal(80 + i, B, cap, Hkv, D, dtype=torch.bfloat16).to(DEV) for i in range(2))
+    lengths = [150, 64, 0]
+    cache.cached_key.copy_(k0)
+    cache.cached_value.copy_(v0)
+    cache.reset(lengths)
+    q, k, v = loop_inputs(82, B, N, Hq, Hkv, D)
+    parents = torch.tensor([-1, 0, 0, 1, 2, 3, -9], dtype=torch.int32, device=DEV)
+    path = torch.tensor([[0, 1, 3, 5], [0, 2, 4, 6], [0, 0, 0, 0]], dtype=torch.int32, device=DEV)
+    counts = torch.tensor([4, 3, 1], dtype=torch.int32, device=DEV)
+    old, before = cache.cache_index.clone(), cache.key_weights.clone()
+    _, lse = cache.attend_tree(q, k, v, parents, return_lse=True)
+    cache.accept(k, v, path, counts)
+    for i in range(path.shape[1]):
+        at = path[:, i].long()[:, None]
+        q_i = q.gather(1, at[:, :, None, None].expand(B, 1, Hq, D))
+        l_i = lse.gather(2, at[:, None].expand(B, Hq, 1)).masked_fill((i >= counts)[:, None, None], math.inf)
+        pj.key_weights(q_i, cache.cached_key, l_i, weights=cache.key_weights, mask=pj.KVLenMask(old + i + 1), out=cache.key_weights)
+    pj.check_status(DEV)
+    grown = (cache.key_weights - before).cpu().double()
+    want, tol = torch.zeros(B, Hkv, cap, dtype=torch.float64), torch.zeros(B, Hkv, cap, dtype=torch.float64)
+    keys = cache.cached_key.cpu()
+    for b in range(B):
+        for i in range(int(counts[b])):
+            n, node = lengths[b] + i + 1, int(path[b, i])
+            for h in range(Hq):
+                _, _, p, _, rel = attention_row(q[b, node, h].cpu(), keys[b, :n, h // 4], keys[b, :n, h // 4], 1 / math.sqrt(D))
+                want[b, h // 4, :n] += p
+                tol[b, h // 4, :n] += p * (2 * rel + 2.0 ** -20)  # (rel of the weight's own score and of the lse that the tree call gave)
+    assert bool(((grown - want).abs() <= tol + 2.0 ** -22 * (want + before.cpu().double())).all())
+    for b in range(B):  # every accepted draft paid one in all for each of its heads
+        assert abs(float(grown[b].sum()) - Hq * int(counts[b])) <= 2.0 ** -12 * Hq * int(counts[b])
