@@ -402,3 +402,54 @@ def test_accepted_drafts_of_a_ragged_batch_get_their_weights():
     assert bool(((grown - want).abs() <= tol + 2.0 ** -22 * (want + before.cpu().double())).all())
     for b in range(B):  # every accepted draft paid one in all for each of its heads
         assert abs(float(grown[b].sum()) - Hq * int(counts[b])) <= 2.0 ** -12 * Hq * int(counts[b])
+
+
+def test_draft_verify_accept_and_evict_in_one_graph():
+    """A step of the loop -- verification, acceptance, a tracked decode step, eviction -- captured once and replayed for three steps of new
+    inputs leaves what the same calls leave one by one."""
+    import probjax_b200 as pj
+
+    B, N, Hq, Hkv, D, cap, keep = 2, 6, 8, 2, 128, 160, 96
+    caches = [pj.DecodeCache(B, cap, Hkv, D, track_weights=True) for _ in range(2)]
+    k0, v0, w0 = (normal(90 + i, *s, dtype=x).to(DEV) for i, (s, x) in enumerate((((B, cap, Hkv, D), torch.bfloat16), ((B, cap, Hkv, D), torch.bfloat16),
+                                                                                  ((B, Hkv, cap), torch.float32))))
+    parents = torch.tensor([-1, 0, 0, 1, 2, 4], dtype=torch.int32, device=DEV)
+
+    def start(c):
+        c.cached_key.copy_(k0)
+        c.cached_value.copy_(v0)
+        c.reset([90, 60])
+        c.key_weights.copy_(w0.abs() * (torch.arange(cap, device=DEV) < 60))
+
+    def step(c, drafts, token, path, counts):
+        o, lse = c.attend_tree(*drafts, parents, return_lse=True)
+        c.accept(drafts[1], drafts[2], path, counts)
+        s = c.step(*token)
+        return o, lse, s, c.evict(keep, recent=8)
+
+    ins = [(loop_inputs(100 + 10 * i, B, N, Hq, Hkv, D), loop_inputs(200 + 10 * i, B, 1, Hq, Hkv, D),
+            torch.tensor([[0, 1, 3, 3], [0, 2, 4, 5]], dtype=torch.int32, device=DEV), torch.tensor([3, 4 - i], dtype=torch.int32, device=DEV)) for i in range(3)]
+    for c in caches:
+        start(c)
+    held = [[x.clone() for x in part] if isinstance(part, list) else part.clone() for part in ins[0]]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(caches[0], *held)
+    start(caches[0])
+    for args in ins:
+        for a, b in zip(held, args):
+            for x, y in zip(a, b) if isinstance(a, list) else ((a, b),):
+                x.copy_(y)
+        graph.replay()
+        want = step(caches[1], *args)
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+        for b in range(B):
+            n = int(caches[1].cache_index[b])
+            assert int(caches[0].cache_index[b]) == n
+            assert torch.equal(caches[0].cached_key[b, :n], caches[1].cached_key[b, :n]) and torch.equal(caches[0].cached_value[b, :n], caches[1].cached_value[b, :n])
+        assert torch.equal(caches[0].key_weights, caches[1].key_weights)
+    assert int(caches[1].cache_index[0]) == keep  # (it was cut on the way)
+    pj.check_status(DEV)
