@@ -453,3 +453,30 @@ def test_draft_verify_accept_and_evict_in_one_graph():
         assert torch.equal(caches[0].key_weights, caches[1].key_weights)
     assert int(caches[1].cache_index[0]) == keep  # (it was cut on the way)
     pj.check_status(DEV)
+
+
+@pytest.mark.parametrize("cap,keep,recent", [(33_000, 5000, 7), (70_001, 20_000, 0), (140_000, 129_999, 50), (300_003, 1000, 50), (300_003, 262_145, 0)])
+@pytest.mark.parametrize("place", ["in place", "other buffers"])
+def test_eviction_from_long_caches_keeps_the_right_keys(cap, keep, recent, place):
+    """Two, four and eight CTAs a head, and more weights than they hold in shared memory.  The kept keys against a stable sort of a copy of
+    the weights, which take 4096 values and zero, so that the threshold cuts through ties."""
+    import probjax_b200 as pj
+
+    Hkv, D = 2, 8
+    g = torch.Generator().manual_seed(cap + keep)
+    k, v = normal(70, 1, cap, Hkv, D, dtype=torch.bfloat16), normal(71, 1, cap, Hkv, D, dtype=torch.bfloat16)
+    w = torch.randint(0, 4096, (1, Hkv, cap), generator=g).float() / 64
+    kd, vd, wd = k.to(DEV), v.to(DEV), w.to(DEV)
+    out = None if place == "in place" else tuple(torch.zeros(s, dtype=x, device=DEV) for s, x in (
+        ((1, keep, Hkv, D), k.dtype), ((1, keep, Hkv, D), k.dtype), ((1, Hkv, keep), w.dtype)))
+    n, idx = pj.evict(kd, vd, wd, [cap], keep, recent=recent, out=out)
+    ko, vo, wo = (kd, vd, wd) if out is None else out
+    assert n.tolist() == [keep]
+    for h in range(Hkv):
+        order = torch.sort(w[0, h, :cap - recent], descending=True, stable=True).indices[:keep - recent]
+        rows = torch.cat([order.sort().values, torch.arange(cap - recent, cap)])
+        assert torch.equal(idx[0, h].cpu().long(), rows)
+        assert torch.equal(ko[0, :keep, h].cpu(), k[0, rows, h]) and torch.equal(vo[0, :keep, h].cpu(), v[0, rows, h])
+        assert torch.equal(wo[0, h, :keep].cpu(), w[0, h, rows])
+    if out is None:
+        assert not bool(wd[:, :, keep:].any())
