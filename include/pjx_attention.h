@@ -465,8 +465,8 @@ size_t pjx_attn_decode_weights_workspace_bytes(int B, int Lq, int Hq, int Hkv, i
 /*
  * The same sum for queries whose attention has been taken: from q [B, Lq, Hq, D], k [B, Lkv, Hkv, D] and the call's
  * natural-log lse [B, Hq, Lq], weights_out[b, hk, j] = weights_in[b, hk, j] + sum over the rows that see key j of
- * exp(sm_scale q.k - lse).  Mask: the band of pjx_attn_fwd_band and kv_lengths.  Rows with lse = +inf add nothing.  A fixed order of
- * summation: results repeat bit by bit.
+ * exp(sm_scale q.k - lse).  Mask: the band of pjx_attn_fwd_band and kv_lengths.  Rows with lse = +inf add nothing, whatever q holds
+ * there.  A fixed order of summation: results repeat bit by bit.
  */
 int pjx_attn_key_weights(const void* q, const void* k, const float* lse, const float* weights_in, float* weights_out,
                          const int32_t* kv_lengths, int B, int Lq, int Lkv, int Hq, int Hkv, int D, int dtype,

@@ -117,10 +117,11 @@ class DecodeCache:
         """Attention of a tree of drafted tokens ``query [B, N, Hq, D]`` over the filled prefix and their ancestors among the
         drafts (:func:`decode_tree`); ``key`` / ``value`` ``[B, N, Hkv, D]`` are the drafts' own and do not enter the cache.
 
-        Nothing is added to ``key_weights``.  For the accepted drafts that is, after :meth:`accept` and before an eviction, one call of :func:`key_weights` for
-        every depth ``i`` of the path (a draft sees the keys up to its own, which is another end for every sequence and depth, and a call
-        has one end a sequence): the queries and ``lse`` rows of drafts ``path[:, i]``, ``lse = +inf`` where ``i >= counts``, the cache's
-        keys, ``mask=KVLenMask(lengths + i + 1)`` with the lengths before the acceptance, ``weights`` and ``out`` the cache's."""
+        Nothing is added to ``key_weights``.  For the accepted drafts that is, after :meth:`accept` and before an eviction, one call of
+        :func:`key_weights` for every depth ``i`` of the path (a draft sees the keys up to its own, which is another end for every sequence
+        and depth, and a call has one end a sequence): the queries and ``lse`` rows of drafts ``path[:, i]``, ``lse = +inf`` where
+        ``i >= counts``, the cache's keys, ``mask=KVLenMask(lengths + i + 1)`` with the lengths before the acceptance, ``weights`` and
+        ``out`` the cache's."""
         return decode_tree(query, key, value, self.cached_key, self.cached_value, parents, kv_lengths=self.cache_index, sm_scale=sm_scale,
                            return_lse=return_lse)
 
@@ -132,7 +133,8 @@ class DecodeCache:
 
     def evict(self, keep: int, *, recent: int = 0) -> torch.Tensor:
         """Cut every sequence to ``keep`` keys per KV head, by ``key_weights`` and with the ``recent`` last ones kept
-        (:func:`evict`), in place.  Returns the kept keys' former indices ``int32 [B, Hkv, keep]``."""
+        (:func:`evict`), in place.  Returns the kept keys' former indices ``int32 [B, Hkv, keep]``.  ``cache_index`` counts the kept keys from
+        then on, not the tokens seen: whoever rotates queries and keys to their positions counts tokens apart."""
         if self.key_weights is None:
             raise ValueError("evict needs a cache with track_weights=True")
         return evict(self.cached_key, self.cached_value, self.key_weights, self.cache_index, keep, recent=recent,

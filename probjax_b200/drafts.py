@@ -95,8 +95,9 @@ def decode_tree(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_cac
     the cache is contiguous ``[B, capacity, Hkv, D]`` or, with ``block_table [B, max_pages]``, a page pool
     ``[num_pages, page_size, Hkv, D]`` with a page size that is a multiple of 16.  At most 256 drafts a sequence.
 
-    A chain of drafts is ``parents = arange(N) - 1``.  Positions for a rotary embedding are ``kv_lengths + depth``
-    (:func:`probjax_b200.rope_axes`).  Returns ``o [B, N, Hq, Dv]`` and, with ``return_lse``, ``lse [B, Hq, N]``; no gradient (inputs
+    A chain of drafts is ``parents = arange(N) - 1``.  Positions for a rotary embedding (:func:`probjax_b200.rope_axes`) are the tokens that
+    the sequence has seen plus ``depth``: ``kv_lengths + depth`` as long as no key has been evicted, a count of the caller's own after that.
+    A NaN or an infinity in the value of a draft that is there reaches the others too (0 times it is NaN); absent drafts may hold anything.  Returns ``o [B, N, Hq, Dv]`` and, with ``return_lse``, ``lse [B, Hq, N]``; no gradient (inputs
     that ask for one are refused)."""
     _require_gpu()
     if implementation not in _IMPL:

@@ -81,7 +81,8 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, weights:
                 sm_scale: float | None = None, out: torch.Tensor | None = None, implementation: str | None = None) -> torch.Tensor:
     """What every key received of an attention call that has been made (``pjx_attn_key_weights``): ``weights`` (float32
     ``[B, Hkv, Lkv]``, ``None``: zeros) plus the sum over the queries that see it of ``exp(sm_scale q.k - lse)``, with the call's own
-    ``mask``, ``sm_scale`` (default ``1/sqrt(D)``) and natural-log ``lse [B, Hq, Lq]``.  ``mask`` may hold key lengths and bands
+    ``mask``, ``sm_scale`` (default ``1/sqrt(D)``) and natural-log ``lse [B, Hq, Lq]``; a row with ``lse = +inf`` adds nothing, whatever
+    its query holds.  ``mask`` may hold key lengths and bands
     (causal, windows, bottom-right causal).  ``out`` takes the sum and may be ``weights`` itself.  No gradient (inputs that ask for one
     are refused)."""
     _require_gpu()
@@ -116,6 +117,9 @@ def evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor, k
     others, those with the largest ``weights`` (float32 ``[B, Hkv, capacity]``; ties go to the lowest index, NaN ranks last).  Shorter
     sequences keep all.  The kept rows move to the front in their order: in place, or into ``out = (k, v, weights)`` of the same layout
     and a capacity of at least ``keep`` (rows behind the kept ones stay as they were there; free weights become 0).
+
+    Keys keep the angles that a rotary embedding gave them, and the new lengths no longer count the tokens seen: positions of further tokens
+    follow a count of the caller's own.  Results share no memory with each other; in place, ``v_cache`` may be ``k_cache``.
 
     Returns ``(lengths, kept)``: the new lengths ``int32 [B]`` (``lengths_out`` takes them and may be the tensor of
     ``kv_lengths``) and the kept keys' former indices ``int32 [B, Hkv, keep]``, ``-1`` behind them."""

@@ -480,3 +480,41 @@ def test_eviction_from_long_caches_keeps_the_right_keys(cap, keep, recent, place
         assert torch.equal(wo[0, h, :keep].cpu(), w[0, h, rows])
     if out is None:
         assert not bool(wd[:, :, keep:].any())
+
+
+def test_positions_count_tokens_and_not_kept_keys():
+    """Decode steps with rotary positions over a cache that is cut on the way: a step's angles follow the tokens seen, the kept keys keep theirs,
+    and attention is that of the kept tokens at their places in the text."""
+    import probjax_b200 as pj
+
+    B, Hq, Hkv, D, cap, keep = 2, 4, 2, 64, 64, 20
+    cache = pj.DecodeCache(B, cap, Hkv, D, track_weights=True)
+    seen = torch.zeros(B, dtype=torch.int32, device=DEV)
+    places = [[[] for _ in range(Hkv)] for _ in range(B)]  # the tokens that every head holds
+    k_all, v_all = [], []
+    for i in range(60):
+        q, k, v = (normal(400 + 3 * i + j, B, 1, h, D) for j, h in enumerate((Hq, Hkv, Hkv)))
+        q, k, v = q.bfloat16().to(DEV), k.bfloat16().to(DEV), v.bfloat16().to(DEV)
+        pos = seen[:, None, None]
+        qr, kr = pj.rope_axes(q, pos, (D,)), pj.rope_axes(k, pos, (D,))
+        o = cache.step(qr, kr, v)
+        k_all.append(kr[:, 0].cpu())
+        v_all.append(v[:, 0].cpu())
+        seen += 1
+        for b in range(B):
+            for h in range(Hkv):
+                places[b][h].append(i)
+        if i % 25 == 24:
+            kept = cache.evict(keep, recent=5).cpu()
+            for b in range(B):
+                for h in range(Hkv):
+                    places[b][h] = [places[b][h][j] for j in kept[b, h].tolist()]
+    assert cache.cache_index.tolist() == [30, 30] and seen.tolist() == [60, 60]
+    for b in range(B):
+        for h in range(Hq):
+            at = places[b][h // 2]
+            keys, vals = torch.stack([k_all[i][b, h // 2] for i in at]), torch.stack([v_all[i][b, h // 2] for i in at])
+            r, _, p, tol, _ = attention_row(qr[b, 0, h].cpu(), keys, vals, 1 / math.sqrt(D))
+            bound = tol + HALF_STEP[torch.bfloat16] * (p @ vals.double().abs() + r.abs())
+            assert bool(((o[b, 0, h].cpu().double() - r).abs() <= bound).all())
+    pj.check_status(DEV)
