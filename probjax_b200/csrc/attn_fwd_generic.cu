@@ -16,6 +16,7 @@
 // Bound by shared-memory loads: every inner loop reads 16 bytes per load (B2 L250 H4 D64 fp32: 84 -> 32 us
 // together with the smaller tile, which doubles the CTAs of grids that leave SMs idle).
 #include "pjx_common.cuh"
+#include "tile_f32.cuh"
 
 namespace pjx {
 namespace {
@@ -24,11 +25,6 @@ constexpr int BN = 64;
 constexpr int PP = BN + 4;  // pitch of the P tile
 constexpr int NT = 256;
 
-__host__ __device__ inline int pitch4(int d) { return (d + 3) / 4 * 4 + 4; }
-__device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast<const float4*>(p); }
-__device__ __forceinline__ float dot4(float4 a, float4 b, float s) {
-  return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, s))));
-}
 __device__ __forceinline__ void axpy4(float4& s, float a, float4 x) {
   s.x = fmaf(a, x.x, s.x);
   s.y = fmaf(a, x.y, s.y);

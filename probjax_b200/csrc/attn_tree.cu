@@ -7,6 +7,7 @@
 //
 // The work is cut into equal runs of (row tile, key tile) pairs, one per CTA (tree_plan.cuh); every segment of a run leaves O,
 // normalised by its own sum, and a base-2 log-sum-exp in fp32.
+#include "tile_f32.cuh"
 #include "tree_plan.cuh"
 
 namespace pjx {
@@ -16,12 +17,6 @@ constexpr int NT = 256;
 constexpr int BN = 64;
 constexpr int PP = BN + 4;
 constexpr int kWords = kTreeMaxNodes / 32;
-
-__host__ __device__ inline int pitch4(int d) { return (d + 3) / 4 * 4 + 4; }
-__device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast<const float4*>(p); }
-__device__ __forceinline__ float dot4(float4 a, float4 b, float s) {
-  return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, s))));
-}
 
 // Row of the cache that holds key `key` of sequence b, -1 for a page outside the pool.
 __device__ __forceinline__ int64_t cache_row(const TreeParams& p, int b, int key) {

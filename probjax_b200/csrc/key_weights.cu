@@ -6,6 +6,7 @@
 // (key_weights_sm100.cu) does not take.  One CTA owns 64 keys of one (sequence, KV head) and walks the packed rows
 // (t, g) in tiles of 64; 16 x 16 threads with 4 x 4 scores each.  Bound by shared-memory loads.
 #include "pjx_common.cuh"
+#include "tile_f32.cuh"
 
 namespace pjx {
 namespace {
@@ -13,11 +14,6 @@ namespace {
 constexpr int NT = 256;
 constexpr int BT = 64;  // keys and rows per tile
 
-__host__ __device__ inline int pitch4(int d) { return (d + 3) / 4 * 4 + 4; }
-__device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast<const float4*>(p); }
-__device__ __forceinline__ float dot4(float4 a, float4 b, float s) {
-  return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, s))));
-}
 // One row of `width` elements, zeros where there is none and up to a multiple of four; u: one of 8 threads.
 template <typename T>
 __device__ __forceinline__ void load_row(float* dst, const T* row, int width, bool there, int u) {

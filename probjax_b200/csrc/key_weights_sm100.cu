@@ -43,13 +43,6 @@ constexpr int BT = 128;          // keys of a tile, rows of a chunk
 constexpr int STEP = BT;         // keys of a step
 constexpr int NTHREADS = 576;
 
-__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, int c2, int c3, int c4) {
-  asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-      "[%0], [%1, {%3, %4, %5, %6, %7}], [%2];\n" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
-      : "memory");
-}
 
 __device__ __forceinline__ void st_shared1(uint32_t addr, float x) { asm volatile("st.shared.f32 [%0], %1;\n" ::"r"(addr), "f"(x) : "memory"); }
 __device__ __forceinline__ float ld_shared1(uint32_t addr) {

@@ -111,6 +111,11 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, weights:
     return out
 
 
+@functools.lru_cache(maxsize=256)
+def _evict_workspace(*sizes) -> int:
+    return _lib.lib().pjx_kv_cache_evict_workspace_bytes(*sizes)
+
+
 def evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor, kv_lengths, keep: int, *, recent: int = 0, out=None,
           lengths_out: torch.Tensor | None = None):
     """Cut every sequence of a cache to ``keep`` keys per KV head (``pjx_kv_cache_evict``): the ``recent`` last ones and, of the
@@ -151,7 +156,7 @@ def evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor, k
     elif tuple(lengths_out.shape) != (B,) or lengths_out.dtype != torch.int32 or lengths_out.device != dev or not lengths_out.is_contiguous():
         raise ValueError(f"evict: lengths_out must be a contiguous int32 [{B}] on {dev}")
     kept = torch.empty((B, Hkv, keep), dtype=torch.int32, device=dev)
-    ws = _workspace(dev, "evict", 8 * B * Hkv)  # pjx_kv_cache_evict_workspace_bytes
+    ws = _workspace(dev, "evict", _evict_workspace(B, Hkv))
     _launch(dev.index, _lib.lib().pjx_kv_cache_evict, _ptr(k_cache), _ptr(v_cache), _ptr(weights), _ptr(lengths), _ptr(ko), _ptr(vo), _ptr(wo),
             _ptr(lengths_out), _ptr(kept), B, Hkv, D, Dv, cap, cap_out, keep, recent, _DTYPES[k_cache.dtype], _ptr(ws), ws.numel(), _stream(dev))
     return lengths_out, kept
