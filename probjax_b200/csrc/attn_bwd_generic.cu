@@ -410,24 +410,24 @@ __global__ void __launch_bounds__(NT) bwd_dkdv_kernel(const BwdParams p) {
   }
 }
 
-template <typename K>
-int set_smem(K kern, size_t bytes, const char* what) {
-  if (bytes <= 48 * 1024) return PJX_OK;
-  return check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), what);
+// `most`: what the kernel's widest call takes, so that another thread's call does not lower the limit before this launch.
+int set_smem(const void* kern, size_t bytes, size_t most, std::atomic<uint64_t>& allowed) {
+  return bytes <= 48 * 1024 ? PJX_OK : allow_smem(kern, (int)most, allowed);
 }
 
 template <typename T_, int NCK, int NCV>
 int launch_widths(const BwdParams& p, cudaStream_t stream) {
-  const size_t smem = bwd_smem_bytes(p.D, p.Dv);
+  const size_t smem = bwd_smem_bytes(p.D, p.Dv), most = bwd_smem_bytes(256, 256);
+  static std::atomic<uint64_t> allowed_q{0}, allowed_k{0};
   int rc;
   auto kq = bwd_dq_kernel<T_, NCK>;
-  if ((rc = set_smem(kq, smem, "cudaFuncSetAttribute(backward dq)"))) return rc;
+  if ((rc = set_smem(reinterpret_cast<const void*>(kq), smem, most, allowed_q))) return rc;
   kq<<<dim3((p.Lq + T - 1) / T, p.Hq, p.B), NT, smem, stream>>>(p);
   count_launch();
   if ((rc = check_cuda(cudaGetLastError(), "backward dq launch"))) return rc;
   if (p.Lkv == 0) return PJX_OK;
   auto kk = bwd_dkdv_kernel<T_, NCK, NCV>;
-  if ((rc = set_smem(kk, smem, "cudaFuncSetAttribute(backward dk/dv)"))) return rc;
+  if ((rc = set_smem(reinterpret_cast<const void*>(kk), smem, most, allowed_k))) return rc;
   kk<<<dim3((p.Lkv + T - 1) / T, p.Hkv, p.B), NT, smem, stream>>>(p);
   count_launch();
   return check_cuda(cudaGetLastError(), "backward dk/dv launch");
@@ -672,8 +672,9 @@ template <typename T_, int NC>
 int launch_jvp_width(const JvpParams& p, cudaStream_t stream) {
   const size_t smem = jvp_smem_bytes(p.D, p.Dv);
   auto kern = jvp_kernel<T_, NC>;
+  static std::atomic<uint64_t> allowed{0};
   int rc;
-  if ((rc = set_smem(kern, smem, "cudaFuncSetAttribute(jvp)"))) return rc;
+  if ((rc = set_smem(reinterpret_cast<const void*>(kern), smem, jvp_smem_bytes(256, 256), allowed))) return rc;
   kern<<<dim3((p.Lq + T - 1) / T, p.Hq, p.B), NT, smem, stream>>>(p);
   count_launch();
   return check_cuda(cudaGetLastError(), "jvp launch");

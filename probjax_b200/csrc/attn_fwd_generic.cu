@@ -214,11 +214,12 @@ __global__ void __launch_bounds__(NT) attn_fwd_generic_kernel(const FwdParams p)
 template <typename T, int NCOL, int RT>
 int launch_t(const FwdParams& p, cudaStream_t stream) {
   constexpr int BM = 16 * RT;
-  const size_t smem = sizeof(float) * ((size_t)(BM + BN) * pitch4(p.D) + (size_t)BN * pitch4(p.Dv) + (size_t)BM * PP);
+  auto smem_bytes = [](int D, int Dv) { return sizeof(float) * ((size_t)(BM + BN) * pitch4(D) + (size_t)BN * pitch4(Dv) + (size_t)BM * PP); };
+  const size_t smem = smem_bytes(p.D, p.Dv);
   auto kern = attn_fwd_generic_kernel<T, NCOL, RT>;
+  static std::atomic<uint64_t> allowed{0};  // (for the widest call: another thread's must not lower it before this launch)
   if (smem > 48 * 1024) {
-    int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
-                        "cudaFuncSetAttribute(generic fwd)");
+    int rc = allow_smem(reinterpret_cast<const void*>(kern), (int)smem_bytes(256, 64 * NCOL), allowed);
     if (rc) return rc;
   }
   dim3 grid((p.Lq + BM - 1) / BM, p.Hq, p.B);

@@ -518,3 +518,33 @@ def test_positions_count_tokens_and_not_kept_keys():
             bound = tol + HALF_STEP[torch.bfloat16] * (p @ vals.double().abs() + r.abs())
             assert bool(((o[b, 0, h].cpu().double() - r).abs() <= bound).all())
     pj.check_status(DEV)
+
+
+def test_two_host_threads_with_different_head_widths_in_training():
+    """The same for the forward and backward kernels on CUDA cores."""
+    import probjax_b200 as pj
+
+    def job(seed, D):
+        q, k, dy = (normal(seed + i, 1, n, 2, D).to(DEV) for i, n in enumerate((70, 90, 70)))
+        o, lse = pj.attention_forward(q, k, k, sm_scale=0.07, return_lse=True)
+        return lambda: (pj.attention_forward(q, k, k, sm_scale=0.07), *pj.attention.attention_backward(q, k, k, o, lse, dy, sm_scale=0.07))
+
+    jobs = [job(320, 196), job(330, 256)]
+    alone = [f() for f in jobs]
+    wrong, start = [], threading.Barrier(2)
+
+    def loop(f, want):
+        try:
+            start.wait(timeout=60)
+            for _ in range(100):
+                if not all(torch.equal(a, b) for a, b in zip(f(), want)):
+                    wrong.append("differs")
+        except Exception as e:
+            wrong.append(e)
+
+    threads = [threading.Thread(target=loop, args=a) for a in zip(jobs, alone)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong[:3]
