@@ -56,7 +56,7 @@ class _DeviceWord:
 
 
 def _status_word(device) -> torch.Tensor:
-    key = device.index or 0
+    key = torch.cuda.current_device() if device.index is None else device.index
     word = _status_words.get(key)
     if word is None:
         # The library's own, not allocated here: in a capture that memory would be the graph's, cleared by every replay.
@@ -465,7 +465,7 @@ def _wants_grad(*tensors) -> bool:
 def _refuse_grad(what: str, *tensors) -> None:
     """Refuses inputs that ask for a gradient or carry a tangent where the call has neither."""
     if torch.is_grad_enabled():
-        asked = any([t.requires_grad for t in tensors if t is not None])
+        asked = any([getattr(t, "requires_grad", False) for t in tensors])
     else:
         asked = False
     if asked or (_forward_ad._current_level >= 0 and _wants_grad(*tensors)):

@@ -244,6 +244,8 @@ def rope_axes(x: torch.Tensor, positions, sections, *, base: float = 10_000.0, s
     else:
         raise ValueError(f"positions must be [T={T}, axes={len(sections)}] or [..., T, axes] with the leading dimensions {list(lead)}, "
                          f"got {tuple(pos.shape)}")
+    if torch.is_grad_enabled() and pos.requires_grad:
+        raise NotImplementedError("rope_axes has no gradient with respect to positions: detach them")
     x4 = x[None] if x.dim() == 3 else x if x.dim() == 4 else x.reshape((math.prod(lead),) + tuple(x.shape[-3:]))
     if _wants_grad(x):
         if out is not None:

@@ -173,7 +173,7 @@ extern "C" int pjx_rope_axes(const void* x, int64_t x_batch_stride, int64_t x_to
     return fail(PJX_ERR_BAD_ARG, "positions must be float32, int32 or int64 (got code %d)", position_type);
   if (B < 0 || T < 0 || H < 1 || D < 1) return fail(PJX_ERR_BAD_ARG, "negative or zero dimension");
   if (axes < 1 || axes > kMaxAxes || !sections) return fail(PJX_ERR_BAD_ARG, "rope: 1 to %d axes with a section each", kMaxAxes);
-  if (!(base > 0.f)) return fail(PJX_ERR_BAD_ARG, "base must be positive");
+  if (!(base > 0.f) || isinf(base)) return fail(PJX_ERR_BAD_ARG, "base must be positive and finite");
   int total = 0;
   for (int a = 0; a < axes; ++a) {
     if (sections[a] < 0 || sections[a] % 2 || sections[a] > D)

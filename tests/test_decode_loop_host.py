@@ -97,3 +97,12 @@ def test_integers_beyond_32_bits_stay_out_of_range():
         assert _int32(torch.tensor([3, 100], dtype=dtype), torch.device("cpu"), (2,), "path").tolist() == [3, 100]
     assert _int32(torch.tensor([5, 2 ** 32 - 1], dtype=torch.uint32), torch.device("cpu"), (2,), "path").tolist() == [5, 2 ** 31 - 1]
     assert _int32(torch.zeros((0, 3), dtype=torch.int64), torch.device("cpu"), (0, 3), "path").shape == (0, 3)
+
+
+def test_rope_axes_refuses_an_infinite_base(L):
+    """Its first frequency would be infinity to the power 0 by way of 0 times infinity."""
+    import ctypes
+
+    sections = (ctypes.c_int32 * 1)(64)
+    for base, rc in ((float("inf"), BAD), (1e30, 0)):
+        assert L.pjx_rope_axes(P, 0, 0, P, P, 0, 0, 1, sections, 0, 4, 2, 64, 0, 1, 0, base, 1, None) == rc  # (no sequence: nothing is launched)

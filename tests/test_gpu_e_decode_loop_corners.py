@@ -548,3 +548,14 @@ def test_two_host_threads_with_different_head_widths_in_training():
     for t in threads:
         t.join()
     assert not wrong, wrong[:3]
+
+
+def test_rope_axes_refuses_positions_that_ask_for_a_gradient():
+    import probjax_b200 as pj
+
+    x, pos = torch.zeros(1, 3, 2, 8, device=DEV), torch.zeros(3, 1, device=DEV, requires_grad=True)
+    with pytest.raises(NotImplementedError, match="positions"):
+        pj.rope_axes(x, pos, (8,))
+    with torch.no_grad():
+        pj.rope_axes(x, pos, (8,))
+    pj.rope_axes(x, pos.detach(), (8,))
