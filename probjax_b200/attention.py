@@ -21,6 +21,7 @@ from typing import Optional
 import numpy as np
 import torch
 import torch.autograd.forward_ad as _forward_ad
+from torch.autograd.graph import increment_version as _increment_version
 
 from . import _lib
 from .masks import (AttentionBias, AttentionMask, LoweredBias, LoweredMask, NoMask, lower_bias, lower_bias_structured,
@@ -101,6 +102,11 @@ def _launch(index: int, fn, *args) -> None:
             rc = fn(*args)
     if rc:
         _lib.check(rc)
+
+
+def _written(*tensors) -> None:
+    """Tells autograd that a kernel has written to these tensors, so that a gradient that needs what was there is refused."""
+    _increment_version([t for t in tensors if t is not None])
 
 
 def _workspace(device, tag: str, nbytes: int) -> torch.Tensor:

@@ -19,7 +19,7 @@ import math
 import torch
 
 from . import _lib
-from .attention import _DTYPES, _IMPL, _launch, _ptr, _require_gpu, _scratch_bytes, _status_word, _stream, _wants_grad, mha
+from .attention import _DTYPES, _IMPL, _launch, _ptr, _require_gpu, _scratch_bytes, _status_word, _stream, _wants_grad, _written, mha
 from .drafts import accept_drafts, decode_tree
 from .eviction import decode_weights, evict, key_weights
 from .masks import CausalFromBottomRightMask, KVLenMask
@@ -222,7 +222,8 @@ def rope_axes(x: torch.Tensor, positions, sections, *, base: float = 10_000.0, s
     by ``position * base**(-2 i / section)``; with ``shared`` the frequencies run through all axes,
     ``base**(-2 p / sum(sections))`` for pair ``p``.  ``interleaved``: pairs are neighbours, otherwise the two halves of the rotated
     part.  A slice of a fused projection is read in place.  Differentiable with respect to ``x`` (``positions`` must not change in place until the
-    gradient has been taken: the backward pass refuses then); ``out`` (dense, may be a dense ``x``) takes the result where no gradient is
+    gradient has been taken: the backward pass refuses then, except after :meth:`DecodeCache.update`, whose writes autograd does not see:
+    pass a copy of ``cache_index``); ``out`` (dense, may be a dense ``x``) takes the result where no gradient is
     wanted.  One axis is :func:`rope_interleaved` with positions per sequence."""
     _require_gpu()
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dim() < 3 or x.dtype not in _DTYPES:
@@ -262,6 +263,8 @@ def rope_axes(x: torch.Tensor, positions, sections, *, base: float = 10_000.0, s
             if first < out.data_ptr() + n and out.data_ptr() < last:
                 raise ValueError("rope_axes: out overlaps x without being it")
     y = _rope_axes_call(x4, pos, sections, base, shared, interleaved, False, out)
+    if out is not None:
+        _written(out)
     return y if x.dim() == 4 else y.reshape(x.shape)
 
 

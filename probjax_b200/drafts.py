@@ -16,7 +16,7 @@ import math
 import torch
 
 from . import _lib
-from .attention import _DTYPES, _IMPL, _launch, _ptr, _refuse_grad, _require_gpu, _status_word, _stream, _workspace
+from .attention import _DTYPES, _IMPL, _launch, _ptr, _refuse_grad, _require_gpu, _status_word, _stream, _workspace, _written
 
 
 def _token_rows(t: torch.Tensor):
@@ -159,4 +159,5 @@ def accept_drafts(k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Tenso
     _launch(dev.index, _lib.lib().pjx_kv_cache_accept, _ptr(k_cache), _ptr(v_cache), _ptr(k_new), kb, kt, _ptr(v_new), vb, vt, _ptr(lengths),
             _ptr(path), _ptr(counts), _ptr(table), B, N, path.shape[1], Hkv, D, Dv, cap, page, max_pages, num_pages, _DTYPES[k_new.dtype],
             _ptr(out), _ptr(overflow), _stream(dev))
+    _written(k_cache, v_cache, given, overflow)
     return out

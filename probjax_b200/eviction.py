@@ -16,7 +16,7 @@ import torch
 
 from . import _lib
 from .attention import (_DTYPES, _IMPL, _as_tensor, _band_args, _check_call, _launch, _ptr, _refuse_grad, _require_gpu, _status_word,
-                        _stream, _workspace)
+                        _stream, _workspace, _written)
 from .drafts import _int32
 from .masks import AttentionMask, split_mask
 
@@ -60,6 +60,7 @@ def decode_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     dev = q.device
     _refuse_grad("decode_weights", q, k_cache, v_cache, weights)
     lengths = None if kv_lengths is None else _int32(kv_lengths, dev, (B,), "kv_lengths")
+    given = out
     weights, out = _weights_args("decode_weights", weights, out, (B, Hkv, cap), dev)
     q, k_cache, v_cache = q.contiguous(), k_cache.contiguous(), v_cache.contiguous()
     o = torch.empty((B, Lq, Hq, Dv), dtype=q.dtype, device=dev)
@@ -74,6 +75,8 @@ def decode_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     _launch(dev.index, _lib.lib().pjx_attn_decode_weights, _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(lengths), _ptr(weights), _ptr(out),
             _ptr(o), _ptr(lse), B, Lq, Hq, Hkv, D, Dv, cap, _DTYPES[q.dtype], 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale),
             int(split_len), _ptr(ws), ws.numel(), _ptr(_status_word(dev)), _stream(dev))
+    if given is not None:
+        _written(given)
     return (o, lse, out) if return_lse else (o, out)
 
 
@@ -102,12 +105,15 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, weights:
     lengths = None if lm.kv_lengths is None else _as_tensor(lm.kv_lengths).to(device=dev, dtype=torch.int32).contiguous()
     if lengths is not None and lengths.numel() != B:
         raise ValueError(f"key_weights: key lengths must hold B={B} entries, got {lengths.numel()}")
+    given = out
     weights, out = _weights_args("key_weights", weights, out, (B, Hkv, Lkv), dev)
     q, k, lse = q.contiguous(), k.contiguous(), lse.contiguous()
     band_lo, band_hi = _band_args(False, lm.band)
     _launch(dev.index, _lib.lib().pjx_attn_key_weights, _ptr(q), _ptr(k), _ptr(lse), _ptr(weights), _ptr(out), _ptr(lengths), B, Lq, Lkv, Hq,
             Hkv, D, _DTYPES[q.dtype], band_lo, band_hi, 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), _IMPL[implementation],
             _ptr(_status_word(dev)), _stream(dev))
+    if given is not None:
+        _written(given)
     return out
 
 
@@ -151,6 +157,7 @@ def evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor, k
             raise ValueError(f"evict: {name} must be a contiguous {dtype} {list(shape)} on {dev}, got {t.dtype} {tuple(t.shape)}")
     if not k_cache.is_contiguous() or not v_cache.is_contiguous():
         raise ValueError("evict: the caches must be contiguous")
+    given = lengths_out
     if lengths_out is None:
         lengths_out = torch.empty_like(lengths)
     elif tuple(lengths_out.shape) != (B,) or lengths_out.dtype != torch.int32 or lengths_out.device != dev or not lengths_out.is_contiguous():
@@ -159,4 +166,5 @@ def evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor, k
     ws = _workspace(dev, "evict", _evict_workspace(B, Hkv))
     _launch(dev.index, _lib.lib().pjx_kv_cache_evict, _ptr(k_cache), _ptr(v_cache), _ptr(weights), _ptr(lengths), _ptr(ko), _ptr(vo), _ptr(wo),
             _ptr(lengths_out), _ptr(kept), B, Hkv, D, Dv, cap, cap_out, keep, recent, _DTYPES[k_cache.dtype], _ptr(ws), ws.numel(), _stream(dev))
+    _written(ko, vo, wo, given)
     return lengths_out, kept

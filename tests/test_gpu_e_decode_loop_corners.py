@@ -559,3 +559,37 @@ def test_rope_axes_refuses_positions_that_ask_for_a_gradient():
     with torch.no_grad():
         pj.rope_axes(x, pos, (8,))
     pj.rope_axes(x, pos.detach(), (8,))
+
+
+def test_results_written_in_place_are_seen_by_autograd():
+    """A gradient that needs what a call has overwritten is refused: lengths that an acceptance or an eviction advances, as rotary positions,
+    and tensors that take results."""
+    import probjax_b200 as pj
+
+    t = lambda i, *s: normal(500 + i, *s).to(DEV)
+    x, k, v, kn, w = t(0, 2, 1, 2, 8).requires_grad_(True), t(1, 2, 32, 2, 8), t(2, 2, 32, 2, 8), t(3, 2, 3, 2, 8), t(4, 2, 2, 32).abs()
+    n = torch.tensor([9, 20], dtype=torch.int32, device=DEV)
+    lse, q = torch.zeros(2, 2, 1, device=DEV), t(5, 2, 1, 2, 8)
+    calls = [
+        (n, lambda: pj.accept_drafts(kn, kn, k, v, [[0, 1], [2, 0]], [2, 1], kv_lengths=n, out=n)),
+        (n, lambda: pj.evict(k, v, w, n, 10, lengths_out=n)),
+        (k, lambda: pj.evict(k, v, w, n, 10)),
+        (v, lambda: pj.accept_drafts(kn, kn, k, v, [[0], [2]], [1, 1], kv_lengths=n)),
+        (w, lambda: pj.decode_weights(q, k, v, w, out=w)),
+        (w, lambda: pj.key_weights(q, k, lse, weights=w, out=w)),
+        (k, lambda: pj.rope_axes(k, torch.zeros(32, 1, device=DEV), (8,), out=k)),
+    ]
+    for changed, call in calls:
+        y = pj.rope_axes(x, n[:, None, None], (8,))
+        leaf = torch.ones((), device=DEV, requires_grad=True)
+        z = (leaf * changed).sum()  # (needs `changed` for the leaf's gradient)
+        call()
+        if changed is n:
+            with pytest.raises(RuntimeError, match="changed in place"):
+                y.sum().backward()
+        with pytest.raises(RuntimeError, match="inplace"):
+            z.backward()
+    with torch.inference_mode():
+        a, b, m = k.clone(), v.clone(), n.clone()
+        pj.evict(a, b, w.clone(), m, 4, lengths_out=m)
+        assert m.tolist() == [4, 4]
