@@ -345,7 +345,8 @@ int launch_combine(const TreeParams& p, int dtype, cudaStream_t stream) {
 
 inline size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
-// Columns of 16 or 64 rows, two CTAs per SM.
+// Columns of 16 or 64 rows.  Two runs per SM: shared memory holds two CTAs where a call's tiles take up to 113 KB (64 rows of width 96, 16
+// of width 128), otherwise (64 rows of width 128: 119 KB) one, and the runs follow one another.
 void generic_geometry(TreeParams& p) {
   const int rows = p.N * (p.Hq / p.Hkv), tile = generic_rows(rows);
   p.column_rows = rows < tile ? rows : tile;

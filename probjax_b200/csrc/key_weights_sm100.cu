@@ -1,7 +1,7 @@
 // Attention received by every key on the tensor cores: transposed scores S^T = K.Q^T with the keys on the lanes of tensor memory, so
 // that a key's sum over all query rows is one thread's: w_j += sum_r exp2(c q_r.k_j - lse2_r), no exchange between threads.
 //
-// With few rows the call is bound by HBM (K once), from some 160 rows per KV head on by the exponentials (16 per clock and SM).
+// With few rows the call is bound by HBM (K once); at 256 rows per KV head the exponentials (16 per clock and SM) take longer than K.
 // 128 keys a step, the even and the odd steps with groups of threads and two score buffers (128 columns each) of their own, so that the
 // MMAs run ahead of the exponentials; rows (t, g) in chunks of up to 128.  The log-sum-exp of a row is subtracted by the MMAs too: one
 // more step of 16 columns multiplies -lse2 / c, split into three 16-bit numbers (24 bits and more), with a constant; read per column and
@@ -12,20 +12,23 @@
 //   warps 2-17   four groups of 128 threads, two per parity: a key has a thread for the first 64 rows of a chunk and one for the
 //                others (with one thread per key, 2.5 warps per scheduler, the kernel waits for latencies)
 //
-// 8 prompts of 32k keys, 8 KV heads of 128 (537 MB of keys), whole calls by CUDA events, us: 4 rows per KV head 105 (5.1 TB/s),
-// 64 rows 101, 128 rows 110-127 between runs, 256 rows 211 (180 for a prompt's window under its causal mask, 204 among other calls),
-// where the exponentials alone take 131 at 1.73 GHz.  Steps at 256 rows (the kernel in a trace, causal): a thread per key 259, two
-// threads 224, log-sum-exps inside the MMAs 198, sums of the second half added a step later and short loops around the MMAs 183.  A part of the exponentials as a
-// polynomial on the FMA pipe (a quarter, a third, a half) is no faster: 187, 185, 209.
+// 8 prompts of 32k keys, 8 KV heads of 128 (537 MB of keys), whole calls by CUDA events, us: 4 rows per KV head 103 (5.2 TB/s),
+// 64 rows 101, 128 rows 107, 256 rows (a prompt's window under its causal mask) 197-210, 173 inside a graph, where the exponentials alone
+// take 131 at 1.73 GHz.  Steps at 256 rows (the kernel in a trace, causal): a thread per key 259, two threads 224, log-sum-exps inside the
+// MMAs 198, sums of the second half added a step later and short loops around the MMAs 183.  A part of the exponentials as a polynomial on
+// the FMA pipe (a quarter, a third, a half) is no faster (187, 185, 209), so they are not the bound; no unit is full, and the compute warps
+// wait for each load of scores before they start on it.
 //
 // Rows apart: a row without keys (lse = +inf) may hold anything in its query, and NaN plus -inf is NaN; a log-sum-exp whose three parts pass
 // the type (fp16: |lse / scale| from 2.6 * 10^8 on) would come out as infinite.  Where a chunk has such a row, the producer leaves what to
 // add to each of its rows in 32 bits (-inf: the row adds nothing, whatever its score) instead of in the MMA's columns, the issuer hands it
-// to the score buffer, and the compute warps take it from there.  A chunk without them pays for a flag.
+// to the score buffer, and the compute warps take it from there: a load from shared memory per row and key (4, 64, 128 rows with such
+// rows among them: 113, 111, 146 us).  A chunk without them pays for a flag (2 us of the 103).
 //
 // RESIDENT: all rows fit into the stages, stay there while the CTA walks the keys of one (sequence, head), and the key steps of all heads
-// are dealt in contiguous runs, one per CTA (a run may go on into the next sequence or head, whose rows it then loads); otherwise the rows stream past every key step out of L2 and the steps are dealt in turn, which balances a
-// causal mask.  Every wait is bounded as in the other tcgen05 kernels.
+// are dealt in contiguous runs, one per CTA (a run may go on into the next sequence or head, whose rows it then loads; with a CTA bound to
+// a head, 100 heads took 180 us instead of 134); otherwise the rows stream past every key step out of L2 and the steps are dealt in turn,
+// which balances a causal mask.  Every wait is bounded as in the other tcgen05 kernels.
 #include <type_traits>
 
 #include "sm100_softmax.cuh"

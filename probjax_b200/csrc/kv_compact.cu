@@ -7,7 +7,8 @@
 //
 // Measured on a cache of 16 ragged sequences of 4k-32k keys, 8 heads of 128, bf16, cut to 8192 keys: the call 213 us; in
 // a trace selection 36 (259 with the weights read again in every pass, 11-bit digits and clusters), movement 177 = 5.8 TB/s of rows
-// read and written.  One sequence of 4001 keys cut to 1024: 11 and 6 us on the device, the call 20.
+// read and written.  One sequence of 4001 keys cut to 1024: 11 and 6 us on the device, the call 20.  In place 190 and 26-28 us: rows that stay
+// are not moved, but a head of one sequence has a CTA per 128 bytes of its rows only.
 //
 // No counterpart in the reference, whose cache only grows (probjax/nn/layers/attention.py:631-643).
 #include <cooperative_groups.h>

@@ -2,10 +2,12 @@
 // every token of every sequence: pair (a, b) of a head vector becomes (a cos - b sin, b cos + a sin) of the angle
 // positions[b, t, axis(pair)] * frequency(pair).  The gradient is the rotation by the negative angle, the same kernel.
 //
-// Bound by HBM: the tensor is read once and written once, 16 bytes per access.  A CTA takes a few tokens.  Its threads issue
+// The floor is HBM's: the tensor is read once and written once, 16 bytes per access.  A CTA takes a few tokens.  Its threads issue
 // their first loads, compute the tokens' cosines and sines meanwhile, one angle each, into shared memory, and the H heads of
 // the tokens share them.  The angle is taken in turns in 64 bits (a position of 10^6 times a frequency near 1 would lose five digits in 32)
 // and reduced to half a turn before it is rounded: two 64-bit operations per (token, pair), nothing next to the traffic.
+//
+// It is not reached (4.6 of 6.55 TB/s): a CTA loads once, forms its angles, synchronises and stores, with nothing of further tokens in flight.
 //
 // Measured: 4 x 4096 tokens of 32 heads of 128 in bf16, three axes, queries out of a fused projection: 58 us = 4.6 TB/s (65 with the
 // loads behind the angles and a 64-bit division per access; 64 and 61 with 128 and 512 angles a CTA), the kernel in a trace; forward and
